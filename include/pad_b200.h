@@ -54,6 +54,7 @@ typedef enum pad_status {
  * the device without a host sync). */
 #define PAD_FLAG_BAD_PAGE_ID 0x1     /* a block_table entry outside [0, num_pages) */
 #define PAD_FLAG_SEQ_LEN_RANGE 0x2   /* seq_len < 0 or > max_pages_per_seq * page_size */
+#define PAD_FLAG_BAD_SEQ_ID 0x4      /* a seq_ids entry outside [0, batch) */
 #define PAD_FLAG_WAIT_TIMEOUT 0x100  /* an in-kernel wait gave up (never expected) */
 
 /* Human-readable text for a status code (static storage). */
@@ -193,6 +194,87 @@ int pad_paged_attention_decode_noalloc(const void* q, const void* k_cache, const
                                        int64_t block_table_stride, const int64_t* out_strides,
                                        float scale, int64_t num_splits, void* stream,
                                        int32_t* error_flags);
+
+/* ---------------------------------------------------------------------------
+ * The 4-bit cache. A token's row of one KV head is head_dim/2 code bytes and
+ * 4 scale bytes, for K and for V (head_dim 32, 64 or 128):
+ *   k/v_cache    [num_pages, page_size, num_kv_heads, head_dim / 2]  uint8
+ *   k/v_scales   [num_pages, page_size, num_kv_heads, 4]             uint8
+ * Code byte i holds dims 2i (low nibble) and 2i + 1 as e2m1 (0 0.5 1 1.5 2 3 4
+ * 6 and their negatives); scale byte j is the power of two 2^(byte - 127) of
+ * dims [32j, 32j + 32), 255 meaning NaN. Scale bytes past head_dim / 32 are
+ * written as 0 and never read. Codes must be 16-byte aligned with strides that
+ * are multiples of 16 bytes, scales 4-byte aligned with strides that are
+ * multiples of 4; last axes contiguous. Strides of uint8 tensors are bytes.
+ *
+ * pad_paged_kv_append_fp4 quantises and writes `tokens` new rows: row t of
+ * k_new / v_new [tokens, num_kv_heads, head_dim] fp16 becomes token
+ * positions[t] of sequence seq_ids[t] (seq_ids NULL: of sequence t, and tokens
+ * <= batch). Per block of 32 with a = max |x|: E = max(floor(log2 a) - 2, -24),
+ * scale byte E + 127, codes round(x / 2^E) to nearest even, saturated at 6. A
+ * block with an Inf or NaN gets scale 255 and zero codes. positions[t] < 0
+ * skips t. A position past the block table sets PAD_FLAG_SEQ_LEN_RANGE, a bad
+ * page id PAD_FLAG_BAD_PAGE_ID, a seq_ids entry outside [0, batch)
+ * PAD_FLAG_BAD_SEQ_ID; nothing is written for that token. One call must not
+ * name the same (sequence, position) twice.
+ *
+ * pad_paged_kv_read_fp4 gives the rows back as fp16 [tokens, num_kv_heads,
+ * head_dim] (exactly what the codes of an appended row stand for); a token
+ * that is skipped or flagged reads as zeros. No counterpart in the reference. */
+int pad_paged_kv_append_fp4(const void* k_new, const void* v_new, void* k_cache, void* k_scales, void* v_cache,
+                            void* v_scales, const int32_t* block_table, const int32_t* positions,
+                            const int32_t* seq_ids, int64_t tokens, int64_t batch, int64_t num_kv_heads,
+                            int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages_per_seq,
+                            const int64_t* k_new_strides, const int64_t* v_new_strides, const int64_t* k_strides,
+                            const int64_t* ks_strides, const int64_t* v_strides, const int64_t* vs_strides,
+                            int64_t block_table_stride, void* stream, int32_t* error_flags);
+int pad_paged_kv_read_fp4(const void* k_cache, const void* k_scales, const void* v_cache, const void* v_scales,
+                          const int32_t* block_table, const int32_t* positions, const int32_t* seq_ids, void* k_out,
+                          void* v_out, int64_t tokens, int64_t batch, int64_t num_kv_heads, int64_t head_dim,
+                          int64_t num_pages, int64_t page_size, int64_t max_pages_per_seq, const int64_t* k_strides,
+                          const int64_t* ks_strides, const int64_t* v_strides, const int64_t* vs_strides,
+                          const int64_t* k_out_strides, const int64_t* v_out_strides, int64_t block_table_stride,
+                          void* stream, int32_t* error_flags);
+
+/* ---------------------------------------------------------------------------
+ * Eviction by accumulated attention weight. Beside a paged cache live
+ *   weights         [num_pages, num_kv_heads, page_size]  fp32
+ *   slot_positions  [num_pages, num_kv_heads, page_size]  int32 (optional)
+ * addressed through the same block table: what a slot's token has received, and
+ * the token's position in its sequence (after an eviction a slot no longer
+ * tells it). Any strides (in elements). A page belongs to one sequence.
+ *
+ * pad_paged_kv_evict_plan chooses, for every sequence b with seq_lens[b] >
+ * budget and every KV head, the `budget` slots to keep: first those that are
+ * recent (slot_positions >= total_lens[b] - recent), then by weight descending
+ * (NaN above all), ties to the lower slot. Kept slots at or above `budget` move
+ * to the slots below it that are not kept:
+ *   src, dst  [batch, num_kv_heads, max_moves] int32, both ascending, -1 behind
+ *             the last move; max_moves = pad_evict_max_moves(...)
+ *   counts    [batch, num_kv_heads] int32, moves of each
+ *   new_lens  [batch] int32, min(seq_lens, budget)
+ * recent > 0 needs slot_positions and total_lens ([batch] int32, tokens each
+ * sequence has seen). Nothing of the cache is touched.
+ *
+ * pad_paged_kv_move copies row src -> row dst of 1 to 4 caches [num_pages,
+ * page_size, num_kv_heads, row] (row_bytes[c] contiguous bytes; cache_strides
+ * [num_caches][3]: page, row and head strides in BYTES), of weights and of
+ * slot_positions (each optional). Within one (sequence, KV head) no dst may be
+ * a src or occur twice, as in a plan. Entries outside the block table set
+ * PAD_FLAG_SEQ_LEN_RANGE and are skipped. No counterpart in the reference. */
+int pad_evict_max_moves(int64_t budget, int64_t page_size, int64_t max_pages_per_seq, int64_t* max_moves);
+int pad_paged_kv_evict_plan(const float* weights, const int32_t* slot_positions, const int32_t* block_table,
+                            const int32_t* seq_lens, const int32_t* total_lens, int32_t* src, int32_t* dst,
+                            int32_t* counts, int32_t* new_lens, int64_t batch, int64_t num_kv_heads,
+                            int64_t num_pages, int64_t page_size, int64_t max_pages_per_seq, int64_t budget,
+                            int64_t recent, const int64_t* weight_strides, const int64_t* position_strides,
+                            int64_t block_table_stride, void* stream, int32_t* error_flags);
+int pad_paged_kv_move(int64_t num_caches, void* const* caches, const int64_t* row_bytes, const int64_t* cache_strides,
+                      const int32_t* block_table, const int32_t* src, const int32_t* dst, const int32_t* counts,
+                      float* weights, int32_t* slot_positions, int64_t batch, int64_t num_kv_heads, int64_t num_pages,
+                      int64_t page_size, int64_t max_pages_per_seq, int64_t max_moves, const int64_t* weight_strides,
+                      const int64_t* position_strides, int64_t block_table_stride, void* stream,
+                      int32_t* error_flags);
 
 #ifdef __cplusplus
 }

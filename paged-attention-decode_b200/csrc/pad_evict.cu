@@ -1,0 +1,526 @@
+// pad_evict.cu -- eviction from a paged cache by accumulated attention weight:
+// which slots survive (plan) and the copies that make them the first ones
+// (move). No counterpart in the reference.
+//
+// Plan, for one (sequence, KV head) of L > budget slots: rank the slots by
+//   (recent first, then weight descending with NaN above all, then slot
+//   ascending)
+// and keep the first `budget`. Holes are slots below `budget` that are not
+// kept, movers are kept slots at or above it; there are equally many, and
+// mover i (ascending) goes to hole i (ascending). Attention does not depend on
+// the order of the slots, so nothing else has to move, and since sources lie
+// at or above `budget` and targets below it, no row is both: the copies are
+// free to run in any order.
+//
+// The ranking is a radix selection on an order-preserving 32-bit key, three
+// digits of 11, 11 and 10 bits from the top, which leaves the key T of the
+// budget-th slot and how many slots equal to T are kept (those of the lowest
+// slots). Weights and positions are read once into shared memory; a pair whose
+// slots fill more than one SM's share is spread over a cluster of up to 8 CTAs
+// that add up their histograms through distributed shared memory.
+//
+// Bound: plan -- HBM bytes for many long sequences (8 bytes a slot), else the
+// latency of its dependent steps (gather, three histogram passes, two scans);
+// move -- HBM bytes, 2 x row bytes a move.
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cstdint>
+
+#include "pad_b200.h"
+#include "pad_error.cuh"
+
+namespace {
+
+namespace cg = cooperative_groups;
+using pad::cuda_fail;
+using pad::fail;
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kMaxCluster = 8;
+constexpr uint32_t kRecentKey = 0xffffffffu, kNanKey = 0xfffffffeu;
+
+struct PlanParams {
+  const float* weights;
+  const int32_t *slot_positions, *block_table, *seq_lens, *total_lens;
+  int32_t *src, *dst, *counts, *new_lens;
+  int64_t w0, w1, w2, p0, p1, p2;  // element strides of weights and slot_positions [page][head][row]
+  int64_t bt_stride;
+  int hkv, num_pages, page_size, page_shift, max_pages, budget, recent, max_moves;
+  int key_cap;  // keys of shared memory per CTA
+  int32_t* error_flags;
+};
+
+// Weight -> key whose unsigned order is the ranking (-0 and +0 are equal).
+__device__ __forceinline__ uint32_t weight_key(float w) {
+  if (w != w) return kNanKey;
+  const uint32_t b = __float_as_uint(w + 0.f);  // -0 + 0 = +0
+  return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+
+struct PlanShared {
+  int hist[3][kBins];
+  int scan[kPlanWarps];
+  int bin, above;         // the digit found in a pass, and the keys above it
+  int eq, movers, holes;  // this CTA's counts, read by the cluster
+};
+
+struct SlotKeys {
+  const PlanParams& p;
+  const uint32_t* cached;
+  int64_t bt_row;
+  int b, h, first;
+  int64_t oldest_recent;  // slots whose position is at least this are recent
+  __device__ __forceinline__ uint32_t load(int slot, bool report) const {
+    const int lp = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
+    const int64_t row = slot - (int64_t)lp * p.page_size;
+    const int page = __ldg(p.block_table + bt_row + lp);
+    if ((unsigned)page >= (unsigned)p.num_pages) {
+      if (report && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_BAD_PAGE_ID);
+      return 0u;
+    }
+    if (p.slot_positions != nullptr &&
+        (int64_t)__ldg(p.slot_positions + page * p.p0 + h * p.p1 + row * p.p2) >= oldest_recent)
+      return kRecentKey;
+    return weight_key(__ldg(p.weights + page * p.w0 + h * p.w1 + row * p.w2));
+  }
+  // Slots past the shared-memory share are read again wherever they are needed.
+  __device__ __forceinline__ uint32_t at(int slot) const {
+    const int i = slot - first;
+    return i < p.key_cap ? cached[i] : load(slot, false);
+  }
+};
+
+// Largest bin d with (keys in bins above d) < need, searched by the whole
+// block; `get(bin)` is the bin's count over the cluster. Sets sh.bin and
+// sh.above.
+template <class Get>
+__device__ void find_bin(PlanShared& sh, int need, Get get) {
+  constexpr int PER = kBins / kPlanThreads;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int c[PER], sum = 0;
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {  // thread t holds bins from the top
+    c[i] = get(kBins - 1 - (tid * PER + i));
+    sum += c[i];
+  }
+  int incl = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  if (lane == 31) sh.scan[warp] = incl;
+  __syncthreads();
+  int above = incl - sum;
+  for (int x = 0; x < warp; ++x) above += sh.scan[x];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    if (above < need && need <= above + c[i]) {
+      sh.bin = kBins - 1 - (tid * PER + i);
+      sh.above = above;
+    }
+    above += c[i];
+  }
+  __syncthreads();
+}
+
+// Exclusive sum over the block's warps of a per-warp count; *total its sum.
+__device__ __forceinline__ int warp_base(PlanShared& sh, int mine, int* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  __syncthreads();
+  if (lane == 0) sh.scan[warp] = mine;
+  __syncthreads();
+  int v = sh.scan[lane], incl = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += y;
+  }
+  *total = __shfl_sync(0xffffffffu, incl, 31);
+  return __shfl_sync(0xffffffffu, incl - v, warp);
+}
+
+__global__ void __launch_bounds__(kPlanThreads, 1) evict_plan_kernel(const __grid_constant__ PlanParams p) {
+  extern __shared__ uint32_t keys[];
+  __shared__ PlanShared sh;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int pair = (int)(blockIdx.x / ranks), b = pair / p.hkv, h = pair % p.hkv;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t cap = (int64_t)p.max_pages * p.page_size;
+  const int raw = __ldg(p.seq_lens + b);
+  const int n = (int)min((int64_t)max(raw, 0), cap);
+  if ((raw < 0 || raw > cap) && tid == 0 && rank == 0 && p.error_flags != nullptr)
+    atomicOr(p.error_flags, PAD_FLAG_SEQ_LEN_RANGE);
+  if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = min(n, p.budget);
+  int32_t* src = p.src + (int64_t)pair * p.max_moves;
+  int32_t* dst = p.dst + (int64_t)pair * p.max_moves;
+  int count = 0;
+  if (n > p.budget) {
+    // this CTA's slots, whole warps' worth of them
+    const int share = (n + ranks - 1) / ranks;
+    const int first = min(n, rank * share), last = min(n, first + share);
+    SlotKeys key{p, keys, (int64_t)b * p.bt_stride, b, h, first,
+                 p.slot_positions != nullptr ? (int64_t)__ldg(p.total_lens + b) - p.recent : 0};
+    for (int x = tid; x < 3 * kBins; x += kPlanThreads) (&sh.hist[0][0])[x] = 0;
+    __syncthreads();
+    for (int s = first + tid; s < last; s += kPlanThreads) {
+      const uint32_t k = key.load(s, true);
+      if (s - first < p.key_cap) keys[s - first] = k;
+      atomicAdd(&sh.hist[0][k >> 21], 1);
+    }
+    uint32_t prefix = 0;
+    int need = p.budget;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      if (pass > 0) {
+        for (int s = first + tid; s < last; s += kPlanThreads) {
+          const uint32_t k = key.at(s);
+          if (pass == 1 ? (k >> 21) == prefix : (k >> 10) == prefix)
+            atomicAdd(&sh.hist[pass][pass == 1 ? (k >> 10) & 2047u : k & 1023u], 1);
+        }
+      }
+      cluster.sync();
+      find_bin(sh, need, [&](int bin) {
+        int c = 0;
+        for (int r = 0; r < ranks; ++r) c += cluster.map_shared_rank(&sh, r)->hist[pass][bin];
+        return c;
+      });
+      need -= sh.above;
+      prefix = pass == 0 ? (uint32_t)sh.bin : (prefix << (pass == 1 ? 11 : 10)) | (uint32_t)sh.bin;
+    }
+    // prefix is the key of the budget-th slot; `need` slots equal to it are kept
+    const uint32_t T = prefix;
+    // each warp walks a contiguous run of the CTA's slots
+    const int per = ((last - first + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
+    const int lo = min(last, first + warp * per), hi = min(last, lo + per);
+    int eq = 0, total;
+    for (int s = lo + lane; s - lane < hi; s += 32) eq += __popc(__ballot_sync(0xffffffffu, s < hi && key.at(s) == T));
+    int eq_base = warp_base(sh, eq, &total);
+    for (int r = 0; r < rank; ++r) eq_base += cluster.map_shared_rank(&sh, r)->hist[2][T & 1023u];
+    const uint32_t below = (1u << lane) - 1u;
+    // which of 32 slots are kept, and the running number of equals before them
+    auto kept = [&](int s, int& seen) {
+      const uint32_t k = s < hi ? key.at(s) : 0u;
+      const uint32_t e = __ballot_sync(0xffffffffu, s < hi && k == T);
+      const bool on = s < hi && (k > T || (k == T && seen + __popc(e & below) < need));
+      seen += __popc(e);
+      return on;
+    };
+    int holes = 0, movers = 0, seen = eq_base;
+    for (int s = lo + lane; s - lane < hi; s += 32) {
+      const bool on = kept(s, seen);
+      movers += __popc(__ballot_sync(0xffffffffu, on && s >= p.budget));
+      holes += __popc(__ballot_sync(0xffffffffu, s < hi && !on && s < p.budget));
+    }
+    int hole_at = warp_base(sh, holes, &total);
+    if (tid == 0) sh.holes = total;
+    int mover_at = warp_base(sh, movers, &total);
+    if (tid == 0) sh.movers = total;
+    cluster.sync();
+    for (int r = 0; r < ranks; ++r) {
+      const PlanShared* o = cluster.map_shared_rank(&sh, r);
+      if (r < rank) {
+        hole_at += o->holes;
+        mover_at += o->movers;
+      }
+      count += o->movers;
+    }
+    seen = eq_base;
+    for (int s = lo + lane; s - lane < hi; s += 32) {
+      const bool on = kept(s, seen);
+      const uint32_t m = __ballot_sync(0xffffffffu, on && s >= p.budget);
+      const uint32_t o = __ballot_sync(0xffffffffu, s < hi && !on && s < p.budget);
+      // (never past max_moves unless the inputs change while the kernel runs)
+      const int mi = mover_at + __popc(m & below), oi = hole_at + __popc(o & below);
+      if (((m >> lane) & 1u) && mi < p.max_moves) src[mi] = s;
+      if (((o >> lane) & 1u) && oi < p.max_moves) dst[oi] = s;
+      mover_at += __popc(m);
+      hole_at += __popc(o);
+    }
+    cluster.sync();  // no CTA leaves while another may read its shared memory
+  }
+  if (tid == 0 && rank == 0) p.counts[pair] = count;
+  for (int x = count + rank * kPlanThreads + tid; x < p.max_moves; x += ranks * kPlanThreads) {
+    src[x] = -1;
+    dst[x] = -1;
+  }
+}
+
+// ----------------------------------------------------------------------------- move
+constexpr int kMoveThreads = 256;
+constexpr int kMaxCaches = 4;
+constexpr int kMoveGrid = 148 * 8;  // every SM full; larger lists loop
+
+struct MoveParams {
+  uint8_t* cache[kMaxCaches];
+  int64_t s0[kMaxCaches], s1[kMaxCaches], s2[kMaxCaches];  // page, row and head strides in bytes
+  int chunks[kMaxCaches], unit_log2[kMaxCaches];           // a row is `chunks` pieces of 2^unit_log2 bytes
+  float* weights;
+  int32_t* slot_positions;
+  const int32_t *block_table, *src, *dst, *counts;
+  int64_t w0, w1, w2, p0, p1, p2, bt_stride;
+  int64_t items;  // (pair, run of moves) pieces of work
+  int hkv, num_pages, page_size, page_shift, max_pages, max_moves, runs;
+  int32_t* error_flags;
+};
+
+__device__ __forceinline__ uint4 load_piece(const uint8_t* x, int unit_log2) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (unit_log2 == 4) v = *reinterpret_cast<const uint4*>(x);
+  else if (unit_log2 == 2) v.x = *reinterpret_cast<const uint32_t*>(x);
+  else if (unit_log2 == 1) v.x = *reinterpret_cast<const uint16_t*>(x);
+  else v.x = *x;
+  return v;
+}
+__device__ __forceinline__ void store_piece(uint8_t* x, const uint4& v, int unit_log2) {
+  if (unit_log2 == 4) *reinterpret_cast<uint4*>(x) = v;
+  else if (unit_log2 == 2) *reinterpret_cast<uint32_t*>(x) = v.x;
+  else if (unit_log2 == 1) *reinterpret_cast<uint16_t*>(x) = (uint16_t)v.x;
+  else *x = (uint8_t)v.x;
+}
+
+// LPM lanes copy one row of every cache (and its weight and position); all
+// loads of a move are issued before its stores.
+template <int LPM>
+__global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_constant__ MoveParams p) {
+  constexpr int MPB = kMoveThreads / LPM;
+  const int m = threadIdx.x / LPM, l = threadIdx.x % LPM;
+  for (int64_t it = blockIdx.x; it < p.items; it += gridDim.x) {
+    const int pair = (int)(it / p.runs);
+    const int i = (int)(it - (int64_t)pair * p.runs) * MPB + m;
+    if (i >= min(__ldg(p.counts + pair), p.max_moves)) continue;
+    const int b = pair / p.hkv, h = pair % p.hkv;
+    const int ss = __ldg(p.src + (int64_t)pair * p.max_moves + i), ds = __ldg(p.dst + (int64_t)pair * p.max_moves + i);
+    const int64_t cap = (int64_t)p.max_pages * p.page_size;
+    if (ss < 0 || ds < 0 || ss >= cap || ds >= cap) {
+      if (l == 0 && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_SEQ_LEN_RANGE);
+      continue;
+    }
+    const int slp = p.page_shift >= 0 ? ss >> p.page_shift : ss / p.page_size;
+    const int dlp = p.page_shift >= 0 ? ds >> p.page_shift : ds / p.page_size;
+    const int64_t sp = __ldg(p.block_table + b * p.bt_stride + slp), dp = __ldg(p.block_table + b * p.bt_stride + dlp);
+    if (sp < 0 || dp < 0 || sp >= p.num_pages || dp >= p.num_pages) {
+      if (l == 0 && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_BAD_PAGE_ID);
+      continue;
+    }
+    const int64_t sr = ss - (int64_t)slp * p.page_size, dr = ds - (int64_t)dlp * p.page_size;
+    uint4 v[kMaxCaches];
+    float w = 0.f;
+    int32_t at = 0;
+#pragma unroll
+    for (int c = 0; c < kMaxCaches; ++c)
+      if (l < p.chunks[c])
+        v[c] = load_piece(p.cache[c] + sp * p.s0[c] + sr * p.s1[c] + h * p.s2[c] + ((int64_t)l << p.unit_log2[c]),
+                          p.unit_log2[c]);
+    if (l == 0 && p.weights != nullptr) w = p.weights[sp * p.w0 + h * p.w1 + sr * p.w2];
+    if (l == LPM - 1 && p.slot_positions != nullptr) at = p.slot_positions[sp * p.p0 + h * p.p1 + sr * p.p2];
+#pragma unroll
+    for (int c = 0; c < kMaxCaches; ++c) {
+      const int64_t from = sp * p.s0[c] + sr * p.s1[c] + h * p.s2[c], to = dp * p.s0[c] + dr * p.s1[c] + h * p.s2[c];
+      if (l < p.chunks[c]) store_piece(p.cache[c] + to + ((int64_t)l << p.unit_log2[c]), v[c], p.unit_log2[c]);
+      for (int x = l + LPM; x < p.chunks[c]; x += LPM)
+        store_piece(p.cache[c] + to + ((int64_t)x << p.unit_log2[c]),
+                    load_piece(p.cache[c] + from + ((int64_t)x << p.unit_log2[c]), p.unit_log2[c]), p.unit_log2[c]);
+    }
+    if (l == 0 && p.weights != nullptr) p.weights[dp * p.w0 + h * p.w1 + dr * p.w2] = w;
+    if (l == LPM - 1 && p.slot_positions != nullptr) p.slot_positions[dp * p.p0 + h * p.p1 + dr * p.p2] = at;
+  }
+}
+
+int shift_of(int64_t page_size) {
+  return (page_size & (page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)page_size) : -1;
+}
+
+int check_common(const char* what, int64_t batch, int64_t num_kv_heads, int64_t num_pages, int64_t page_size,
+                 int64_t max_pages, int64_t bt_stride) {
+  if (batch < 0 || num_kv_heads <= 0 || num_pages < 0 || page_size <= 0 || max_pages < 0)
+    return fail(PAD_ERR_INVALID_ARGUMENT, "%s: negative or zero size", what);
+  if (bt_stride < max_pages)
+    return fail(PAD_ERR_INVALID_ARGUMENT, "%s: block_table row stride smaller than its width", what);
+  if (num_pages > INT32_MAX || page_size > INT32_MAX || max_pages > INT32_MAX ||
+      max_pages * page_size > INT32_MAX / 2 || batch > INT32_MAX / num_kv_heads / kMaxCluster)
+    return fail(PAD_ERR_UNSUPPORTED, "%s: sizes exceed 32-bit indexing", what);
+  return PAD_OK;
+}
+
+constexpr int kMaxDevices = 64;
+
+// Keys of shared memory a plan CTA may hold beside its static part.
+constexpr int kKeyCapMax = (227 * 1024 - (int)sizeof(PlanShared) - 1024) / 4 / 256 * 256;
+
+}  // namespace
+
+extern "C" int pad_evict_max_moves(int64_t budget, int64_t page_size, int64_t max_pages_per_seq, int64_t* max_moves) {
+  if (max_moves == nullptr) return fail(PAD_ERR_INVALID_ARGUMENT, "evict_plan: null output pointer");
+  if (budget < 1 || page_size <= 0 || max_pages_per_seq < 0 || (max_pages_per_seq > 0 && page_size > INT64_MAX / max_pages_per_seq))
+    return fail(PAD_ERR_INVALID_ARGUMENT, "evict_plan: budget and page_size must be positive");
+  *max_moves = std::max<int64_t>(0, std::min(budget, max_pages_per_seq * page_size - budget));
+  return PAD_OK;
+}
+
+extern "C" int pad_paged_kv_evict_plan(const float* weights, const int32_t* slot_positions, const int32_t* block_table,
+                                       const int32_t* seq_lens, const int32_t* total_lens, int32_t* src, int32_t* dst,
+                                       int32_t* counts, int32_t* new_lens, int64_t batch, int64_t num_kv_heads,
+                                       int64_t num_pages, int64_t page_size, int64_t max_pages_per_seq, int64_t budget,
+                                       int64_t recent, const int64_t* weight_strides, const int64_t* position_strides,
+                                       int64_t block_table_stride, void* stream, int32_t* error_flags) {
+  int st = check_common("evict_plan", batch, num_kv_heads, num_pages, page_size, max_pages_per_seq, block_table_stride);
+  if (st != PAD_OK) return st;
+  if (budget < 1) return fail(PAD_ERR_INVALID_ARGUMENT, "evict_plan: budget must be at least 1");
+  if (recent < 0 || recent > budget)
+    return fail(PAD_ERR_INVALID_ARGUMENT, "evict_plan: recent must lie in [0, budget]");
+  if (recent > 0 && slot_positions == nullptr)
+    return fail(PAD_ERR_INVALID_ARGUMENT, "evict_plan: recent needs slot_positions");
+  if (batch == 0) return PAD_OK;
+  int64_t moves = 0;
+  if ((st = pad_evict_max_moves(budget, page_size, max_pages_per_seq, &moves)) != PAD_OK) return st;
+  if (seq_lens == nullptr || counts == nullptr || new_lens == nullptr ||
+      (moves > 0 && (weights == nullptr || block_table == nullptr || src == nullptr || dst == nullptr ||
+                     weight_strides == nullptr)) ||
+      (slot_positions != nullptr && (total_lens == nullptr || position_strides == nullptr)))
+    return fail(PAD_ERR_INVALID_ARGUMENT, "evict_plan: null pointer argument");
+  const int64_t cap = max_pages_per_seq * page_size, pairs = batch * num_kv_heads;
+  PlanParams p = {};
+  p.weights = weights;
+  // without a recent window the positions decide nothing
+  p.slot_positions = recent > 0 ? slot_positions : nullptr;
+  p.block_table = block_table;
+  p.seq_lens = seq_lens;
+  p.total_lens = total_lens;
+  p.src = src;
+  p.dst = dst;
+  p.counts = counts;
+  p.new_lens = new_lens;
+  if (weight_strides != nullptr) {
+    p.w0 = weight_strides[0];
+    p.w1 = weight_strides[1];
+    p.w2 = weight_strides[2];
+  }
+  if (p.slot_positions != nullptr) {
+    p.p0 = position_strides[0];
+    p.p1 = position_strides[1];
+    p.p2 = position_strides[2];
+  }
+  p.bt_stride = block_table_stride;
+  p.hkv = (int)num_kv_heads;
+  p.num_pages = (int)num_pages;
+  p.page_size = (int)page_size;
+  p.page_shift = shift_of(page_size);
+  p.max_pages = (int)max_pages_per_seq;
+  p.budget = (int)std::min<int64_t>(budget, INT32_MAX);
+  p.recent = (int)std::min<int64_t>(recent, INT32_MAX);
+  p.max_moves = (int)moves;
+  p.error_flags = error_flags;
+  // a CTA per 8192 slots of a sequence, up to a cluster of 8
+  int ranks = 1;
+  while (ranks < kMaxCluster && cap > (int64_t)ranks * 8192) ranks *= 2;
+  const int64_t share = (cap + ranks - 1) / ranks;
+  p.key_cap = (int)std::min<int64_t>(kKeyCapMax, (share + 255) / 256 * 256);
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  if (device < 0 || device >= kMaxDevices) return fail(PAD_ERR_INVALID_ARGUMENT, "device %d out of range", device);
+  static std::atomic<bool> smem_set[kMaxDevices];  // set twice by racing threads at worst
+  if (!smem_set[device].load()) {
+    e = cudaFuncSetAttribute(evict_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeyCapMax * 4);
+    if (e != cudaSuccess) return cuda_fail(e, "configuring the evict_plan kernel");
+    smem_set[device].store(true);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(pairs * ranks));
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.dynamicSmemBytes = (size_t)p.key_cap * 4;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  void* args[] = {&p};
+  e = cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(&evict_plan_kernel), args);
+  return e == cudaSuccess ? PAD_OK : cuda_fail(e, "launching the evict_plan kernel");
+}
+
+extern "C" int pad_paged_kv_move(int64_t num_caches, void* const* caches, const int64_t* row_bytes,
+                                 const int64_t* cache_strides, const int32_t* block_table, const int32_t* src,
+                                 const int32_t* dst, const int32_t* counts, float* weights, int32_t* slot_positions,
+                                 int64_t batch, int64_t num_kv_heads, int64_t num_pages, int64_t page_size,
+                                 int64_t max_pages_per_seq, int64_t max_moves, const int64_t* weight_strides,
+                                 const int64_t* position_strides, int64_t block_table_stride, void* stream,
+                                 int32_t* error_flags) {
+  int st = check_common("kv_move", batch, num_kv_heads, num_pages, page_size, max_pages_per_seq, block_table_stride);
+  if (st != PAD_OK) return st;
+  if (num_caches < 1 || num_caches > kMaxCaches)
+    return fail(PAD_ERR_INVALID_ARGUMENT, "kv_move: 1 to %d caches, not %lld", kMaxCaches, (long long)num_caches);
+  if (max_moves < 0) return fail(PAD_ERR_INVALID_ARGUMENT, "kv_move: negative or zero size");
+  if (max_moves > INT32_MAX) return fail(PAD_ERR_UNSUPPORTED, "kv_move: max_moves exceeds int32");
+  if (batch == 0 || max_moves == 0 || num_pages == 0) return PAD_OK;
+  if (caches == nullptr || row_bytes == nullptr || cache_strides == nullptr || block_table == nullptr ||
+      src == nullptr || dst == nullptr || counts == nullptr || (weights != nullptr && weight_strides == nullptr) ||
+      (slot_positions != nullptr && position_strides == nullptr))
+    return fail(PAD_ERR_INVALID_ARGUMENT, "kv_move: null pointer argument");
+  MoveParams p = {};
+  int most = 1;
+  for (int c = 0; c < num_caches; ++c) {
+    if (caches[c] == nullptr) return fail(PAD_ERR_INVALID_ARGUMENT, "kv_move: null pointer argument");
+    if (row_bytes[c] <= 0 || row_bytes[c] > INT32_MAX)
+      return fail(PAD_ERR_INVALID_ARGUMENT, "kv_move: row of %lld bytes", (long long)row_bytes[c]);
+    const int64_t* s = cache_strides + 3 * c;
+    // the widest of 16, 4, 2 and 1 bytes that address and strides allow
+    const uint64_t all = (uint64_t)reinterpret_cast<uintptr_t>(caches[c]) | (uint64_t)row_bytes[c] | (uint64_t)s[0] |
+                         (uint64_t)s[1] | (uint64_t)s[2];
+    p.unit_log2[c] = all % 16 == 0 ? 4 : all % 4 == 0 ? 2 : all % 2 == 0 ? 1 : 0;
+    p.cache[c] = static_cast<uint8_t*>(caches[c]);
+    p.s0[c] = s[0];
+    p.s1[c] = s[1];
+    p.s2[c] = s[2];
+    p.chunks[c] = (int)(row_bytes[c] >> p.unit_log2[c]);
+    most = std::max(most, p.chunks[c]);
+  }
+  p.weights = weights;
+  p.slot_positions = slot_positions;
+  p.block_table = block_table;
+  p.src = src;
+  p.dst = dst;
+  p.counts = counts;
+  if (weights != nullptr) {
+    p.w0 = weight_strides[0];
+    p.w1 = weight_strides[1];
+    p.w2 = weight_strides[2];
+  }
+  if (slot_positions != nullptr) {
+    p.p0 = position_strides[0];
+    p.p1 = position_strides[1];
+    p.p2 = position_strides[2];
+  }
+  p.bt_stride = block_table_stride;
+  p.hkv = (int)num_kv_heads;
+  p.num_pages = (int)num_pages;
+  p.page_size = (int)page_size;
+  p.page_shift = shift_of(page_size);
+  p.max_pages = (int)max_pages_per_seq;
+  p.max_moves = (int)max_moves;
+  p.error_flags = error_flags;
+  // lanes per move: enough for the widest row's pieces, 16 at most (a 256-byte
+  // row's 16 pieces; longer rows loop)
+  const int lpm = most <= 4 ? 4 : most <= 8 ? 8 : 16;
+  const int mpb = kMoveThreads / lpm;
+  p.runs = (int)((max_moves + mpb - 1) / mpb);
+  p.items = batch * num_kv_heads * (int64_t)p.runs;
+  const unsigned grid = (unsigned)std::min<int64_t>(p.items, kMoveGrid);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (lpm == 4) kv_move_kernel<4><<<grid, kMoveThreads, 0, s>>>(p);
+  else if (lpm == 8) kv_move_kernel<8><<<grid, kMoveThreads, 0, s>>>(p);
+  else kv_move_kernel<16><<<grid, kMoveThreads, 0, s>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? PAD_OK : cuda_fail(e, "launching the kv_move kernel");
+}

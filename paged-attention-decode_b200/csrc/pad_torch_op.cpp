@@ -14,8 +14,10 @@
 #include <torch/library.h>
 
 #include <cstdint>
+#include <initializer_list>
 #include <map>
 #include <mutex>
+#include <tuple>
 #include <utility>
 
 #include "pad_b200.h"
@@ -174,6 +176,173 @@ void kv_append(const at::Tensor& k_new_in, const at::Tensor& v_new_in, const at:
         "kv_append");
 }
 
+struct Strides {  // of a tensor's first axes, as the C entry points take them
+  int64_t s[4] = {0, 0, 0, 0};
+  explicit Strides(const at::Tensor& t) {
+    for (int64_t i = 0; i < t.dim() && i < 4; ++i) s[i] = t.stride(i);
+  }
+};
+
+void check_on(const at::Device& dev, std::initializer_list<const at::Tensor*> all, const char* what) {
+  for (const at::Tensor* t : all)
+    TORCH_CHECK(t->device() == dev, "libpad_b200 ", what, ": every tensor must be on ", dev.str());
+}
+
+// The 4-bit caches of one call: codes [P, page, Hkv, D/2], scales [P, page, Hkv, 4].
+void check_fp4(const at::Tensor& k, const at::Tensor& ks, const at::Tensor& v, const at::Tensor& vs, const char* what) {
+  TORCH_CHECK(k.dim() == 4 && ks.dim() == 4 && v.sizes() == k.sizes() && vs.sizes() == ks.sizes() &&
+                  ks.size(0) == k.size(0) && ks.size(1) == k.size(1) && ks.size(2) == k.size(2) && ks.size(3) == 4,
+              "libpad_b200 ", what, ": codes must be [pages, page_size, Hkv, D/2], scales [pages, page_size, Hkv, 4]");
+  for (const at::Tensor* t : {&k, &ks, &v, &vs})
+    TORCH_CHECK(t->scalar_type() == at::kByte, "libpad_b200 ", what, ": codes and scales must be uint8");
+}
+
+void kv_append_fp4(const at::Tensor& k_new, const at::Tensor& v_new, const at::Tensor& k, const at::Tensor& ks,
+                   const at::Tensor& v, const at::Tensor& vs, const at::Tensor& bt_in, const at::Tensor& pos_in,
+                   const c10::optional<at::Tensor>& ids_in) {
+  const at::Device dev = k.device();
+  check_fp4(k, ks, v, vs, "kv_append_fp4");
+  check_on(dev, {&k_new, &v_new, &ks, &v, &vs}, "kv_append_fp4");
+  TORCH_CHECK(k_new.dim() == 3 && v_new.sizes() == k_new.sizes() && k_new.scalar_type() == at::kHalf &&
+                  v_new.scalar_type() == at::kHalf && k_new.size(1) == k.size(2) && k_new.size(2) == 2 * k.size(3),
+              "libpad_b200 kv_append_fp4: k_new and v_new must be fp16 [tokens, Hkv, D] of the cache's heads");
+  TORCH_CHECK(bt_in.dim() == 2 && pos_in.dim() == 1 && pos_in.size(0) == k_new.size(0) &&
+                  (!ids_in.has_value() || (ids_in->dim() == 1 && ids_in->size(0) == k_new.size(0))),
+              "libpad_b200 kv_append_fp4: block_table must be [B, max_pages], positions and seq_ids [tokens]");
+  c10::cuda::CUDAGuard guard(dev);
+  const at::Tensor bt = as_int32_rows(bt_in, dev), pos = as_int32_rows(pos_in, dev);
+  const at::Tensor ids = ids_in.has_value() ? as_int32_rows(*ids_in, dev) : at::Tensor();
+  const at::Tensor kn = k_new.stride(2) == 1 ? k_new : k_new.contiguous();
+  const at::Tensor vn = v_new.stride(2) == 1 ? v_new : v_new.contiguous();
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  StreamState& st = state_for(dev, stream);
+  const Strides kns(kn), vns(vn), k_s(k), ks_s(ks), v_s(v), vs_s(vs);
+  check(pad_paged_kv_append_fp4(kn.data_ptr(), vn.data_ptr(), k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(),
+                                bt.data_ptr<int32_t>(), pos.data_ptr<int32_t>(),
+                                ids.defined() ? ids.data_ptr<int32_t>() : nullptr, kn.size(0), bt.size(0), kn.size(1),
+                                kn.size(2), k.size(0), k.size(1), bt.size(1), kns.s, vns.s, k_s.s, ks_s.s, v_s.s,
+                                vs_s.s, bt.stride(0), stream, st.flags.data_ptr<int32_t>()),
+        "kv_append_fp4");
+}
+
+std::tuple<at::Tensor, at::Tensor> kv_read_fp4(const at::Tensor& k, const at::Tensor& ks, const at::Tensor& v,
+                                               const at::Tensor& vs, const at::Tensor& bt_in, const at::Tensor& pos_in,
+                                               const c10::optional<at::Tensor>& ids_in) {
+  const at::Device dev = k.device();
+  check_fp4(k, ks, v, vs, "kv_read_fp4");
+  check_on(dev, {&ks, &v, &vs}, "kv_read_fp4");
+  TORCH_CHECK(bt_in.dim() == 2 && pos_in.dim() == 1 &&
+                  (!ids_in.has_value() || (ids_in->dim() == 1 && ids_in->size(0) == pos_in.size(0))),
+              "libpad_b200 kv_read_fp4: block_table must be [B, max_pages], positions and seq_ids [tokens]");
+  c10::cuda::CUDAGuard guard(dev);
+  const at::Tensor bt = as_int32_rows(bt_in, dev), pos = as_int32_rows(pos_in, dev);
+  const at::Tensor ids = ids_in.has_value() ? as_int32_rows(*ids_in, dev) : at::Tensor();
+  const int64_t tokens = pos.size(0), hkv = k.size(2), d = 2 * k.size(3);
+  at::Tensor ko = at::empty({tokens, hkv, d}, k.options().dtype(at::kHalf)), vo = at::empty_like(ko);
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  StreamState& st = state_for(dev, stream);
+  const Strides kos(ko), vos(vo), k_s(k), ks_s(ks), v_s(v), vs_s(vs);
+  check(pad_paged_kv_read_fp4(k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), bt.data_ptr<int32_t>(),
+                              pos.data_ptr<int32_t>(), ids.defined() ? ids.data_ptr<int32_t>() : nullptr,
+                              ko.data_ptr(), vo.data_ptr(), tokens, bt.size(0), hkv, d, k.size(0), k.size(1),
+                              bt.size(1), k_s.s, ks_s.s, v_s.s, vs_s.s, kos.s, vos.s, bt.stride(0), stream,
+                              st.flags.data_ptr<int32_t>()),
+        "kv_read_fp4");
+  return {ko, vo};
+}
+
+// weights / slot_positions of a cache: [pages, Hkv, page_size] of one type.
+void check_slots(const at::Tensor& t, at::ScalarType type, int64_t pages, int64_t hkv, int64_t ps, const char* what) {
+  TORCH_CHECK(t.dim() == 3 && t.scalar_type() == type && t.size(0) == pages && t.size(1) == hkv && t.size(2) == ps,
+              "libpad_b200 ", what, ": weights (fp32) and slot_positions (int32) must be [pages, Hkv, page_size]");
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> kv_evict_plan(
+    const at::Tensor& weights, const at::Tensor& bt_in, const at::Tensor& sl_in, int64_t budget, int64_t recent,
+    const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& total_in) {
+  const at::Device dev = weights.device();
+  TORCH_CHECK(weights.dim() == 3 && bt_in.dim() == 2 && sl_in.dim() == 1 && sl_in.size(0) == bt_in.size(0),
+              "libpad_b200 kv_evict_plan: weights must be [pages, Hkv, page_size], block_table [B, max_pages], "
+              "seq_lens [B]");
+  const int64_t pages = weights.size(0), hkv = weights.size(1), ps = weights.size(2), batch = bt_in.size(0);
+  check_slots(weights, at::kFloat, pages, hkv, ps, "kv_evict_plan");
+  TORCH_CHECK(positions.has_value() == total_in.has_value(),
+              "libpad_b200 kv_evict_plan: slot_positions and total_lens go together");
+  if (positions.has_value()) {
+    check_slots(*positions, at::kInt, pages, hkv, ps, "kv_evict_plan");
+    check_on(dev, {&*positions}, "kv_evict_plan");
+    TORCH_CHECK(total_in->dim() == 1 && total_in->size(0) == batch, "libpad_b200 kv_evict_plan: total_lens must be [B]");
+  }
+  c10::cuda::CUDAGuard guard(dev);
+  const at::Tensor bt = as_int32_rows(bt_in, dev), sl = as_int32_rows(sl_in, dev);
+  const at::Tensor total = total_in.has_value() ? as_int32_rows(*total_in, dev) : at::Tensor();
+  int64_t moves = 0;
+  check(pad_evict_max_moves(budget, ps, bt.size(1), &moves), "kv_evict_plan");
+  const auto opt = weights.options().dtype(at::kInt);
+  at::Tensor src = at::empty({batch, hkv, moves}, opt), dst = at::empty({batch, hkv, moves}, opt);
+  at::Tensor counts = at::empty({batch, hkv}, opt), lens = at::empty({batch}, opt);
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  StreamState& st = state_for(dev, stream);
+  const Strides ws(weights), pst(positions.has_value() ? *positions : weights);
+  check(pad_paged_kv_evict_plan(weights.data_ptr<float>(), positions.has_value() ? positions->data_ptr<int32_t>() : nullptr,
+                                bt.data_ptr<int32_t>(), sl.data_ptr<int32_t>(),
+                                total.defined() ? total.data_ptr<int32_t>() : nullptr, src.data_ptr<int32_t>(),
+                                dst.data_ptr<int32_t>(), counts.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), batch,
+                                hkv, pages, ps, bt.size(1), budget, recent, ws.s, pst.s, bt.stride(0), stream,
+                                st.flags.data_ptr<int32_t>()),
+        "kv_evict_plan");
+  return {src, dst, counts, lens};
+}
+
+void kv_move(at::TensorList caches, const at::Tensor& bt_in, const at::Tensor& src, const at::Tensor& dst,
+             const at::Tensor& counts, const c10::optional<at::Tensor>& weights,
+             const c10::optional<at::Tensor>& positions) {
+  TORCH_CHECK(caches.size() >= 1 && caches.size() <= 4, "libpad_b200 kv_move: 1 to 4 caches");
+  const at::Tensor& first = caches[0];
+  TORCH_CHECK(first.dim() == 4, "libpad_b200 kv_move: caches must be [pages, page_size, Hkv, row]");
+  const at::Device dev = first.device();
+  const int64_t pages = first.size(0), ps = first.size(1), hkv = first.size(2), batch = bt_in.size(0);
+  void* ptr[4];
+  int64_t bytes[4], strides[12];
+  for (size_t c = 0; c < caches.size(); ++c) {
+    const at::Tensor& t = caches[c];
+    TORCH_CHECK(t.dim() == 4 && t.size(0) == pages && t.size(1) == ps && t.size(2) == hkv && t.stride(3) == 1,
+                "libpad_b200 kv_move: caches must be [pages, page_size, Hkv, row] with a contiguous row");
+    check_on(dev, {&t}, "kv_move");
+    const int64_t item = t.element_size();
+    ptr[c] = t.data_ptr();
+    bytes[c] = t.size(3) * item;
+    for (int i = 0; i < 3; ++i) strides[3 * c + i] = t.stride(i) * item;
+  }
+  TORCH_CHECK(bt_in.dim() == 2 && src.dim() == 3 && src.size(0) == batch && src.size(1) == hkv &&
+                  dst.sizes() == src.sizes() && counts.dim() == 2 && counts.size(0) == batch &&
+                  counts.size(1) == hkv && src.scalar_type() == at::kInt && dst.scalar_type() == at::kInt &&
+                  counts.scalar_type() == at::kInt && src.is_contiguous() && dst.is_contiguous() &&
+                  counts.is_contiguous(),
+              "libpad_b200 kv_move: src, dst [B, Hkv, moves] and counts [B, Hkv] must be contiguous int32, as a plan "
+              "returns them");
+  check_on(dev, {&src, &dst, &counts}, "kv_move");
+  if (weights.has_value()) {
+    check_slots(*weights, at::kFloat, pages, hkv, ps, "kv_move");
+    check_on(dev, {&*weights}, "kv_move");
+  }
+  if (positions.has_value()) {
+    check_slots(*positions, at::kInt, pages, hkv, ps, "kv_move");
+    check_on(dev, {&*positions}, "kv_move");
+  }
+  c10::cuda::CUDAGuard guard(dev);
+  const at::Tensor bt = as_int32_rows(bt_in, dev);
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  StreamState& st = state_for(dev, stream);
+  const Strides ws(weights.has_value() ? *weights : src), pst(positions.has_value() ? *positions : src);
+  check(pad_paged_kv_move((int64_t)caches.size(), ptr, bytes, strides, bt.data_ptr<int32_t>(), src.data_ptr<int32_t>(),
+                          dst.data_ptr<int32_t>(), counts.data_ptr<int32_t>(),
+                          weights.has_value() ? weights->data_ptr<float>() : nullptr,
+                          positions.has_value() ? positions->data_ptr<int32_t>() : nullptr, batch, hkv, pages, ps,
+                          bt.size(1), src.size(2), ws.s, pst.s, bt.stride(0), stream, st.flags.data_ptr<int32_t>()),
+        "kv_move");
+}
+
 // The error-flag word of `device`'s current stream (the kernels OR
 // PAD_FLAG_* bits into it; the caller reads and clears it).
 at::Tensor error_flags(int64_t device) {
@@ -191,6 +360,14 @@ TORCH_LIBRARY(pad_b200, m) {
         "Tensor kv_last_page_len, int num_splits, float scale, Tensor(a!)? out) -> Tensor");
   m.def("kv_append(Tensor k_new, Tensor v_new, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, "
         "Tensor positions) -> ()");
+  m.def("kv_append_fp4(Tensor k_new, Tensor v_new, Tensor(a!) k_cache, Tensor(b!) k_scales, Tensor(c!) v_cache, "
+        "Tensor(d!) v_scales, Tensor block_table, Tensor positions, Tensor? seq_ids) -> ()");
+  m.def("kv_read_fp4(Tensor k_cache, Tensor k_scales, Tensor v_cache, Tensor v_scales, Tensor block_table, "
+        "Tensor positions, Tensor? seq_ids) -> (Tensor, Tensor)");
+  m.def("kv_evict_plan(Tensor weights, Tensor block_table, Tensor seq_lens, int budget, int recent, "
+        "Tensor? slot_positions, Tensor? total_lens) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("kv_move(Tensor(a!)[] caches, Tensor block_table, Tensor src, Tensor dst, Tensor counts, "
+        "Tensor(b!)? weights, Tensor(c!)? slot_positions) -> ()");
   m.def("error_flags(int device) -> Tensor", &error_flags);
 }
 
@@ -198,4 +375,8 @@ TORCH_LIBRARY_IMPL(pad_b200, CUDA, m) {
   m.impl("decode", &decode);
   m.impl("decode_csr", &decode_csr);
   m.impl("kv_append", &kv_append);
+  m.impl("kv_append_fp4", &kv_append_fp4);
+  m.impl("kv_read_fp4", &kv_read_fp4);
+  m.impl("kv_evict_plan", &kv_evict_plan);
+  m.impl("kv_move", &kv_move);
 }

@@ -23,7 +23,7 @@ INCLUDE = os.path.join(REPO, "include")
 LIB_NAME = "libpad_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 OPS_PATH = os.path.join(HERE, "_pad_torch_ops.so")
-SOURCES = ["pad_decode.cu", "pad_kv_append.cu"]
+SOURCES = ["pad_decode.cu", "pad_kv_append.cu", "pad_kv_fp4.cu", "pad_evict.cu"]
 OPS_SOURCE = "pad_torch_op.cpp"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -1,0 +1,72 @@
+"""Eviction from a paged cache by accumulated attention weight.
+
+Beside the cache live ``weights`` (fp32) and, if recent tokens are to be kept
+whatever they weigh, ``slot_positions`` (int32), both [num_pages, Hkv,
+page_size] and addressed through the cache's block table: what each slot's
+token has received so far (the decode with weights adds to it) and the token's
+position in its sequence. Every KV head keeps its own tokens. The reference has
+no counterpart.
+"""
+
+from __future__ import annotations
+
+from typing import Sequence
+
+import torch
+
+from . import _lib
+from .kernel_cuda_v4 import _check_values, _raise_if_checking
+
+_OPS = _lib.ops()
+
+
+def paged_kv_evict_plan(weights: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int,
+                        recent: int = 0, *, slot_positions: torch.Tensor | None = None,
+                        total_lens: torch.Tensor | None = None):
+    """Which slots to keep, as the moves that make them the first ``budget``.
+
+    For every sequence with seq_lens[b] > budget and every KV head the slots
+    kept are first those whose slot_positions are at least total_lens[b] -
+    recent (total_lens [B]: tokens the sequence has seen), then the heaviest
+    (NaN above all), ties to the lower slot. Returns (src, dst, counts,
+    new_lens): move i < counts[b, h] copies slot src[b, h, i] to dst[b, h, i]
+    (both ascending, -1 behind the last), and new_lens = min(seq_lens, budget).
+    Slots keep their place unless they lie at or above the budget, so their
+    order says nothing about age afterwards; attention does not depend on it."""
+    assert weights.is_cuda, "pad_b200 requires CUDA tensors"
+    assert weights.dtype == torch.float32 and weights.dim() == 3, "weights must be fp32 [num_pages, Hkv, page_size]"
+    assert budget >= 1, "budget must be >= 1"
+    assert 0 <= recent <= budget, "recent must lie in [0, budget]"
+    assert recent == 0 or slot_positions is not None, "recent needs slot_positions"
+    if slot_positions is not None and total_lens is None:
+        total_lens = seq_lens
+    _check_values(weights.device)
+    got = _OPS.kv_evict_plan(weights, block_table, seq_lens, budget, recent, slot_positions,
+                             total_lens if slot_positions is not None else None)
+    _raise_if_checking(weights.device)
+    return got
+
+
+def paged_kv_move(caches: Sequence[torch.Tensor], block_table: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+                  counts: torch.Tensor, *, weights: torch.Tensor | None = None,
+                  slot_positions: torch.Tensor | None = None) -> None:
+    """Carry out a plan's moves, in place: slot src[b, h, i] -> dst[b, h, i] for
+    i < counts[b, h], in 1 to 4 caches [num_pages, page_size, Hkv, row] of any
+    type (an fp16 cache's K and V, or a 4-bit cache's four tensors) and in
+    weights and slot_positions. No dst may be a src or occur twice."""
+    assert len(caches) >= 1 and all(c.is_cuda for c in caches), "pad_b200 requires CUDA tensors"
+    _check_values(caches[0].device)
+    _OPS.kv_move(list(caches), block_table, src, dst, counts, weights, slot_positions)
+    _raise_if_checking(caches[0].device)
+
+
+def paged_kv_evict(caches: Sequence[torch.Tensor], weights: torch.Tensor, block_table: torch.Tensor,
+                   seq_lens: torch.Tensor, budget: int, recent: int = 0, *,
+                   slot_positions: torch.Tensor | None = None,
+                   total_lens: torch.Tensor | None = None) -> torch.Tensor:
+    """Cut every sequence to ``budget`` slots in place (paged_kv_evict_plan, then
+    paged_kv_move) and return the new seq_lens. The pages behind them are free."""
+    src, dst, counts, new_lens = paged_kv_evict_plan(weights, block_table, seq_lens, budget, recent,
+                                                     slot_positions=slot_positions, total_lens=total_lens)
+    paged_kv_move(caches, block_table, src, dst, counts, weights=weights, slot_positions=slot_positions)
+    return new_lens

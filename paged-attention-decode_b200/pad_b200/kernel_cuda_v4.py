@@ -72,6 +72,8 @@ def _raise_for_flags(flags: int) -> None:
         raise ValueError("block_table contains an invalid physical page id")
     if flags & _lib.PAD_FLAG_SEQ_LEN_RANGE:
         raise ValueError("seq_lens contains negative values or values larger than block_table can address")
+    if flags & _lib.PAD_FLAG_BAD_SEQ_ID:
+        raise ValueError("seq_ids contains an entry that is no sequence of block_table")
     if flags & _lib.PAD_FLAG_WAIT_TIMEOUT:
         raise RuntimeError("libpad_b200: an in-kernel wait timed out")
 
@@ -125,6 +127,18 @@ def read_error_flags(device: torch.device | None = None, reset: bool = True) -> 
     if reset:
         flags.zero_()
     return v
+
+
+def _check_values(device: torch.device) -> None:
+    """With PAD_B200_CHECK=1: forget flags of earlier calls (syncs)."""
+    if _CHECK_VALUES:
+        read_error_flags(device)
+
+
+def _raise_if_checking(device: torch.device) -> None:
+    """With PAD_B200_CHECK=1: raise for the flags of the call just made (syncs)."""
+    if _CHECK_VALUES:
+        _raise_for_flags(read_error_flags(device))
 
 
 def paged_kv_indices(block_table: torch.Tensor, seq_lens: torch.Tensor, page_size: int):

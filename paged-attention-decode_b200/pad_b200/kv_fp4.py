@@ -1,0 +1,67 @@
+"""The paged KV cache in microscaled 4-bit floating point.
+
+A row (one token of one KV head) of K or V is ``head_dim/2`` bytes of e2m1
+codes, two to a byte with the lower dim in the low nibble, and 4 scale bytes of
+which the first ``head_dim/32`` are used: byte j is the power of two
+``2^(byte - 127)`` of dims [32j, 32j + 32), 255 meaning NaN. That is 4.25 bits
+a value at head_dim 128 against 16, laid out as the fp16 cache is::
+
+    k_cache, v_cache    [num_pages, page_size, Hkv, head_dim / 2]  uint8
+    k_scales, v_scales  [num_pages, page_size, Hkv, 4]             uint8
+
+The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .kernel_cuda_v4 import _check_values, _raise_if_checking
+
+_OPS = _lib.ops()
+FP4_HEAD_DIMS = (32, 64, 128)
+
+
+def paged_kv_cache_fp4(num_pages: int, page_size: int, num_kv_heads: int, head_dim: int, device="cuda"):
+    """A new cache of zeros: (k_cache, k_scales, v_cache, v_scales)."""
+    assert head_dim in FP4_HEAD_DIMS, f"head_dim must be one of {FP4_HEAD_DIMS}"
+    rows = (num_pages, page_size, num_kv_heads)
+    new = lambda n: torch.zeros((*rows, n), dtype=torch.uint8, device=device)  # noqa: E731
+    return new(head_dim // 2), new(4), new(head_dim // 2), new(4)
+
+
+def paged_kv_append_fp4(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch.Tensor, k_scales: torch.Tensor,
+                        v_cache: torch.Tensor, v_scales: torch.Tensor, block_table: torch.Tensor,
+                        positions: torch.Tensor, seq_ids: torch.Tensor | None = None) -> None:
+    """Quantise new tokens and write them into the 4-bit cache in place.
+
+    Row t of k_new / v_new [tokens, Hkv, D] fp16 becomes token positions[t] of
+    sequence seq_ids[t] (None: of sequence t, one token of each sequence at
+    most), so one call takes a decoding step or whole prompts; positions[t] < 0
+    skips t. Per block of 32 dims the scale is the power of two that puts the
+    largest magnitude into [4, 8), at least 2^-24, and the codes are rounded to
+    nearest even and saturate at 6; a block with an Inf or NaN becomes NaN. A
+    call must not name the same (sequence, position) twice."""
+    assert k_new.is_cuda and k_cache.is_cuda, "pad_b200 requires CUDA tensors"
+    assert k_new.dtype == torch.float16 and v_new.dtype == torch.float16, "pad_b200 expects fp16 k_new/v_new"
+    assert k_new.dim() == 3 and k_new.shape[2] in FP4_HEAD_DIMS, f"head_dim must be one of {FP4_HEAD_DIMS}"
+    assert seq_ids is not None or k_new.shape[0] <= block_table.shape[0], "more tokens than sequences need seq_ids"
+    _check_values(k_cache.device)
+    _OPS.kv_append_fp4(k_new, v_new, k_cache, k_scales, v_cache, v_scales, block_table, positions, seq_ids)
+    _raise_if_checking(k_cache.device)
+
+
+def paged_kv_read_fp4(k_cache: torch.Tensor, k_scales: torch.Tensor, v_cache: torch.Tensor, v_scales: torch.Tensor,
+                      block_table: torch.Tensor, positions: torch.Tensor, seq_ids: torch.Tensor | None = None):
+    """The fp16 values (k, v) [tokens, Hkv, D] that the 4-bit cache holds for
+    token positions[t] of sequence seq_ids[t] (None: of sequence t) -- what a
+    later chunk of a prompt attends to. Exact for rows written by
+    paged_kv_append_fp4; positions[t] < 0 reads as zeros."""
+    assert k_cache.is_cuda, "pad_b200 requires CUDA tensors"
+    assert 2 * k_cache.shape[3] in FP4_HEAD_DIMS, f"head_dim must be one of {FP4_HEAD_DIMS}"
+    assert seq_ids is not None or positions.shape[0] <= block_table.shape[0], "more tokens than sequences need seq_ids"
+    _check_values(k_cache.device)
+    got = _OPS.kv_read_fp4(k_cache, k_scales, v_cache, v_scales, block_table, positions, seq_ids)
+    _raise_if_checking(k_cache.device)
+    return got
