@@ -55,6 +55,7 @@ typedef enum pad_status {
 #define PAD_FLAG_BAD_PAGE_ID 0x1     /* a block_table entry outside [0, num_pages) */
 #define PAD_FLAG_SEQ_LEN_RANGE 0x2   /* seq_len < 0 or > max_pages_per_seq * page_size */
 #define PAD_FLAG_BAD_SEQ_ID 0x4      /* a seq_ids entry outside [0, batch) */
+#define PAD_FLAG_SHARED_PAGE 0x8     /* more tokens than the pool's pages hold: sequences share pages */
 #define PAD_FLAG_WAIT_TIMEOUT 0x100  /* an in-kernel wait gave up (never expected) */
 
 /* Human-readable text for a status code (static storage). */
@@ -244,6 +245,18 @@ int pad_paged_kv_read_fp4(const void* k_cache, const void* k_scales, const void*
  * the token's position in its sequence (after an eviction a slot no longer
  * tells it). Any strides (in elements). A page belongs to one sequence.
  *
+ * pad_paged_attention_decode_weights is pad_paged_attention_decode and then,
+ * for every slot t < seq_lens[b] and KV head,
+ *   weights = (t >= seq_lens[b] - num_new ? 0 : weights) + the softmax
+ *             probabilities of the token, summed over the KV head's query heads
+ * so that slots of the num_new newest tokens need no clearing; with
+ * slot_positions these slots also get total_lens[b] - seq_lens[b] + t. The
+ * workspace (pad_decode_weights_workspace_bytes) also holds the call's scores,
+ * 4 bytes per query head and token that the batch can hold: of min(batch *
+ * max_pages_per_seq, num_pages) pages. Sequences that share pages lose weight
+ * (no atomics: results are repeatable); PAD_FLAG_SHARED_PAGE is set when they
+ * hold more tokens than the pool.
+ *
  * pad_paged_kv_evict_plan chooses, for every sequence b with seq_lens[b] >
  * budget and every KV head, the `budget` slots to keep: first those that are
  * recent (slot_positions >= total_lens[b] - recent), then by weight descending
@@ -262,6 +275,19 @@ int pad_paged_kv_read_fp4(const void* k_cache, const void* k_scales, const void*
  * slot_positions (each optional). Within one (sequence, KV head) no dst may be
  * a src or occur twice, as in a plan. Entries outside the block table set
  * PAD_FLAG_SEQ_LEN_RANGE and are skipped. No counterpart in the reference. */
+int pad_decode_weights_workspace_bytes(int device, int64_t batch, int64_t num_kv_heads, int64_t gqa_ratio,
+                                       int64_t head_dim, int64_t num_pages, int64_t page_size,
+                                       int64_t max_pages_per_seq, int64_t num_splits, size_t* bytes);
+int pad_paged_attention_decode_weights(const void* q, const void* k_cache, const void* v_cache,
+                                       const int32_t* block_table, const int32_t* seq_lens, void* out,
+                                       float* weights, int32_t* slot_positions, const int32_t* total_lens,
+                                       int64_t num_new, int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+                                       int64_t head_dim, int64_t num_pages, int64_t page_size,
+                                       int64_t max_pages_per_seq, const int64_t* q_strides, const int64_t* k_strides,
+                                       const int64_t* v_strides, int64_t block_table_stride,
+                                       const int64_t* out_strides, const int64_t* weight_strides,
+                                       const int64_t* position_strides, float scale, int64_t num_splits,
+                                       void* workspace, size_t workspace_bytes, void* stream, int32_t* error_flags);
 int pad_evict_max_moves(int64_t budget, int64_t page_size, int64_t max_pages_per_seq, int64_t* max_moves);
 int pad_paged_kv_evict_plan(const float* weights, const int32_t* slot_positions, const int32_t* block_table,
                             const int32_t* seq_lens, const int32_t* total_lens, int32_t* src, int32_t* dst,

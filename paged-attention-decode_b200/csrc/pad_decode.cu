@@ -14,7 +14,7 @@
 #include <string>
 
 #include "pad_b200.h"
-#include "pad_decode_kernels.cuh"
+#include "pad_decode_instance.cuh"
 #include "pad_error.cuh"
 
 namespace {
@@ -22,57 +22,19 @@ namespace {
 using namespace pad;
 
 // ----------------------------------------------------------------- instances
-struct Instance {
-  const void* kernel;          // decode_stream_kernel<TR>
-  const void* merge_small;     // merge_kernel<D, 128>: few partials per split pair
-  const void* merge_mid;       // merge_kernel<D, 256, D/32, 4>: a handful of partials, D split over CTAs
-  const void* merge_large;     // merge_kernel<D, 256, D/32, 8>: many partials (long context)
-  int merge_dsplit;
-  int smem_bytes;
-  int segw;                    // bytes per row segment (TMA box inner extent)
-  bool swz;
-  int hg;                      // KV heads per tile
-  int tt;                      // tokens per tile
-};
-
 // Columns of D one wide-merge CTA folds (the merge grid splits D by it).
 #ifndef PAD_MERGE_COLS
 #define PAD_MERGE_COLS 32
 #endif
 constexpr int kMergeCols = PAD_MERGE_COLS;
 
-template <int D, int NT, int HG, bool SWZ>
-Instance make_instance() {
-  using TR = Traits<D, NT, HG, SWZ>;
-  Instance in;
-  in.kernel = reinterpret_cast<const void*>(&decode_stream_kernel<TR>);
-  in.merge_small = reinterpret_cast<const void*>(&merge_kernel<D, 128, 1, 4>);
-  in.merge_mid = reinterpret_cast<const void*>(&merge_kernel<D, 256, (D >= 2 * kMergeCols ? D / kMergeCols : 1), 4>);
-  in.merge_large = reinterpret_cast<const void*>(&merge_kernel<D, 256, (D >= 2 * kMergeCols ? D / kMergeCols : 1), 8>);
-  in.merge_dsplit = D >= 2 * kMergeCols ? D / kMergeCols : 1;
-  in.smem_bytes = TR::SMEM_BYTES;
-  in.segw = TR::SEGW;
-  in.swz = SWZ;
-  in.hg = HG;
-  in.tt = TR::TT;
-  return in;
-}
-
-template <int D, int NT, int HG>
-Instance pick_swz(bool swz) {
-  return swz ? make_instance<D, NT, HG, true>() : make_instance<D, NT, HG, false>();
-}
-
-template <int D, int NT>
-Instance pick_hg(int hg, bool swz) {
-  switch (hg) {
-    case 8:
-      if constexpr (NT == 1) return pick_swz<D, NT, 8>(swz);
-      else return pick_swz<D, NT, 4>(swz);  // not reached: G > 8 caps the head group at 4
-    case 4: return pick_swz<D, NT, 4>(swz);
-    case 2: return pick_swz<D, NT, 2>(swz);
-    default: return pick_swz<D, NT, 1>(swz);
-  }
+template <int D>
+void set_merge(Instance* in) {
+  constexpr int DS = D >= 2 * kMergeCols ? D / kMergeCols : 1;
+  in->merge_small = reinterpret_cast<const void*>(&merge_kernel<D, 128, 1, 4>);
+  in->merge_mid = reinterpret_cast<const void*>(&merge_kernel<D, 256, DS, 4>);
+  in->merge_large = reinterpret_cast<const void*>(&merge_kernel<D, 256, DS, 8>);
+  in->merge_dsplit = DS;
 }
 
 // KV heads per tile: the largest of 8, 4, 2, 1 dividing num_kv_heads (at
@@ -96,15 +58,16 @@ int head_group_for(int64_t hkv, int64_t gqa) {
 constexpr int64_t kMergeWide = PAD_MERGE_WIDE, kMergeDeep = PAD_MERGE_DEEP;
 constexpr int64_t kFewPairs = 16;  // the num_splits=None heuristic: see make_plan
 
-bool pick_instance(int64_t head_dim, int64_t gqa, int hg, bool swz, Instance* out) {
-  const bool nt1 = gqa <= 8;
+bool pick_instance(int64_t head_dim, int64_t gqa, int hg, bool swz, Instance* out, bool weights = false) {
+  if (!(weights ? pick_decode_weights(head_dim, gqa, hg, swz, out) : pick_decode<false>(head_dim, gqa, hg, swz, out)))
+    return false;
   switch (head_dim) {
-    case 16: *out = nt1 ? pick_hg<16, 1>(hg, swz) : pick_hg<16, 2>(hg, swz); return true;
-    case 32: *out = nt1 ? pick_hg<32, 1>(hg, swz) : pick_hg<32, 2>(hg, swz); return true;
-    case 64: *out = nt1 ? pick_hg<64, 1>(hg, swz) : pick_hg<64, 2>(hg, swz); return true;
-    case 128: *out = nt1 ? pick_hg<128, 1>(hg, swz) : pick_hg<128, 2>(hg, swz); return true;
-    default: return false;
+    case 16: set_merge<16>(out); break;
+    case 32: set_merge<32>(out); break;
+    case 64: set_merge<64>(out); break;
+    default: set_merge<128>(out); break;
   }
+  return true;
 }
 
 // Largest power of two that divides page_size, capped at the tile's token
@@ -117,7 +80,7 @@ int box_rows_for(int64_t page_size, int tt) {
 
 // Per-device, per-instance cached facts: opt-in shared memory set, occupancy.
 constexpr int kMaxDevices = 64;
-constexpr int kNumInstanceKeys = 4 * 2 * 4 * 2;
+constexpr int kNumInstanceKeys = 2 * 4 * 2 * 4 * 2;
 struct DeviceCache {
   int num_sms = 0;
   int occ[kNumInstanceKeys] = {};
@@ -126,10 +89,10 @@ struct DeviceCache {
 DeviceCache g_dev[kMaxDevices];
 std::mutex g_mu;
 
-int instance_key(int64_t head_dim, int64_t gqa, int hg, bool swz) {
+int instance_key(int64_t head_dim, int64_t gqa, int hg, bool swz, bool weights = false) {
   const int di = head_dim == 16 ? 0 : head_dim == 32 ? 1 : head_dim == 64 ? 2 : 3;
   const int hi = hg == 1 ? 0 : hg == 2 ? 1 : hg == 4 ? 2 : 3;
-  return ((di * 2 + (gqa <= 8 ? 0 : 1)) * 4 + hi) * 2 + (swz ? 1 : 0);
+  return (((weights ? 4 : 0) + di) * 2 + (gqa <= 8 ? 0 : 1)) * 8 + hi * 2 + (swz ? 1 : 0);
 }
 
 int prepare_device(int device, const Instance& in, int key, int* num_sms, int* occ) {
@@ -182,14 +145,19 @@ struct Plan {
   int64_t partitions = 0;
   int64_t slots = 0;
   size_t off_meta = 0, off_ml = 0, off_o = 0, bytes = 0;
+  // the decode with attention weights
+  int64_t raw_tiles = 0;
+  size_t off_raw = 0, off_tiles = 0, off_pairs = 0, off_total = 0;
 };
 
 size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // max_pages: block-table width (dense) or total pages of the index (CSR,
 // csr = true), which bounds the tiles differently.
+// weight_pages >= 0: the decode with attention weights, over that many pages.
 int make_plan(int device, int64_t batch, int64_t hkv, int64_t gqa, int64_t head_dim, int64_t page_size,
-              int64_t max_pages, int64_t num_splits, Plan* plan, bool csr = false) {
+              int64_t max_pages, int64_t num_splits, Plan* plan, bool csr = false, int64_t weight_pages = -1) {
+  const bool weights = weight_pages >= 0;
   if (batch < 0 || hkv <= 0 || gqa <= 0 || page_size <= 0 || max_pages < 0)
     return fail(PAD_ERR_INVALID_ARGUMENT,
                 "invalid sizes: batch=%lld num_kv_heads=%lld gqa_ratio=%lld page_size=%lld max_pages=%lld",
@@ -207,9 +175,9 @@ int make_plan(int device, int64_t batch, int64_t hkv, int64_t gqa, int64_t head_
     return fail(PAD_ERR_UNSUPPORTED, "problem too large for 32-bit tile indexing (%lld tiles)", (long long)tiles_ub);
   plan->box_rows = box_rows_for(page_size, tt);
   const bool swz = plan->box_rows >= 8;
-  if (!pick_instance(head_dim, gqa, hg, swz, &plan->inst))
+  if (!pick_instance(head_dim, gqa, hg, swz, &plan->inst, weights))
     return fail(PAD_ERR_UNSUPPORTED, "no kernel instance for head_dim %lld", (long long)head_dim);
-  plan->key = instance_key(head_dim, gqa, hg, swz);
+  plan->key = instance_key(head_dim, gqa, hg, swz, weights);
   int sms = 0, occ = 0;
   int st = prepare_device(device, plan->inst, plan->key, &sms, &occ);
   if (st != PAD_OK) return st;
@@ -239,6 +207,18 @@ int make_plan(int device, int64_t batch, int64_t hkv, int64_t gqa, int64_t head_
   plan->off_ml = align_up((size_t)std::max<int64_t>(parts, batch * groups) * sizeof(int4), 256);
   plan->off_o = align_up(plan->off_ml + (size_t)plan->slots * hg * gqa * sizeof(float2), 256);
   plan->bytes = align_up(plan->off_o + (size_t)plan->slots * hg * gqa * head_dim * sizeof(float), 256);
+  if (weights) {
+    // Scores: no more tiles than the table can name, nor than the pool's pages
+    // fill when each belongs to one sequence (whose last tile may be partial).
+    if (weight_pages > INT64_MAX / page_size)
+      return fail(PAD_ERR_UNSUPPORTED, "num_pages * page_size exceeds 64 bits");
+    plan->raw_tiles = std::min(tiles_ub, groups * (weight_pages * page_size / tt + batch));
+    plan->off_total = plan->bytes;
+    plan->off_pairs = plan->off_total + 256;
+    plan->off_tiles = align_up(plan->off_pairs + (size_t)(batch * groups) * sizeof(int2), 256);
+    plan->off_raw = align_up(plan->off_tiles + (size_t)plan->raw_tiles * sizeof(int4), 256);
+    plan->bytes = align_up(plan->off_raw + (size_t)plan->raw_tiles * kTileRows * gqa * sizeof(float), 256);
+  }
   return PAD_OK;
 }
 
@@ -375,6 +355,24 @@ int pad_decode_workspace_bytes(int device, int64_t batch, int64_t num_kv_heads, 
 
 namespace {
 
+// The attention weights of a decode, where they are asked for.
+struct WeightArgs {
+  float* weights;
+  const int64_t* weight_strides;
+  int32_t* slot_positions;
+  const int64_t* position_strides;
+  const int32_t* total_lens;
+  int64_t num_new;
+};
+
+int check_weights(const WeightArgs& w) {
+  if (w.weights == nullptr || w.weight_strides == nullptr) return fail(PAD_ERR_INVALID_ARGUMENT, "null weights");
+  if (w.slot_positions != nullptr && (w.position_strides == nullptr || w.total_lens == nullptr))
+    return fail(PAD_ERR_INVALID_ARGUMENT, "slot_positions need position_strides and total_lens");
+  if (w.num_new < 0) return fail(PAD_ERR_INVALID_ARGUMENT, "num_new must not be negative");
+  return PAD_OK;
+}
+
 // Shared body of the dense and the CSR entry points (csr_indptr == nullptr:
 // dense block table + seq_lens; else block_table is the CSR `indices` array
 // of max_pages_per_seq = nnz entries).
@@ -384,7 +382,7 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
                 int64_t max_pages_per_seq, const int64_t* q_strides, const int64_t* k_strides,
                 const int64_t* v_strides, int64_t block_table_stride, const int64_t* out_strides, float scale,
                 int64_t num_splits, void* workspace, size_t workspace_bytes, void* stream, int32_t* error_flags,
-                bool static_scratch = false) {
+                bool static_scratch = false, const WeightArgs* wa = nullptr) {
   const bool csr = csr_indptr != nullptr;
   // ---- shape-only checks (no device access, no sync)
   if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_pages < 0 || page_size <= 0 ||
@@ -430,7 +428,8 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   Plan plan;
-  int st = make_plan(device, batch, num_kv_heads, gqa, head_dim, page_size, max_pages_per_seq, num_splits, &plan, csr);
+  int st = make_plan(device, batch, num_kv_heads, gqa, head_dim, page_size, max_pages_per_seq, num_splits, &plan, csr,
+                     wa != nullptr ? num_pages : -1);
   if (st != PAD_OK) return st;
   if (static_scratch && plan.bytes > workspace_bytes)
     return fail(PAD_ERR_WORKSPACE,
@@ -492,6 +491,13 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
   // (PAD_B200_L2_WARM overrides, for A/B timing; 0 turns it off)
   prm.l2_warm = env_int("PAD_B200_L2_WARM", 4);
   prm.scale_log2 = scale * kLog2e;
+  if (wa != nullptr) {
+    prm.track.raw = reinterpret_cast<float*>(ws + plan.off_raw);
+    prm.track.tiles = reinterpret_cast<int4*>(ws + plan.off_tiles);
+    prm.track.pairs = reinterpret_cast<int2*>(ws + plan.off_pairs);
+    prm.track.total = reinterpret_cast<int*>(ws + plan.off_total);
+    prm.track.raw_tiles = (int)plan.raw_tiles;
+  }
 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   void* args[] = {&prm};
@@ -539,6 +545,33 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
     e = cudaLaunchKernelExC(&cfg, wide ? (deep ? in.merge_large : in.merge_mid) : in.merge_small, margs);
     if (e != cudaSuccess) return cuda_fail(e, "launching the merge kernel");
   }
+  if (wa != nullptr) {
+    WeightParams wp = {};
+    wp.track = prm.track;
+    wp.ml = prm.ws_ml;
+    wp.block_table = block_table;
+    wp.total_lens = wa->total_lens;
+    wp.weights = wa->weights;
+    wp.slot_positions = wa->slot_positions;
+    wp.w0 = wa->weight_strides[0];
+    wp.w1 = wa->weight_strides[1];
+    wp.w2 = wa->weight_strides[2];
+    if (wa->slot_positions != nullptr) {
+      wp.p0 = wa->position_strides[0];
+      wp.p1 = wa->position_strides[1];
+      wp.p2 = wa->position_strides[2];
+    }
+    wp.bt_stride = block_table_stride;
+    wp.hg = in.hg;
+    wp.gqa = (int)gqa;
+    wp.tt = in.tt;
+    wp.ngroups = (int)(num_kv_heads / in.hg);
+    wp.page_size = (int)page_size;
+    wp.page_shift = prm.page_shift;
+    wp.num_pages = (int)num_pages;
+    wp.num_new = (int)std::min<int64_t>(wa->num_new, INT32_MAX);
+    if ((st = launch_weights(wp, s)) != PAD_OK) return st;
+  }
   return PAD_OK;
 }
 
@@ -580,6 +613,39 @@ int pad_paged_attention_decode_csr(const void* q, const void* k_cache, const voi
   return decode_impl(q, k_cache, v_cache, kv_indices, nullptr, kv_indptr, kv_last_page_len, out, batch, num_q_heads,
                      num_kv_heads, head_dim, num_pages, page_size, nnz_pages, q_strides, k_strides, v_strides,
                      nnz_pages, out_strides, scale, num_splits, workspace, workspace_bytes, stream, error_flags);
+}
+
+int pad_decode_weights_workspace_bytes(int device, int64_t batch, int64_t num_kv_heads, int64_t gqa_ratio,
+                                       int64_t head_dim, int64_t num_pages, int64_t page_size,
+                                       int64_t max_pages_per_seq, int64_t num_splits, size_t* bytes) {
+  if (bytes == nullptr) return fail(PAD_ERR_INVALID_ARGUMENT, "null output pointer");
+  if (num_pages < 0) return fail(PAD_ERR_INVALID_ARGUMENT, "negative num_pages");
+  Plan plan;
+  int st = make_plan(device, batch, num_kv_heads, gqa_ratio, head_dim, page_size, max_pages_per_seq, num_splits, &plan,
+                     false, num_pages);
+  if (st == PAD_OK) *bytes = plan.bytes;
+  return st;
+}
+
+int pad_paged_attention_decode_weights(const void* q, const void* k_cache, const void* v_cache,
+                                       const int32_t* block_table, const int32_t* seq_lens, void* out,
+                                       float* weights, int32_t* slot_positions, const int32_t* total_lens,
+                                       int64_t num_new, int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+                                       int64_t head_dim, int64_t num_pages, int64_t page_size,
+                                       int64_t max_pages_per_seq, const int64_t* q_strides, const int64_t* k_strides,
+                                       const int64_t* v_strides, int64_t block_table_stride,
+                                       const int64_t* out_strides, const int64_t* weight_strides,
+                                       const int64_t* position_strides, float scale, int64_t num_splits,
+                                       void* workspace, size_t workspace_bytes, void* stream, int32_t* error_flags) {
+  const WeightArgs wa{weights, weight_strides, slot_positions, position_strides, total_lens, num_new};
+  if (batch > 0 && num_pages > 0 && max_pages_per_seq > 0) {
+    const int st = check_weights(wa);
+    if (st != PAD_OK) return st;
+  }
+  return decode_impl(q, k_cache, v_cache, block_table, seq_lens, nullptr, nullptr, out, batch, num_q_heads,
+                     num_kv_heads, head_dim, num_pages, page_size, max_pages_per_seq, q_strides, k_strides, v_strides,
+                     block_table_stride, out_strides, scale, num_splits, workspace, workspace_bytes, stream,
+                     error_flags, false, &wa);
 }
 
 // ----------------------------------------------------------------- no-alloc entry

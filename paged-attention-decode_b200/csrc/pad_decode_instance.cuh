@@ -1,0 +1,68 @@
+// pad_decode_instance.cuh -- the instances of the decode kernel and their choice.
+#pragma once
+
+#include "pad_decode_kernels.cuh"
+
+namespace pad {
+
+struct Instance {
+  const void* kernel;          // decode_stream_kernel<TR>
+  const void* merge_small;     // merge_kernel<D, 128>: few partials per split pair
+  const void* merge_mid;       // merge_kernel<D, 256, D/32, 4>: a handful of partials, D split over CTAs
+  const void* merge_large;     // merge_kernel<D, 256, D/32, 8>: many partials (long context)
+  int merge_dsplit;
+  int smem_bytes;
+  int segw;                    // bytes per row segment (TMA box inner extent)
+  bool swz;
+  int hg;                      // KV heads per tile
+  int tt;                      // tokens per tile
+};
+
+// The decode kernel's part of an instance (the merge kernels are filled in by
+// pad_decode.cu, the one translation unit that instantiates them).
+template <int D, int NT, int HG, bool SWZ, bool WT>
+Instance make_instance() {
+  using TR = Traits<D, NT, HG, SWZ, WT>;
+  Instance in = {};
+  in.kernel = reinterpret_cast<const void*>(&decode_stream_kernel<TR>);
+  in.smem_bytes = TR::SMEM_BYTES;
+  in.segw = TR::SEGW;
+  in.swz = SWZ;
+  in.hg = HG;
+  in.tt = TR::TT;
+  return in;
+}
+
+template <int D, int NT, int HG, bool WT>
+Instance pick_swz(bool swz) {
+  return swz ? make_instance<D, NT, HG, true, WT>() : make_instance<D, NT, HG, false, WT>();
+}
+
+template <int D, int NT, bool WT>
+Instance pick_hg(int hg, bool swz) {
+  switch (hg) {
+    case 8:
+      if constexpr (NT == 1) return pick_swz<D, NT, 8, WT>(swz);
+      else return pick_swz<D, NT, 4, WT>(swz);  // not reached: G > 8 caps the head group at 4
+    case 4: return pick_swz<D, NT, 4, WT>(swz);
+    case 2: return pick_swz<D, NT, 2, WT>(swz);
+    default: return pick_swz<D, NT, 1, WT>(swz);
+  }
+}
+
+template <bool WT>
+bool pick_decode(int64_t head_dim, int64_t gqa, int hg, bool swz, Instance* out) {
+  const bool nt1 = gqa <= 8;
+  switch (head_dim) {
+    case 16: *out = nt1 ? pick_hg<16, 1, WT>(hg, swz) : pick_hg<16, 2, WT>(hg, swz); return true;
+    case 32: *out = nt1 ? pick_hg<32, 1, WT>(hg, swz) : pick_hg<32, 2, WT>(hg, swz); return true;
+    case 64: *out = nt1 ? pick_hg<64, 1, WT>(hg, swz) : pick_hg<64, 2, WT>(hg, swz); return true;
+    case 128: *out = nt1 ? pick_hg<128, 1, WT>(hg, swz) : pick_hg<128, 2, WT>(hg, swz); return true;
+    default: return false;
+  }
+}
+
+// The instances that keep their scores (pad_decode_weights.cu).
+bool pick_decode_weights(int64_t head_dim, int64_t gqa, int hg, bool swz, Instance* out);
+
+}  // namespace pad

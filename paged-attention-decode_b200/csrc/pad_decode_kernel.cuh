@@ -28,6 +28,7 @@
 #include <cstdint>
 
 #include "pad_ptx.cuh"
+#include "pad_track.cuh"
 
 namespace pad {
 
@@ -65,11 +66,13 @@ struct __align__(64) DecodeParams {
   int meta_by_pair;  // merge descriptors indexed by pair (else by partition)
   int l2_warm;       // guessed first tiles prefetched into L2 before the dependency wait (0: none)
   float scale_log2;  // scale * log2(e)
+  TrackParams track; // used by the instances that keep scores (Traits::WT)
 };
 
 // Compile-time shape of one kernel instance.
-template <int D_, int NT_, int HG_, bool SWZ_>
+template <int D_, int NT_, int HG_, bool SWZ_, bool WT_ = false>
 struct Traits {
+  static constexpr bool WT = WT_;           // keeps the scores for the attention weights
   static constexpr int D = D_;
   static constexpr int NT = NT_;            // n8 tiles of query rows: G <= 8*NT
   static constexpr int HG = HG_;            // KV heads per tile

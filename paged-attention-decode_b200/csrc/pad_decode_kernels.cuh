@@ -337,6 +337,9 @@ __global__ void __launch_bounds__(kThreads, 1) decode_stream_kernel(const __grid
     }
     const int ntiles = t1 - t0;
     if (lane == 0 && !p.meta_by_pair) p.ws_meta[w] = make_int4(-1, 0, 0, 0);
+    if constexpr (TR::WT) {
+      if (lane == 0 && w == 0) *p.track.total = total;
+    }
     if (lane == 0) PAD_STAMP(7);
     if (ntiles <= 0) {
       // An empty partition (more partitions than tiles) can sit between the
@@ -448,6 +451,14 @@ __global__ void __launch_bounds__(kThreads, 1) decode_stream_kernel(const __grid
           const int last_owner = part_owner((int64_t)c.pair_start + c.n - 1, total, W);
           p.ws_meta[p.meta_by_pair ? pair : w] =
               split ? make_int4(pair, pair + w, last_owner - w + 1, 1) : make_int4(-1, 0, 0, 0);
+        }
+        if constexpr (TR::WT) {
+          if (t0 + k < p.track.raw_tiles) p.track.tiles[t0 + k] = make_int4(c.b, c.hg, c.i, c.seq);
+          else raise_flag(p, PAD_FLAG_SHARED_PAGE);
+          if (c.i == 0) {
+            const int owner = split ? part_owner((int64_t)c.pair_start + c.n - 1, total, W) : w;
+            p.track.pairs[pair] = make_int2(pair + w, owner - w + 1);
+          }
         }
       }
       if (k == 0 && lane == 0) PAD_STAMP(2);
@@ -686,6 +697,23 @@ __global__ void __launch_bounds__(kThreads, 1) decode_stream_kernel(const __grid
         sc[nt][2] = v_hi ? sc[nt][2] * p.scale_log2 : -INFINITY;
         sc[nt][3] = v_hi ? sc[nt][3] * p.scale_log2 : -INFINITY;
       }
+      if constexpr (TR::WT) {
+        // the scores go to the kernel that turns them into attention weights
+        // once every (m, l) is known: [tile][head row][token]
+        if (t0 + k < p.track.raw_tiles) {
+          float* raw = p.track.raw + (int64_t)(t0 + k) * (HG * G * TT) + hl * G * TT + t_base + (lane >> 2);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int g = nt * 8 + gl + j;
+              if (g < G) {
+                raw[g * TT] = sc[nt][j];
+                raw[g * TT + 8] = sc[nt][j + 2];
+              }
+            }
+        }
+      }
       // online softmax (per query row, over this warp's tokens)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -772,7 +800,7 @@ __global__ void __launch_bounds__(kThreads, 1) decode_stream_kernel(const __grid
             if (g >= G) continue;
             const float L = lsum[nt][j];
             const float inv = L > 0.f ? 1.f / L : 0.f;
-            if (split && (lane >> 2) == 0) p.ws_ml[prow + g] = make_float2(m_run[nt][j], L);
+            if ((split || TR::WT) && (lane >> 2) == 0) p.ws_ml[prow + g] = make_float2(m_run[nt][j], L);
 #pragma unroll
             for (int mt = 0; mt < KSTEPS; ++mt)
 #pragma unroll
@@ -882,9 +910,10 @@ __global__ void __launch_bounds__(kThreads, 1) decode_stream_kernel(const __grid
             }
             o4[x] = v;
           }
+        }
+        if (split || TR::WT)
           for (int x = ctid; x < HG * G; x += 32 * kConsumerWarps)
             p.ws_ml[(int64_t)dsc.slot * HG * G + x] = sML[(x / G) * 8 * NT + x % G];
-        }
         // No trailing sync: the next epilogue's first sync orders these reads
         // before any warp writes the buffer again.
       }

@@ -257,6 +257,64 @@ void check_slots(const at::Tensor& t, at::ScalarType type, int64_t pages, int64_
               "libpad_b200 ", what, ": weights (fp32) and slot_positions (int32) must be [pages, Hkv, page_size]");
 }
 
+// What a decode with attention weights takes beside the decode's arguments.
+struct Tracked {
+  at::Tensor total;
+  Strides ws, ps;
+  Tracked(const at::Tensor& weights, const c10::optional<at::Tensor>& positions,
+          const c10::optional<at::Tensor>& total_in, int64_t num_new, int64_t pages, int64_t hkv, int64_t page_size,
+          int64_t batch, const at::Device& dev, const char* what)
+      : ws(weights), ps(positions.has_value() ? *positions : weights) {
+    check_slots(weights, at::kFloat, pages, hkv, page_size, what);
+    check_on(dev, {&weights}, what);
+    TORCH_CHECK(num_new >= 0, "libpad_b200 ", what, ": num_new must not be negative");
+    TORCH_CHECK(positions.has_value() == total_in.has_value(), "libpad_b200 ", what,
+                ": slot_positions and total_lens go together");
+    if (positions.has_value()) {
+      check_slots(*positions, at::kInt, pages, hkv, page_size, what);
+      check_on(dev, {&*positions}, what);
+      TORCH_CHECK(total_in->dim() == 1 && total_in->size(0) == batch, "libpad_b200 ", what,
+                  ": total_lens must be [B]");
+      total = as_int32_rows(*total_in, dev);
+    }
+  }
+  const int32_t* total_ptr() const { return total.defined() ? total.data_ptr<int32_t>() : nullptr; }
+};
+
+// Decode, and the attention weights of the cached tokens. The workspace, tens
+// of times the decode's own, is the call's: two captured graphs never share one.
+at::Tensor decode_weights(const at::Tensor& q_in, const at::Tensor& k, const at::Tensor& v, const at::Tensor& bt_in,
+                          const at::Tensor& sl_in, int64_t num_splits, double scale,
+                          const c10::optional<at::Tensor>& out_in, const at::Tensor& weights, int64_t num_new,
+                          const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& total_in) {
+  TORCH_CHECK(q_in.dim() == 3 && k.dim() == 4 && v.sizes() == k.sizes(), "bad q / k_cache / v_cache shapes");
+  const at::Device dev = q_in.device();
+  check_on(dev, {&k, &v}, "decode_weights");
+  c10::cuda::CUDAGuard guard(dev);
+  const int64_t batch = q_in.size(0), hq = q_in.size(1), d = q_in.size(2), pages = k.size(0), ps = k.size(1),
+                hkv = k.size(2);
+  const Tracked tr(weights, positions, total_in, num_new, pages, hkv, ps, batch, dev, "decode_weights");
+  const at::Tensor q = tma_ready(q_in);
+  const at::Tensor bt = as_int32_rows(bt_in, dev), sl = as_int32_rows(sl_in, dev);
+  at::Tensor out = prepare_out(out_in, q_in);
+  if (batch == 0) return out;
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  StreamState& st = state_for(dev, stream);
+  const Strides qs(q), ks(k), vs(v), os(out);
+  size_t bytes = 0;
+  check(pad_decode_weights_workspace_bytes((int)dev.index(), batch, hkv, hq / hkv, d, pages, ps, bt.size(1),
+                                           num_splits, &bytes),
+        "workspace size");
+  const at::Tensor ws = at::empty({(int64_t)bytes}, st.flags.options().dtype(at::kByte));
+  check(pad_paged_attention_decode_weights(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), bt.data_ptr<int32_t>(), sl.data_ptr<int32_t>(), out.data_ptr(),
+            weights.data_ptr<float>(), positions.has_value() ? positions->data_ptr<int32_t>() : nullptr,
+            tr.total_ptr(), num_new, batch, hq, hkv, d, pages, ps, bt.size(1), qs.s, ks.s, vs.s, bt.stride(0), os.s,
+            tr.ws.s, tr.ps.s, (float)scale, num_splits, ws.data_ptr(), bytes, stream, st.flags.data_ptr<int32_t>()),
+        "decode_weights");
+  return out;
+}
+
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> kv_evict_plan(
     const at::Tensor& weights, const at::Tensor& bt_in, const at::Tensor& sl_in, int64_t budget, int64_t recent,
     const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& total_in) {
@@ -360,6 +418,9 @@ TORCH_LIBRARY(pad_b200, m) {
         "Tensor kv_last_page_len, int num_splits, float scale, Tensor(a!)? out) -> Tensor");
   m.def("kv_append(Tensor k_new, Tensor v_new, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor block_table, "
         "Tensor positions) -> ()");
+  m.def("decode_weights(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, int num_splits, "
+        "float scale, Tensor(a!)? out, Tensor(b!) weights, int num_new, Tensor(c!)? slot_positions, "
+        "Tensor? total_lens) -> Tensor");
   m.def("kv_append_fp4(Tensor k_new, Tensor v_new, Tensor(a!) k_cache, Tensor(b!) k_scales, Tensor(c!) v_cache, "
         "Tensor(d!) v_scales, Tensor block_table, Tensor positions, Tensor? seq_ids) -> ()");
   m.def("kv_read_fp4(Tensor k_cache, Tensor k_scales, Tensor v_cache, Tensor v_scales, Tensor block_table, "
@@ -375,6 +436,7 @@ TORCH_LIBRARY_IMPL(pad_b200, CUDA, m) {
   m.impl("decode", &decode);
   m.impl("decode_csr", &decode_csr);
   m.impl("kv_append", &kv_append);
+  m.impl("decode_weights", &decode_weights);
   m.impl("kv_append_fp4", &kv_append_fp4);
   m.impl("kv_read_fp4", &kv_read_fp4);
   m.impl("kv_evict_plan", &kv_evict_plan);

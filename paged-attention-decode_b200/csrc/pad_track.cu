@@ -1,0 +1,27 @@
+// pad_track.cu -- the launch of the attention-weight kernel (pad_track.cuh).
+#include <algorithm>
+
+#include "pad_error.cuh"
+#include "pad_track.cuh"
+#include "pad_track_kernel.cuh"
+
+namespace pad {
+
+int launch_weights(const WeightParams& p, cudaStream_t stream) {
+  if (p.track.raw_tiles == 0) return PAD_OK;
+  WeightParams prm = p;
+  void* args[] = {&prm};
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)std::min(p.track.raw_tiles, kWeightGrid));
+  cfg.blockDim = dim3(kWeightThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // overlap its launch with the kernel before
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(&weights_kernel), args);
+  return e == cudaSuccess ? PAD_OK : cuda_fail(e, "launching the attention-weight kernel");
+}
+
+}  // namespace pad

@@ -26,6 +26,7 @@ PAD_ERR_CUDA = 4
 PAD_FLAG_BAD_PAGE_ID = 0x1
 PAD_FLAG_SEQ_LEN_RANGE = 0x2
 PAD_FLAG_BAD_SEQ_ID = 0x4
+PAD_FLAG_SHARED_PAGE = 0x8
 PAD_FLAG_WAIT_TIMEOUT = 0x100
 
 # (name, restype, argtypes) for every symbol the header declares
@@ -47,6 +48,11 @@ SIGNATURES = {
     "pad_paged_kv_append": (ctypes.c_int, [_vp] * 6 + [_c_i64] * 6 + [_c_i64p] * 4 + [_c_i64, _vp, _vp]),
     "pad_paged_kv_append_fp4": (ctypes.c_int, [_vp] * 9 + [_c_i64] * 7 + [_c_i64p] * 6 + [_c_i64, _vp, _vp]),
     "pad_paged_kv_read_fp4": (ctypes.c_int, [_vp] * 9 + [_c_i64] * 7 + [_c_i64p] * 6 + [_c_i64, _vp, _vp]),
+    "pad_decode_weights_workspace_bytes": (ctypes.c_int, [ctypes.c_int] + [_c_i64] * 8
+                                           + [ctypes.POINTER(ctypes.c_size_t)]),
+    "pad_paged_attention_decode_weights": (ctypes.c_int, [_vp] * 9 + [_c_i64] * 8
+                                           + [_c_i64p, _c_i64p, _c_i64p, _c_i64, _c_i64p, _c_i64p, _c_i64p,
+                                              ctypes.c_float, _c_i64, _vp, ctypes.c_size_t, _vp, _vp]),
     "pad_evict_max_moves": (ctypes.c_int, [_c_i64] * 3 + [_c_i64p]),
     "pad_paged_kv_evict_plan": (ctypes.c_int, [_vp] * 9 + [_c_i64] * 7 + [_c_i64p] * 2 + [_c_i64, _vp, _vp]),
     "pad_paged_kv_move": (ctypes.c_int, [_c_i64, ctypes.POINTER(_vp), _c_i64p, _c_i64p] + [_vp] * 6 + [_c_i64] * 6

@@ -23,7 +23,8 @@ INCLUDE = os.path.join(REPO, "include")
 LIB_NAME = "libpad_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 OPS_PATH = os.path.join(HERE, "_pad_torch_ops.so")
-SOURCES = ["pad_decode.cu", "pad_kv_append.cu", "pad_kv_fp4.cu", "pad_evict.cu"]
+OBJ_DIR = os.path.join(PKG_ROOT, "_build")
+SOURCES = ["pad_decode.cu", "pad_decode_weights.cu", "pad_track.cu", "pad_kv_append.cu", "pad_kv_fp4.cu", "pad_evict.cu"]
 OPS_SOURCE = "pad_torch_op.cpp"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -70,12 +71,26 @@ def _build_ops() -> None:
 
 def build(force: bool = False, verbose: bool = False) -> str:
     if force or _stale(LIB_PATH, _inputs()):
-        cmd = [_nvcc(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2",
-               "-shared", "-I", INCLUDE, "-o", LIB_PATH + ".tmp"]
-        if verbose:
-            cmd += ["-Xptxas", "-v"]
-        cmd += [os.path.join(CSRC, s) for s in SOURCES]
-        subprocess.run(cmd, check=True, cwd=CSRC)
+        # one nvcc per source, side by side; sources newer than their object
+        # (or any header newer than it) are compiled again
+        headers = [f for f in _inputs() if not f.endswith(".cu")]
+        os.makedirs(OBJ_DIR, exist_ok=True)
+        objs, running = [], []
+        for src in SOURCES:
+            obj = os.path.join(OBJ_DIR, src + ".o")
+            objs.append(obj)
+            if not force and not verbose and not _stale(obj, [os.path.join(CSRC, src), *headers]):
+                continue
+            cmd = [_nvcc(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "-I", INCLUDE,
+                   *(["-Xptxas", "-v"] if verbose else []), "-c", os.path.join(CSRC, src), "-o", obj + ".tmp"]
+            running.append((obj, subprocess.Popen(cmd, cwd=CSRC)))
+        failed = [obj for obj, p in running if p.wait() != 0]
+        if failed:
+            raise RuntimeError(f"nvcc failed for {', '.join(os.path.basename(f) for f in failed)}")
+        for obj, _ in running:
+            os.replace(obj + ".tmp", obj)
+        subprocess.run([_nvcc(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", LIB_PATH + ".tmp", *objs],
+                       check=True, cwd=CSRC)
         os.replace(LIB_PATH + ".tmp", LIB_PATH)
     if force or _stale(OPS_PATH, [os.path.join(CSRC, OPS_SOURCE), LIB_PATH]):
         _build_ops()

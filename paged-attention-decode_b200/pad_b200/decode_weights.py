@@ -1,0 +1,64 @@
+"""Decode that also accumulates each cached token's attention weight -- what an
+eviction (pad_b200.evict) decides by. The reference has no counterpart."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+from .kernel_cuda_v4 import _SUPPORTED_HEAD_DIMS, _check_values, _raise_if_checking
+
+_OPS = _lib.ops()
+
+
+def paged_attention_decode_weights(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    weights: torch.Tensor,
+    num_new: int = 1,
+    num_splits: int | None = None,
+    scale: float | None = None,
+    *,
+    slot_positions: torch.Tensor | None = None,
+    total_lens: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """paged_attention_decode_cuda_v4, and ``weights`` updated in place.
+
+    weights [num_pages, Hkv, page_size] fp32 gains, for every cached token and
+    KV head, the token's softmax probability summed over the KV head's query
+    heads. The num_new last tokens of each sequence are new: their weight is
+    set, not added to, so a page's slots need no clearing before they are used
+    (num_new = 0 only adds). slot_positions [num_pages, Hkv, page_size] int32,
+    if given, gets the new tokens' positions, counted from total_lens [B] (the
+    tokens each sequence has seen; None: seq_lens, as before any eviction).
+    Sequences must not share pages."""
+    assert q.is_cuda and k_cache.is_cuda and v_cache.is_cuda, "pad_b200 requires CUDA tensors"
+    assert q.dtype == torch.float16 and k_cache.dtype == torch.float16 and v_cache.dtype == torch.float16, (
+        "pad_b200 expects fp16 q/k_cache/v_cache"
+    )
+    assert q.dim() == 3 and k_cache.dim() == 4, "q must be [B, Hq, D] and k_cache [num_pages, page_size, Hkv, D]"
+    assert v_cache.shape == k_cache.shape, "v_cache must have k_cache's shape"
+    batch, num_q_heads, head_dim = q.shape
+    num_pages, page_size, num_kv_heads, cache_head_dim = k_cache.shape
+    assert cache_head_dim == head_dim, "q head_dim must match the KV cache head_dim"
+    assert num_q_heads % num_kv_heads == 0, "num_q_heads must be divisible by num_kv_heads (GQA)"
+    assert head_dim in _SUPPORTED_HEAD_DIMS, f"head_dim must be one of {_SUPPORTED_HEAD_DIMS}"
+    assert block_table.dim() == 2 and block_table.shape[0] == batch, "block_table must be [B, max_pages]"
+    assert seq_lens.dim() == 1 and seq_lens.shape[0] == batch, "seq_lens must be [B]"
+    assert num_splits is None or num_splits >= 1, "num_splits must be >= 1"
+    assert num_new >= 0, "num_new must be >= 0"
+    assert slot_positions is not None or total_lens is None, "total_lens goes with slot_positions"
+    if slot_positions is not None and total_lens is None:
+        total_lens = seq_lens
+    _check_values(q.device)
+    out = _OPS.decode_weights(q, k_cache, v_cache, block_table, seq_lens, 0 if num_splits is None else int(num_splits),
+                              float(scale) if scale is not None else 1.0 / math.sqrt(head_dim), out, weights,
+                              int(num_new), slot_positions, total_lens)
+    _raise_if_checking(q.device)
+    return out
