@@ -237,6 +237,31 @@ int pad_paged_kv_read_fp4(const void* k_cache, const void* k_scales, const void*
                           const int64_t* k_out_strides, const int64_t* v_out_strides, int64_t block_table_stride,
                           void* stream, int32_t* error_flags);
 
+/* Decode attention over the 4-bit cache: pad_paged_attention_decode with K and
+ * V what their codes and scales stand for (scales up to 2^15; above, values
+ * leave fp16's range and become infinite, and a NaN scale makes the sequences
+ * that attend to it NaN). head_dim 32, 64 or 128, gqa_ratio up to 16. q must be
+ * 16-byte aligned with strides that are multiples of 8 elements, out 4-byte
+ * aligned with even strides. weights, slot_positions, total_lens and num_new
+ * are those of pad_paged_attention_decode_weights below; weights NULL leaves
+ * them out. num_splits >= 1: partitions per (sequence, KV head group), as for
+ * the decode. The workspace (pad_decode_fp4_workspace_bytes; with_weights 0 or
+ * 1; num_pages matters with weights alone) needs no initialisation. A bad page
+ * id reads as zero rows. */
+int pad_decode_fp4_workspace_bytes(int device, int64_t batch, int64_t num_kv_heads, int64_t gqa_ratio,
+                                   int64_t head_dim, int64_t num_pages, int64_t page_size,
+                                   int64_t max_pages_per_seq, int64_t num_splits, int with_weights, size_t* bytes);
+int pad_paged_attention_decode_fp4(const void* q, const void* k_cache, const void* k_scales, const void* v_cache,
+                                   const void* v_scales, const int32_t* block_table, const int32_t* seq_lens,
+                                   void* out, float* weights, int32_t* slot_positions, const int32_t* total_lens,
+                                   int64_t num_new, int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+                                   int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages_per_seq,
+                                   const int64_t* q_strides, const int64_t* k_strides, const int64_t* ks_strides,
+                                   const int64_t* v_strides, const int64_t* vs_strides, int64_t block_table_stride,
+                                   const int64_t* out_strides, const int64_t* weight_strides,
+                                   const int64_t* position_strides, float scale, int64_t num_splits, void* workspace,
+                                   size_t workspace_bytes, void* stream, int32_t* error_flags);
+
 /* ---------------------------------------------------------------------------
  * Eviction by accumulated attention weight. Beside a paged cache live
  *   weights         [num_pages, num_kv_heads, page_size]  fp32

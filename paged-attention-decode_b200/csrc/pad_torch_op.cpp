@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cstdint>
 #include <initializer_list>
 #include <map>
@@ -176,12 +177,27 @@ void kv_append(const at::Tensor& k_new_in, const at::Tensor& v_new_in, const at:
         "kv_append");
 }
 
-struct Strides {  // of a tensor's first axes, as the C entry points take them
+// A tensor's strides as the C entry points take them. The stride of an axis of
+// one element means nothing (torch keeps any number there): it becomes what a
+// dense tensor would have.
+struct Strides {
   int64_t s[4] = {0, 0, 0, 0};
   explicit Strides(const at::Tensor& t) {
-    for (int64_t i = 0; i < t.dim() && i < 4; ++i) s[i] = t.stride(i);
+    int64_t dense = 1;
+    for (int64_t i = std::min<int64_t>(t.dim(), 4) - 1; i >= 0; --i) {
+      s[i] = t.size(i) == 1 ? dense : t.stride(i);
+      dense = s[i] * std::max<int64_t>(t.size(i), 1);
+    }
   }
 };
+
+// q as the kernels read it: rows of 16-byte pieces (a copy where it is not).
+at::Tensor aligned_rows(const at::Tensor& q) {
+  const Strides st(q);
+  const bool ok = st.s[2] == 1 && st.s[0] % 8 == 0 && st.s[1] % 8 == 0 && st.s[0] > 0 && st.s[1] > 0 &&
+                  reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0;
+  return ok ? q : q.clone(at::MemoryFormat::Contiguous);
+}
 
 void check_on(const at::Device& dev, std::initializer_list<const at::Tensor*> all, const char* what) {
   for (const at::Tensor* t : all)
@@ -212,8 +228,8 @@ void kv_append_fp4(const at::Tensor& k_new, const at::Tensor& v_new, const at::T
   c10::cuda::CUDAGuard guard(dev);
   const at::Tensor bt = as_int32_rows(bt_in, dev), pos = as_int32_rows(pos_in, dev);
   const at::Tensor ids = ids_in.has_value() ? as_int32_rows(*ids_in, dev) : at::Tensor();
-  const at::Tensor kn = k_new.stride(2) == 1 ? k_new : k_new.contiguous();
-  const at::Tensor vn = v_new.stride(2) == 1 ? v_new : v_new.contiguous();
+  const at::Tensor kn = Strides(k_new).s[2] == 1 ? k_new : k_new.contiguous();
+  const at::Tensor vn = Strides(v_new).s[2] == 1 ? v_new : v_new.contiguous();
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   StreamState& st = state_for(dev, stream);
   const Strides kns(kn), vns(vn), k_s(k), ks_s(ks), v_s(v), vs_s(vs);
@@ -221,7 +237,7 @@ void kv_append_fp4(const at::Tensor& k_new, const at::Tensor& v_new, const at::T
                                 bt.data_ptr<int32_t>(), pos.data_ptr<int32_t>(),
                                 ids.defined() ? ids.data_ptr<int32_t>() : nullptr, kn.size(0), bt.size(0), kn.size(1),
                                 kn.size(2), k.size(0), k.size(1), bt.size(1), kns.s, vns.s, k_s.s, ks_s.s, v_s.s,
-                                vs_s.s, bt.stride(0), stream, st.flags.data_ptr<int32_t>()),
+                                vs_s.s, Strides(bt).s[0], stream, st.flags.data_ptr<int32_t>()),
         "kv_append_fp4");
 }
 
@@ -245,7 +261,7 @@ std::tuple<at::Tensor, at::Tensor> kv_read_fp4(const at::Tensor& k, const at::Te
   check(pad_paged_kv_read_fp4(k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), bt.data_ptr<int32_t>(),
                               pos.data_ptr<int32_t>(), ids.defined() ? ids.data_ptr<int32_t>() : nullptr,
                               ko.data_ptr(), vo.data_ptr(), tokens, bt.size(0), hkv, d, k.size(0), k.size(1),
-                              bt.size(1), k_s.s, ks_s.s, v_s.s, vs_s.s, kos.s, vos.s, bt.stride(0), stream,
+                              bt.size(1), k_s.s, ks_s.s, v_s.s, vs_s.s, kos.s, vos.s, Strides(bt).s[0], stream,
                               st.flags.data_ptr<int32_t>()),
         "kv_read_fp4");
   return {ko, vo};
@@ -294,7 +310,7 @@ at::Tensor decode_weights(const at::Tensor& q_in, const at::Tensor& k, const at:
   const int64_t batch = q_in.size(0), hq = q_in.size(1), d = q_in.size(2), pages = k.size(0), ps = k.size(1),
                 hkv = k.size(2);
   const Tracked tr(weights, positions, total_in, num_new, pages, hkv, ps, batch, dev, "decode_weights");
-  const at::Tensor q = tma_ready(q_in);
+  const at::Tensor q = aligned_rows(q_in);
   const at::Tensor bt = as_int32_rows(bt_in, dev), sl = as_int32_rows(sl_in, dev);
   at::Tensor out = prepare_out(out_in, q_in);
   if (batch == 0) return out;
@@ -309,9 +325,50 @@ at::Tensor decode_weights(const at::Tensor& q_in, const at::Tensor& k, const at:
   check(pad_paged_attention_decode_weights(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), bt.data_ptr<int32_t>(), sl.data_ptr<int32_t>(), out.data_ptr(),
             weights.data_ptr<float>(), positions.has_value() ? positions->data_ptr<int32_t>() : nullptr,
-            tr.total_ptr(), num_new, batch, hq, hkv, d, pages, ps, bt.size(1), qs.s, ks.s, vs.s, bt.stride(0), os.s,
+            tr.total_ptr(), num_new, batch, hq, hkv, d, pages, ps, bt.size(1), qs.s, ks.s, vs.s, Strides(bt).s[0], os.s,
             tr.ws.s, tr.ps.s, (float)scale, num_splits, ws.data_ptr(), bytes, stream, st.flags.data_ptr<int32_t>()),
         "decode_weights");
+  return out;
+}
+
+at::Tensor decode_fp4(const at::Tensor& q_in, const at::Tensor& k, const at::Tensor& ks, const at::Tensor& v,
+                      const at::Tensor& vs, const at::Tensor& bt_in, const at::Tensor& sl_in, int64_t num_splits,
+                      double scale, const c10::optional<at::Tensor>& out_in, const c10::optional<at::Tensor>& weights,
+                      int64_t num_new, const c10::optional<at::Tensor>& positions,
+                      const c10::optional<at::Tensor>& total_in) {
+  const at::Device dev = q_in.device();
+  check_fp4(k, ks, v, vs, "decode_fp4");
+  check_on(dev, {&k, &ks, &v, &vs}, "decode_fp4");
+  TORCH_CHECK(q_in.dim() == 3 && q_in.scalar_type() == at::kHalf && q_in.size(2) == 2 * k.size(3),
+              "libpad_b200 decode_fp4: q must be fp16 [B, Hq, D] of the cache's head_dim");
+  TORCH_CHECK(bt_in.dim() == 2 && bt_in.size(0) == q_in.size(0) && sl_in.dim() == 1 && sl_in.size(0) == q_in.size(0),
+              "libpad_b200 decode_fp4: block_table must be [B, max_pages], seq_lens [B]");
+  TORCH_CHECK(weights.has_value() || !positions.has_value(), "libpad_b200 decode_fp4: slot_positions need weights");
+  c10::cuda::CUDAGuard guard(dev);
+  const int64_t batch = q_in.size(0), hq = q_in.size(1), d = q_in.size(2), pages = k.size(0), ps = k.size(1),
+                hkv = k.size(2);
+  c10::optional<Tracked> tr;
+  if (weights.has_value()) tr.emplace(*weights, positions, total_in, num_new, pages, hkv, ps, batch, dev, "decode_fp4");
+  const at::Tensor q = aligned_rows(q_in);
+  const at::Tensor bt = as_int32_rows(bt_in, dev), sl = as_int32_rows(sl_in, dev);
+  at::Tensor out = prepare_out(out_in, q_in);
+  if (batch == 0) return out;
+  cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  StreamState& st = state_for(dev, stream);
+  const Strides qs(q), k_s(k), ks_s(ks), v_s(v), vs_s(vs), os(out);
+  size_t bytes = 0;
+  check(pad_decode_fp4_workspace_bytes((int)dev.index(), batch, hkv, hq / hkv, d, pages, ps, bt.size(1), num_splits,
+                                       weights.has_value() ? 1 : 0, &bytes),
+        "workspace size");
+  const at::Tensor ws = at::empty({(int64_t)bytes}, k.options());
+  check(pad_paged_attention_decode_fp4(
+            q.data_ptr(), k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), bt.data_ptr<int32_t>(),
+            sl.data_ptr<int32_t>(), out.data_ptr(), tr ? weights->data_ptr<float>() : nullptr,
+            positions.has_value() ? positions->data_ptr<int32_t>() : nullptr, tr ? tr->total_ptr() : nullptr, num_new,
+            batch, hq, hkv, d, pages, ps, bt.size(1), qs.s, k_s.s, ks_s.s, v_s.s, vs_s.s, Strides(bt).s[0], os.s,
+            tr ? tr->ws.s : nullptr, tr ? tr->ps.s : nullptr, (float)scale, num_splits, ws.data_ptr(), bytes, stream,
+            st.flags.data_ptr<int32_t>()),
+        "decode_fp4");
   return out;
 }
 
@@ -346,7 +403,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> kv_evict_plan(
                                 bt.data_ptr<int32_t>(), sl.data_ptr<int32_t>(),
                                 total.defined() ? total.data_ptr<int32_t>() : nullptr, src.data_ptr<int32_t>(),
                                 dst.data_ptr<int32_t>(), counts.data_ptr<int32_t>(), lens.data_ptr<int32_t>(), batch,
-                                hkv, pages, ps, bt.size(1), budget, recent, ws.s, pst.s, bt.stride(0), stream,
+                                hkv, pages, ps, bt.size(1), budget, recent, ws.s, pst.s, Strides(bt).s[0], stream,
                                 st.flags.data_ptr<int32_t>()),
         "kv_evict_plan");
   return {src, dst, counts, lens};
@@ -364,13 +421,14 @@ void kv_move(at::TensorList caches, const at::Tensor& bt_in, const at::Tensor& s
   int64_t bytes[4], strides[12];
   for (size_t c = 0; c < caches.size(); ++c) {
     const at::Tensor& t = caches[c];
-    TORCH_CHECK(t.dim() == 4 && t.size(0) == pages && t.size(1) == ps && t.size(2) == hkv && t.stride(3) == 1,
+    TORCH_CHECK(t.dim() == 4 && t.size(0) == pages && t.size(1) == ps && t.size(2) == hkv && Strides(t).s[3] == 1,
                 "libpad_b200 kv_move: caches must be [pages, page_size, Hkv, row] with a contiguous row");
     check_on(dev, {&t}, "kv_move");
     const int64_t item = t.element_size();
     ptr[c] = t.data_ptr();
     bytes[c] = t.size(3) * item;
-    for (int i = 0; i < 3; ++i) strides[3 * c + i] = t.stride(i) * item;
+    const Strides st(t);
+    for (int i = 0; i < 3; ++i) strides[3 * c + i] = st.s[i] * item;
   }
   TORCH_CHECK(bt_in.dim() == 2 && src.dim() == 3 && src.size(0) == batch && src.size(1) == hkv &&
                   dst.sizes() == src.sizes() && counts.dim() == 2 && counts.size(0) == batch &&
@@ -397,7 +455,7 @@ void kv_move(at::TensorList caches, const at::Tensor& bt_in, const at::Tensor& s
                           dst.data_ptr<int32_t>(), counts.data_ptr<int32_t>(),
                           weights.has_value() ? weights->data_ptr<float>() : nullptr,
                           positions.has_value() ? positions->data_ptr<int32_t>() : nullptr, batch, hkv, pages, ps,
-                          bt.size(1), src.size(2), ws.s, pst.s, bt.stride(0), stream, st.flags.data_ptr<int32_t>()),
+                          bt.size(1), src.size(2), ws.s, pst.s, Strides(bt).s[0], stream, st.flags.data_ptr<int32_t>()),
         "kv_move");
 }
 
@@ -421,6 +479,9 @@ TORCH_LIBRARY(pad_b200, m) {
   m.def("decode_weights(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, int num_splits, "
         "float scale, Tensor(a!)? out, Tensor(b!) weights, int num_new, Tensor(c!)? slot_positions, "
         "Tensor? total_lens) -> Tensor");
+  m.def("decode_fp4(Tensor q, Tensor k_cache, Tensor k_scales, Tensor v_cache, Tensor v_scales, Tensor block_table, "
+        "Tensor seq_lens, int num_splits, float scale, Tensor(a!)? out, Tensor(b!)? weights, int num_new, "
+        "Tensor(c!)? slot_positions, Tensor? total_lens) -> Tensor");
   m.def("kv_append_fp4(Tensor k_new, Tensor v_new, Tensor(a!) k_cache, Tensor(b!) k_scales, Tensor(c!) v_cache, "
         "Tensor(d!) v_scales, Tensor block_table, Tensor positions, Tensor? seq_ids) -> ()");
   m.def("kv_read_fp4(Tensor k_cache, Tensor k_scales, Tensor v_cache, Tensor v_scales, Tensor block_table, "
@@ -437,6 +498,7 @@ TORCH_LIBRARY_IMPL(pad_b200, CUDA, m) {
   m.impl("decode_csr", &decode_csr);
   m.impl("kv_append", &kv_append);
   m.impl("decode_weights", &decode_weights);
+  m.impl("decode_fp4", &decode_fp4);
   m.impl("kv_append_fp4", &kv_append_fp4);
   m.impl("kv_read_fp4", &kv_read_fp4);
   m.impl("kv_evict_plan", &kv_evict_plan);

@@ -14,7 +14,7 @@ from .kernel_cuda_v4 import (paged_attention_decode_csr, paged_attention_decode_
                              partitions, read_error_flags, workspace_bytes)
 from .decode_weights import paged_attention_decode_weights  # noqa: F401
 from .evict import paged_kv_evict, paged_kv_evict_plan, paged_kv_move  # noqa: F401
-from .kv_fp4 import paged_kv_append_fp4, paged_kv_cache_fp4, paged_kv_read_fp4  # noqa: F401
+from .kv_fp4 import paged_attention_decode_fp4, paged_kv_append_fp4, paged_kv_cache_fp4, paged_kv_read_fp4  # noqa: F401
 from ._lib import PadError  # noqa: F401
 
 
@@ -41,5 +41,5 @@ def paged_attention_decode_v4(q, k_cache, v_cache, block_table, seq_lens, num_sp
 __all__ = ["paged_attention_decode_cuda_v4", "paged_attention_decode_v4", "paged_attention_decode_csr",
            "paged_kv_indices", "paged_kv_append", "partitions", "workspace_bytes",
            "read_error_flags", "paged_attention_decode_weights", "paged_kv_cache_fp4", "paged_kv_append_fp4",
-           "paged_kv_read_fp4",
+           "paged_kv_read_fp4", "paged_attention_decode_fp4",
            "paged_kv_evict_plan", "paged_kv_move", "paged_kv_evict", "PadError"]

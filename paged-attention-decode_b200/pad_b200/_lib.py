@@ -48,6 +48,11 @@ SIGNATURES = {
     "pad_paged_kv_append": (ctypes.c_int, [_vp] * 6 + [_c_i64] * 6 + [_c_i64p] * 4 + [_c_i64, _vp, _vp]),
     "pad_paged_kv_append_fp4": (ctypes.c_int, [_vp] * 9 + [_c_i64] * 7 + [_c_i64p] * 6 + [_c_i64, _vp, _vp]),
     "pad_paged_kv_read_fp4": (ctypes.c_int, [_vp] * 9 + [_c_i64] * 7 + [_c_i64p] * 6 + [_c_i64, _vp, _vp]),
+    "pad_decode_fp4_workspace_bytes": (ctypes.c_int, [ctypes.c_int] + [_c_i64] * 8
+                                       + [ctypes.c_int, ctypes.POINTER(ctypes.c_size_t)]),
+    "pad_paged_attention_decode_fp4": (ctypes.c_int, [_vp] * 11 + [_c_i64] * 8
+                                       + [_c_i64p] * 5 + [_c_i64] + [_c_i64p] * 3
+                                       + [ctypes.c_float, _c_i64, _vp, ctypes.c_size_t, _vp, _vp]),
     "pad_decode_weights_workspace_bytes": (ctypes.c_int, [ctypes.c_int] + [_c_i64] * 8
                                            + [ctypes.POINTER(ctypes.c_size_t)]),
     "pad_paged_attention_decode_weights": (ctypes.c_int, [_vp] * 9 + [_c_i64] * 8

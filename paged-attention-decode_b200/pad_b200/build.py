@@ -24,7 +24,8 @@ LIB_NAME = "libpad_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 OPS_PATH = os.path.join(HERE, "_pad_torch_ops.so")
 OBJ_DIR = os.path.join(PKG_ROOT, "_build")
-SOURCES = ["pad_decode.cu", "pad_decode_weights.cu", "pad_track.cu", "pad_kv_append.cu", "pad_kv_fp4.cu", "pad_evict.cu"]
+SOURCES = ["pad_decode.cu", "pad_decode_weights.cu", "pad_decode_fp4.cu", "pad_track.cu", "pad_kv_append.cu",
+           "pad_kv_fp4.cu", "pad_evict.cu"]
 OPS_SOURCE = "pad_torch_op.cpp"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -14,6 +14,8 @@ The reference has no counterpart.
 
 from __future__ import annotations
 
+import math
+
 import torch
 
 from . import _lib
@@ -65,3 +67,46 @@ def paged_kv_read_fp4(k_cache: torch.Tensor, k_scales: torch.Tensor, v_cache: to
     got = _OPS.kv_read_fp4(k_cache, k_scales, v_cache, v_scales, block_table, positions, seq_ids)
     _raise_if_checking(k_cache.device)
     return got
+
+
+def paged_attention_decode_fp4(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    k_scales: torch.Tensor,
+    v_cache: torch.Tensor,
+    v_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    num_splits: int | None = None,
+    scale: float | None = None,
+    *,
+    weights: torch.Tensor | None = None,
+    num_new: int = 1,
+    slot_positions: torch.Tensor | None = None,
+    total_lens: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Decode attention over the 4-bit cache: paged_attention_decode_cuda_v4 with
+    K and V what their codes and scales stand for.
+
+    q [B, Hq, D] fp16 -> out [B, Hq, D] fp16; head_dim 32, 64 or 128, up to 16
+    query heads per KV head. weights, num_new, slot_positions and total_lens
+    are those of paged_attention_decode_weights (weights=None: not tracked)."""
+    assert q.is_cuda and k_cache.is_cuda and v_cache.is_cuda, "pad_b200 requires CUDA tensors"
+    assert q.dtype == torch.float16 and q.dim() == 3, "pad_b200 expects fp16 q [B, Hq, D]"
+    batch, num_q_heads, head_dim = q.shape
+    assert head_dim in FP4_HEAD_DIMS, f"head_dim must be one of {FP4_HEAD_DIMS}"
+    assert num_q_heads % k_cache.shape[2] == 0, "num_q_heads must be divisible by num_kv_heads (GQA)"
+    assert num_splits is None or num_splits >= 1, "num_splits must be >= 1"
+    assert num_new >= 0, "num_new must be >= 0"
+    assert weights is not None or slot_positions is None, "slot_positions go with weights"
+    assert slot_positions is not None or total_lens is None, "total_lens goes with slot_positions"
+    if slot_positions is not None and total_lens is None:
+        total_lens = seq_lens
+    _check_values(q.device)
+    out = _OPS.decode_fp4(q, k_cache, k_scales, v_cache, v_scales, block_table, seq_lens,
+                          0 if num_splits is None else int(num_splits),
+                          float(scale) if scale is not None else 1.0 / math.sqrt(head_dim), out, weights, int(num_new),
+                          slot_positions, total_lens)
+    _raise_if_checking(q.device)
+    return out

@@ -18,10 +18,10 @@ def quantise(x):
     e = np.maximum(e - 3, -24)
     with np.errstate(invalid="ignore"):
         y = np.where(fine[..., None], blocks, 0.0) / np.ldexp(1.0, e)[..., None]
-    dist = np.abs(np.abs(y)[..., None] - MAGNITUDES)
-    # nearest magnitude; a tie goes to the even code
-    tie = np.where(np.arange(8) % 2 == 0, 0.0, 1e-9)
-    code = (dist + tie).argmin(-1).astype(np.uint8) | (np.signbit(y).astype(np.uint8) << 3)
+    # nearest magnitude; a tie (on a midpoint) goes to the even code
+    a, mid = np.abs(y), (MAGNITUDES[:-1] + MAGNITUDES[1:]) / 2
+    code = sum(((a > m) | ((a == m) & (i % 2 == 1))).astype(np.uint8) for i, m in enumerate(mid))
+    code = code | (np.signbit(y).astype(np.uint8) << 3)
     code = np.where(fine[..., None], code, 0).reshape(x.shape).astype(np.uint8)
     scales = np.zeros((*x.shape[:-1], 4), dtype=np.uint8)
     scales[..., : d // 32] = np.where(fine, e + 127, 255)
