@@ -37,15 +37,6 @@ void set_merge(Instance* in) {
   in->merge_dsplit = DS;
 }
 
-// KV heads per tile: the largest of 8, 4, 2, 1 dividing num_kv_heads (at
-// most 4 when a head has more than 8 query rows, to fit shared memory).
-int head_group_for(int64_t hkv, int64_t gqa) {
-  const int cap = gqa <= 8 ? 8 : 4;
-  for (int hg = cap; hg > 1; hg /= 2)
-    if (hkv % hg == 0) return hg;
-  return 1;
-}
-
 // Merge variant by partials per split pair (partitions / pairs): up to
 // kMergeWide the 128-thread kernel (one CTA per query row); above it D is
 // split over CTAs, and above kMergeDeep each thread keeps 8 loads in flight.
@@ -56,7 +47,6 @@ int head_group_for(int64_t hkv, int64_t gqa) {
 #define PAD_MERGE_DEEP 32
 #endif
 constexpr int64_t kMergeWide = PAD_MERGE_WIDE, kMergeDeep = PAD_MERGE_DEEP;
-constexpr int64_t kFewPairs = 16;  // the num_splits=None heuristic: see make_plan
 
 bool pick_instance(int64_t head_dim, int64_t gqa, int hg, bool swz, Instance* out, bool weights = false) {
   if (!(weights ? pick_decode_weights(head_dim, gqa, hg, swz, out) : pick_decode<false>(head_dim, gqa, hg, swz, out)))
@@ -306,6 +296,63 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 }  // namespace
 
+namespace pad {
+
+int launch_merge(const MergeLaunch& m, cudaStream_t stream) {
+  Instance in = {};
+  switch (m.head_dim) {
+    case 16: set_merge<16>(&in); break;
+    case 32: set_merge<32>(&in); break;
+    case 64: set_merge<64>(&in); break;
+    default: set_merge<128>(&in); break;
+  }
+  MergeLaunch a = m;
+  void* args[] = {&a.ws_o, &a.ws_ml, &a.ws_meta, &a.out, &a.out_sb, &a.out_sh, &a.ngroups, &a.rows, &a.guess_ncap,
+                  &a.guess_parts};
+  cudaLaunchConfig_t cfg = {};
+  const int64_t pairs = m.batch * m.ngroups;
+  const bool wide = m.partitions > kMergeWide * pairs;
+  cfg.gridDim = dim3((unsigned)(m.meta_by_pair ? pairs : m.partitions), (unsigned)m.rows,
+                     wide ? (unsigned)in.merge_dsplit : 1u);
+  // A split pair has about partitions / pairs partials: fold a handful with a
+  // small block, long-context splits (hundreds of partials) with a wide one.
+  cfg.blockDim = dim3(wide ? 256 : 128);
+  cfg.dynamicSmemBytes = 0;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // overlap its launch with the decode tail
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const bool deep = m.partitions > kMergeDeep * pairs;  // 8 loads in flight
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, wide ? (deep ? in.merge_large : in.merge_mid) : in.merge_small, args);
+  return e == cudaSuccess ? PAD_OK : cuda_fail(e, "launching the merge kernel");
+}
+
+int sm_count(int device, int* num_sms) {
+  if (device < 0 || device >= kMaxDevices) return fail(PAD_ERR_INVALID_ARGUMENT, "device %d out of range", device);
+  std::lock_guard<std::mutex> lk(g_mu);
+  if (g_dev[device].num_sms == 0) {
+    int n = 0;
+    const cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute(SM count)");
+    g_dev[device].num_sms = n;
+  }
+  *num_sms = g_dev[device].num_sms;
+  return PAD_OK;
+}
+
+// KV heads per tile: the largest of 8, 4, 2, 1 dividing num_kv_heads (at
+// most 4 when a head has more than 8 query rows, to fit shared memory).
+int head_group_for(int64_t hkv, int64_t gqa) {
+  const int cap = gqa <= 8 ? 8 : 4;
+  for (int hg = cap; hg > 1; hg /= 2)
+    if (hkv % hg == 0) return hg;
+  return 1;
+}
+
+}  // namespace pad
+
 // =============================================================================
 extern "C" {
 
@@ -518,32 +565,23 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
   }
   if (e != cudaSuccess) return cuda_fail(e, "launching the decode kernel");
   if (plan.partitions > 1) {
-    const float* a0 = prm.ws_o;
-    const float2* a1 = prm.ws_ml;
-    const int4* a2 = prm.ws_meta;
-    __half* a3 = prm.out;
-    int ngroups = (int)(num_kv_heads / in.hg), rows = (int)(gqa * in.hg);
+    MergeLaunch m = {};
+    m.ws_o = prm.ws_o;
+    m.ws_ml = prm.ws_ml;
+    m.ws_meta = prm.ws_meta;
+    m.out = prm.out;
+    m.out_sb = prm.out_sb;
+    m.out_sh = prm.out_sh;
+    m.ngroups = (int)(num_kv_heads / in.hg);
+    m.rows = (int)(gqa * in.hg);
     // closed-form split descriptors for a dense batch of full rows (grid by pair)
-    int guess_ncap = 0, guess_parts = (int)plan.partitions;
-    if (prm.meta_by_pair && !csr) guess_ncap = (int)((max_pages_per_seq * page_size + in.tt - 1) / in.tt);
-    void* margs[] = {&a0, &a1, &a2, &a3, &prm.out_sb, &prm.out_sh, &ngroups, &rows, &guess_ncap, &guess_parts};
-    cudaLaunchConfig_t cfg = {};
-    const bool wide = plan.partitions > kMergeWide * batch * ngroups;
-    const int64_t merge_x = prm.meta_by_pair ? batch * ngroups : plan.partitions;
-    cfg.gridDim = dim3((unsigned)merge_x, (unsigned)rows, wide ? (unsigned)in.merge_dsplit : 1u);
-    // A split pair has about partitions / pairs partials: fold a handful with a
-    // small block, long-context splits (hundreds of partials) with a wide one.
-    cfg.blockDim = dim3(wide ? 256 : 128);
-    cfg.dynamicSmemBytes = 0;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // overlap its launch with the decode tail
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const bool deep = plan.partitions > kMergeDeep * batch * ngroups;  // 8 loads in flight
-    e = cudaLaunchKernelExC(&cfg, wide ? (deep ? in.merge_large : in.merge_mid) : in.merge_small, margs);
-    if (e != cudaSuccess) return cuda_fail(e, "launching the merge kernel");
+    m.guess_ncap = prm.meta_by_pair && !csr ? (int)((max_pages_per_seq * page_size + in.tt - 1) / in.tt) : 0;
+    m.guess_parts = (int)plan.partitions;
+    m.batch = batch;
+    m.partitions = plan.partitions;
+    m.head_dim = head_dim;
+    m.meta_by_pair = prm.meta_by_pair;
+    if ((st = launch_merge(m, s)) != PAD_OK) return st;
   }
   if (wa != nullptr) {
     WeightParams wp = {};

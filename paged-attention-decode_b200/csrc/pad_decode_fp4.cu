@@ -1,142 +1,128 @@
-// pad_decode_fp4.cu -- decode attention over the 4-bit paged cache (format:
-// pad_fp4.cuh). One CTA per (sequence, KV head): a warp takes every fourth
-// token, a lane D/32 of its dims, for all G query heads, with an online softmax
-// in base 2; the four warps' states are joined through shared memory. Attention
-// weights take a second pass over K, when (M, L) is known.
+// pad_decode_fp4.cu -- host side of the decode over the 4-bit paged cache
+// (pad_decode_fp4_kernel.cuh): argument checks, the plan and the launches.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <climits>
 #include <cmath>
 #include <cstdint>
 
 #include "pad_b200.h"
+#include "pad_decode_fp4_kernel.cuh"
+#include "pad_decode_instance.cuh"
 #include "pad_error.cuh"
-#include "pad_fp4.cuh"
-#include "pad_ptx.cuh"
 
 namespace {
 
 using namespace pad;
 
-constexpr int kWarps = 4;
 constexpr int kMaxG = 16;
-
-struct Params {
-  const __half* q;
-  const uint8_t *k, *ks, *v, *vs;
-  const int32_t *block_table, *seq_lens, *total_lens;
-  __half* out;
-  float* weights;
-  int32_t* slot_positions;
-  int32_t* error_flags;
-  int64_t q0, q1, k0, k1, k2, ks0, ks1, ks2, v0, v1, v2, vs0, vs1, vs2, o0, o1, w0, w1, w2, p0, p1, p2, bt_stride;
-  int hkv, gqa, num_pages, page_size, max_pages, num_new;
-  float scale_log2;
-};
-
-__device__ __forceinline__ float code_value(uint32_t n) {
-  const float m = (float)(n & 7u);
-  const float v = m <= 4.f ? 0.5f * m : (m == 7.f ? 6.f : m - 2.f);
-  return (n & 8u) ? -v : v;
-}
-
-// This lane's D/32 dims of a row (at least one byte: D = 32 shares it).
-template <int D>
-__device__ __forceinline__ void row_values(const uint8_t* codes, const uint8_t* scales, int lane, float (&x)[D / 32]) {
-  constexpr int E = D / 32;
-  const int d0 = lane * E;
-  const float f = fp4_scale_f32(scales[d0 / 32]);
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const uint32_t b = codes[(d0 + e) / 2];
-    x[e] = code_value(((d0 + e) & 1) ? b >> 4 : b & 15u) * f;
-  }
-}
-
-template <int D>
-__global__ void __launch_bounds__(32 * kWarps) decode_fp4_kernel(const __grid_constant__ Params p) {
-  constexpr int E = D / 32;
-  __shared__ float so[kWarps][D];
-  __shared__ float sm[kWarps][kMaxG], sl[kWarps][kMaxG];
-  const int b = blockIdx.x / p.hkv, h = blockIdx.x % p.hkv;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t cap = (int64_t)p.max_pages * p.page_size;
-  const int raw = p.seq_lens[b];
-  const int n = (int)min((int64_t)max(raw, 0), cap);
-  if (raw != n && threadIdx.x == 0 && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_SEQ_LEN_RANGE);
-  for (int g = 0; g < p.gqa; ++g) {
-    const __half* qr = p.q + b * p.q0 + (int64_t)(h * p.gqa + g) * p.q1 + lane * E;
-    float q[E], acc[E], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      q[e] = __half2float(qr[e]);
-      acc[e] = 0.f;
-    }
-    auto page_of = [&](int t) {
-      const int page = p.block_table[b * p.bt_stride + t / p.page_size];
-      if ((unsigned)page < (unsigned)p.num_pages) return (int64_t)page;
-      if (lane == 0 && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_BAD_PAGE_ID);
-      return (int64_t)-1;
-    };
-    auto score = [&](int64_t page, int64_t row) {
-      float x[E], s = 0.f;
-      row_values<D>(p.k + page * p.k0 + row * p.k1 + h * p.k2, p.ks + page * p.ks0 + row * p.ks1 + h * p.ks2, lane, x);
-#pragma unroll
-      for (int e = 0; e < E; ++e) s += q[e] * x[e];
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      return s * p.scale_log2;
-    };
-    for (int t = warp; t < n; t += kWarps) {
-      const int64_t page = page_of(t), row = t % p.page_size;
-      const float s = page < 0 ? 0.f : score(page, row);
-      const float mn = fmaxf(m, s), mu = mn == -INFINITY ? 0.f : mn;
-      const float al = ex2(m - mu), w = ex2(s - mu);
-      float x[E] = {};
-      if (page >= 0)
-        row_values<D>(p.v + page * p.v0 + row * p.v1 + h * p.v2, p.vs + page * p.vs0 + row * p.vs1 + h * p.vs2, lane, x);
-      l = l * al + w;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * al + w * x[e];
-      m = mn;
-    }
-    if (lane == 0) {
-      sm[warp][g] = m;
-      sl[warp][g] = l;
-    }
-#pragma unroll
-    for (int e = 0; e < E; ++e) so[warp][lane * E + e] = acc[e];
-    __syncthreads();
-    float M = -INFINITY, L = 0.f;
-    for (int x = 0; x < kWarps; ++x) M = fmaxf(M, sm[x][g]);
-    const float Mu = M == -INFINITY ? 0.f : M;
-    for (int x = 0; x < kWarps; ++x) L += sl[x][g] * ex2(sm[x][g] - Mu);
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    for (int d = threadIdx.x; d < D; d += 32 * kWarps) {
-      float o = 0.f;
-      for (int x = 0; x < kWarps; ++x) o += so[x][d] * ex2(sm[x][g] - Mu);
-      p.out[b * p.o0 + (int64_t)(h * p.gqa + g) * p.o1 + d] = __float2half_rn(o * inv);
-    }
-    if (p.weights != nullptr) {
-      for (int t = warp; t < n; t += kWarps) {
-        const int64_t page = page_of(t), row = t % p.page_size;
-        if (page < 0) continue;
-        const float w = ex2(score(page, row) - Mu) * inv;
-        if (lane != 0) continue;
-        const bool fresh = t >= n - p.num_new;
-        float* at = p.weights + page * p.w0 + h * p.w1 + row * p.w2;
-        *at = fresh && g == 0 ? w : *at + w;
-        if (fresh && p.slot_positions != nullptr)
-          p.slot_positions[page * p.p0 + h * p.p1 + row * p.p2] = p.total_lens[b] - n + t;
-      }
-    }
-    __syncthreads();
-  }
-}
+constexpr int kFp4Devices = 64;
+constexpr int kTile = 32;  // tokens of a tile, Fp4Traits::TT
 
 bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+
+struct Fp4Instance {
+  const void* kernel;
+  int smem_bytes, threads, key;
+};
+
+template <int D, int NT, bool WT>
+Fp4Instance instance(int key) {
+  using TR = Fp4Traits<D, NT, WT>;
+  static_assert(TR::TT == kTile, "tile");
+  return {reinterpret_cast<const void*>(&decode_fp4_kernel<TR>), TR::SMEM_BYTES, TR::THREADS, key};
+}
+
+// Query heads per KV head up to 8 fill one n8 tile of the tensor cores, more
+// take two (and half the warps, for their registers).
+template <int D>
+Fp4Instance pick(int64_t gqa, bool weights, int key) {
+  if (gqa <= 8) return weights ? instance<D, 1, true>(key) : instance<D, 1, false>(key + 1);
+  return weights ? instance<D, 2, true>(key + 2) : instance<D, 2, false>(key + 3);
+}
+
+constexpr int kInstances = 12;
+
+int prepare(int device, const Fp4Instance& in) {
+  static std::atomic<bool> done[kFp4Devices][kInstances];  // set twice by racing threads at worst
+  if (device < 0 || device >= kFp4Devices) return fail(PAD_ERR_INVALID_ARGUMENT, "device %d out of range", device);
+  if (!done[device][in.key].load()) {
+    const cudaError_t e = cudaFuncSetAttribute(in.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, in.smem_bytes);
+    if (e != cudaSuccess) return cuda_fail(e, "configuring the decode_fp4 kernel");
+    done[device][in.key].store(true);
+  }
+  return PAD_OK;
+}
+
+struct Fp4Plan {
+  int hg = 1;
+  int64_t partitions = 1, slots = 0, raw_tiles = 0;
+  size_t off_ml = 0, off_o = 0, off_total = 0, off_pairs = 0, off_tiles = 0, off_raw = 0, bytes = 0;
+};
+
+int make_plan(int device, int64_t batch, int64_t hkv, int64_t gqa, int64_t head_dim, int64_t num_pages,
+              int64_t page_size, int64_t max_pages, int64_t num_splits, bool weights, Fp4Plan* plan) {
+  const char* what = "decode_fp4";
+  if (batch < 0 || hkv <= 0 || gqa <= 0 || num_pages < 0 || page_size <= 0 || max_pages < 0)
+    return fail(PAD_ERR_INVALID_ARGUMENT, "%s: negative or zero size", what);
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128)
+    return fail(PAD_ERR_UNSUPPORTED, "%s: head_dim %lld not supported (32, 64 or 128)", what, (long long)head_dim);
+  if (gqa > kMaxG) return fail(PAD_ERR_UNSUPPORTED, "%s: gqa_ratio %lld > 16 not supported", what, (long long)gqa);
+  if (num_pages > INT32_MAX || max_pages > INT32_MAX || page_size > INT32_MAX || hkv > INT32_MAX ||
+      max_pages * page_size > INT32_MAX / 2)
+    return fail(PAD_ERR_UNSUPPORTED, "%s: problem too large for 32-bit indexing", what);
+  plan->hg = head_group_for(hkv, gqa);
+  const int64_t groups = hkv / plan->hg, tiles = (max_pages * page_size + kTile - 1) / kTile;
+  if (batch > INT32_MAX / 4 / groups || batch * groups > INT32_MAX / 4 / std::max<int64_t>(tiles, 1))
+    return fail(PAD_ERR_UNSUPPORTED, "%s: problem too large for 32-bit indexing", what);
+  const int64_t tiles_ub = batch * groups * tiles, pairs = batch * groups;
+  int64_t parts;
+  if (num_splits <= 0) {
+    int sms = 0;
+    const int st = sm_count(device, &sms);
+    if (st != PAD_OK) return st;
+    parts = std::min<int64_t>(sms, tiles_ub);
+  } else {
+    if (num_splits > ((int64_t)1 << 30) / std::max<int64_t>(pairs, 1))
+      return fail(PAD_ERR_UNSUPPORTED, "%s: num_splits %lld too large", what, (long long)num_splits);
+    parts = num_splits * pairs;
+  }
+  plan->partitions = std::max<int64_t>(parts, 1);
+  plan->slots = plan->partitions + pairs;
+  const int64_t rows = plan->hg * gqa;
+  plan->off_ml = align_up((size_t)std::max(plan->partitions, pairs) * sizeof(int4), 256);
+  plan->off_o = align_up(plan->off_ml + (size_t)(plan->slots * rows) * sizeof(float2), 256);
+  plan->bytes = align_up(plan->off_o + (size_t)(plan->slots * rows * head_dim) * sizeof(float), 256);
+  if (weights) {
+    // as for the fp16 decode: no more tiles than the table names or the pool holds
+    plan->raw_tiles = std::min(tiles_ub, groups * (num_pages * page_size / kTile + batch));
+    plan->off_total = plan->bytes;
+    plan->off_pairs = plan->off_total + 256;
+    plan->off_tiles = align_up(plan->off_pairs + (size_t)pairs * sizeof(int2), 256);
+    plan->off_raw = align_up(plan->off_tiles + (size_t)plan->raw_tiles * sizeof(int4), 256);
+    plan->bytes = align_up(plan->off_raw + (size_t)(plan->raw_tiles * rows * kTile) * sizeof(float), 256);
+  }
+  return PAD_OK;
+}
+
+// Offsets within a code cache are kept in 32 bits, in units of the largest
+// power of two (16 to 64 bytes) that divides every stride; the largest must fit.
+int offset_shift(const int64_t* k, const int64_t* v, int64_t pages, int64_t ps, int64_t hkv) {
+  uint64_t all = 0;
+  for (int i = 0; i < 3; ++i) all |= (uint64_t)k[i] | (uint64_t)v[i];
+  int shift = 4;
+  while (shift < 6 && (all >> shift) % 2 == 0) ++shift;
+  for (const int64_t* s : {k, v}) {
+    if (s[0] < 0 || s[1] < 0 || s[2] < 0) return -1;
+    const double last = (double)(pages - 1) * (double)s[0] + (double)(ps - 1) * (double)s[1] + (double)(hkv - 1) * (double)s[2];
+    if (pages > 0 && last / (double)(1 << shift) >= 4294967296.0) return -1;
+  }
+  return shift;
+}
 
 }  // namespace
 
@@ -145,8 +131,11 @@ extern "C" int pad_decode_fp4_workspace_bytes(int device, int64_t batch, int64_t
                                               int64_t max_pages_per_seq, int64_t num_splits, int with_weights,
                                               size_t* bytes) {
   if (bytes == nullptr) return fail(PAD_ERR_INVALID_ARGUMENT, "decode_fp4: null output pointer");
-  *bytes = 256;
-  return PAD_OK;
+  Fp4Plan plan;
+  const int st = make_plan(device, batch, num_kv_heads, gqa_ratio, head_dim, num_pages, page_size, max_pages_per_seq,
+                           num_splits, with_weights != 0, &plan);
+  if (st == PAD_OK) *bytes = plan.bytes;
+  return st;
 }
 
 extern "C" int pad_paged_attention_decode_fp4(
@@ -193,10 +182,30 @@ extern "C" int pad_paged_attention_decode_fp4(
     return fail(PAD_ERR_UNSUPPORTED, "%s: codes must be 16-byte aligned, scales 4-byte aligned", what);
   if (block_table_stride < max_pages_per_seq)
     return fail(PAD_ERR_INVALID_ARGUMENT, "%s: block_table row stride smaller than its width", what);
-  if (num_pages > INT32_MAX || max_pages_per_seq > INT32_MAX || page_size > INT32_MAX ||
-      max_pages_per_seq * page_size > INT32_MAX / 2 || batch > INT32_MAX / num_q_heads / 4)
-    return fail(PAD_ERR_UNSUPPORTED, "%s: problem too large for 32-bit indexing", what);
-  Params p = {};
+  int device = 0;
+  cudaError_t e = cudaSuccess;
+  // the sizes are checked before the device is asked for
+  Fp4Plan plan;
+  int st = make_plan(0, batch, num_kv_heads, gqa, head_dim, num_pages, page_size, max_pages_per_seq,
+                     std::max<int64_t>(num_splits, 1), weights != nullptr, &plan);
+  if (st != PAD_OK) return st;
+  const int shift = offset_shift(k_strides, v_strides, num_pages, page_size, num_kv_heads);
+  if (shift < 0)
+    return fail(PAD_ERR_UNSUPPORTED, "%s: cache strides are negative or reach past 2^32 units of 16 to 64 bytes", what);
+  if ((e = cudaGetDevice(&device)) != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  if (num_splits <= 0 && (st = make_plan(device, batch, num_kv_heads, gqa, head_dim, num_pages, page_size,
+                                         max_pages_per_seq, num_splits, weights != nullptr, &plan)) != PAD_OK)
+    return st;
+  if (workspace == nullptr || workspace_bytes < plan.bytes)
+    return fail(PAD_ERR_WORKSPACE, "%s: workspace of %zu bytes needed, %zu given", what, plan.bytes,
+                workspace == nullptr ? (size_t)0 : workspace_bytes);
+  if (!aligned(workspace, 16)) return fail(PAD_ERR_WORKSPACE, "%s: workspace must be 16-byte aligned", what);
+  const Fp4Instance in = head_dim == 32   ? pick<32>(gqa, weights != nullptr, 0)
+                         : head_dim == 64 ? pick<64>(gqa, weights != nullptr, 4)
+                                          : pick<128>(gqa, weights != nullptr, 8);
+  if ((st = prepare(device, in)) != PAD_OK) return st;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  Fp4DecodeParams p = {};
   p.q = static_cast<const __half*>(q);
   p.k = static_cast<const uint8_t*>(k_cache);
   p.ks = static_cast<const uint8_t*>(k_scales);
@@ -204,32 +213,108 @@ extern "C" int pad_paged_attention_decode_fp4(
   p.vs = static_cast<const uint8_t*>(v_scales);
   p.block_table = block_table;
   p.seq_lens = seq_lens;
-  p.total_lens = total_lens;
   p.out = static_cast<__half*>(out);
-  p.weights = weights;
-  p.slot_positions = slot_positions;
+  p.ws_meta = reinterpret_cast<int4*>(ws);
+  p.ws_ml = reinterpret_cast<float2*>(ws + plan.off_ml);
+  p.ws_o = reinterpret_cast<float*>(ws + plan.off_o);
   p.error_flags = error_flags;
-  p.q0 = q_strides[0], p.q1 = q_strides[1];
-  p.k0 = k_strides[0], p.k1 = k_strides[1], p.k2 = k_strides[2];
-  p.ks0 = ks_strides[0], p.ks1 = ks_strides[1], p.ks2 = ks_strides[2];
-  p.v0 = v_strides[0], p.v1 = v_strides[1], p.v2 = v_strides[2];
-  p.vs0 = vs_strides[0], p.vs1 = vs_strides[1], p.vs2 = vs_strides[2];
-  p.o0 = out_strides[0], p.o1 = out_strides[1];
-  if (weights != nullptr) p.w0 = weight_strides[0], p.w1 = weight_strides[1], p.w2 = weight_strides[2];
-  if (slot_positions != nullptr) p.p0 = position_strides[0], p.p1 = position_strides[1], p.p2 = position_strides[2];
+  p.q0 = q_strides[0];
+  p.q1 = q_strides[1];
   p.bt_stride = block_table_stride;
+  p.out_sb = out_strides[0];
+  p.out_sh = out_strides[1];
+  p.k0 = k_strides[0] >> shift;
+  p.k1 = k_strides[1] >> shift;
+  p.k2 = k_strides[2] >> shift;
+  p.v0 = v_strides[0] >> shift;
+  p.v1 = v_strides[1] >> shift;
+  p.v2 = v_strides[2] >> shift;
+  p.ks0 = ks_strides[0];
+  p.ks1 = ks_strides[1];
+  p.ks2 = ks_strides[2];
+  p.vs0 = vs_strides[0];
+  p.vs1 = vs_strides[1];
+  p.vs2 = vs_strides[2];
+  p.batch = (int)batch;
   p.hkv = (int)num_kv_heads;
   p.gqa = (int)gqa;
-  p.num_pages = (int)num_pages;
+  p.hg_log2 = __builtin_ctz((unsigned)plan.hg);
   p.page_size = (int)page_size;
+  p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)page_size) : -1;
+  p.num_pages = (int)num_pages;
   p.max_pages = (int)max_pages_per_seq;
-  p.num_new = (int)std::min<int64_t>(num_new, INT32_MAX);
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.off_shift = shift;
+  p.same_off = p.k0 == p.v0 && p.k1 == p.v1 && p.k2 == p.v2;
+  const int64_t pairs = batch * (num_kv_heads / plan.hg);
+  p.meta_by_pair = pairs < plan.partitions ? 1 : 0;
+  p.scale_log2 = scale * kLog2e;
+  if (weights != nullptr) {
+    p.track.raw = reinterpret_cast<float*>(ws + plan.off_raw);
+    p.track.tiles = reinterpret_cast<int4*>(ws + plan.off_tiles);
+    p.track.pairs = reinterpret_cast<int2*>(ws + plan.off_pairs);
+    p.track.total = reinterpret_cast<int*>(ws + plan.off_total);
+    p.track.raw_tiles = (int)plan.raw_tiles;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const unsigned grid = (unsigned)(batch * num_kv_heads);
-  if (head_dim == 32) decode_fp4_kernel<32><<<grid, 32 * kWarps, 0, s>>>(p);
-  else if (head_dim == 64) decode_fp4_kernel<64><<<grid, 32 * kWarps, 0, s>>>(p);
-  else decode_fp4_kernel<128><<<grid, 32 * kWarps, 0, s>>>(p);
-  const cudaError_t e = cudaGetLastError();
-  return e == cudaSuccess ? PAD_OK : cuda_fail(e, "launching the decode_fp4 kernel");
+  {
+    void* args[] = {&p};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)plan.partitions);
+    cfg.blockDim = dim3((unsigned)in.threads);
+    cfg.dynamicSmemBytes = (size_t)in.smem_bytes;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    if ((e = cudaLaunchKernelExC(&cfg, in.kernel, args)) != cudaSuccess)
+      return cuda_fail(e, "launching the decode_fp4 kernel");
+  }
+  if (plan.partitions > 1) {
+    MergeLaunch m = {};
+    m.ws_o = p.ws_o;
+    m.ws_ml = p.ws_ml;
+    m.ws_meta = p.ws_meta;
+    m.out = p.out;
+    m.out_sb = p.out_sb;
+    m.out_sh = p.out_sh;
+    m.ngroups = (int)(num_kv_heads / plan.hg);
+    m.rows = (int)(gqa * plan.hg);
+    m.guess_ncap = p.meta_by_pair ? (int)((max_pages_per_seq * page_size + kTile - 1) / kTile) : 0;
+    m.guess_parts = (int)plan.partitions;
+    m.batch = batch;
+    m.partitions = plan.partitions;
+    m.head_dim = head_dim;
+    m.meta_by_pair = p.meta_by_pair;
+    if ((st = launch_merge(m, s)) != PAD_OK) return st;
+  }
+  if (weights != nullptr) {
+    WeightParams wp = {};
+    wp.track = p.track;
+    wp.ml = p.ws_ml;
+    wp.block_table = block_table;
+    wp.total_lens = total_lens;
+    wp.weights = weights;
+    wp.slot_positions = slot_positions;
+    wp.w0 = weight_strides[0];
+    wp.w1 = weight_strides[1];
+    wp.w2 = weight_strides[2];
+    if (slot_positions != nullptr) {
+      wp.p0 = position_strides[0];
+      wp.p1 = position_strides[1];
+      wp.p2 = position_strides[2];
+    }
+    wp.bt_stride = block_table_stride;
+    wp.hg = plan.hg;
+    wp.gqa = (int)gqa;
+    wp.tt = kTile;
+    wp.ngroups = (int)(num_kv_heads / plan.hg);
+    wp.page_size = (int)page_size;
+    wp.page_shift = p.page_shift;
+    wp.num_pages = (int)num_pages;
+    wp.num_new = (int)std::min<int64_t>(num_new, INT32_MAX);
+    if ((st = launch_weights(wp, s)) != PAD_OK) return st;
+  }
+  return PAD_OK;
 }

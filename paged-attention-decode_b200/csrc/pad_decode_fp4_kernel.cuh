@@ -1,0 +1,621 @@
+// pad_decode_fp4_kernel.cuh -- decode attention over the 4-bit paged cache
+// (format: pad_fp4.cuh), the split-K phase; merge_kernel joins its partials.
+//
+// Work unit: a tile of 32 tokens of a head group of HG KV heads. The batch is
+// one list of tiles ordered (sequence, head group, tile) and every CTA takes an
+// equal contiguous range of it, as the fp16 decode does.
+//
+// At 4.25 bits a value the arithmetic, not the copy, is close to the limit (an
+// SM is sent about 43 values a clock at full bandwidth, and every one has to
+// become fp16), so the kernel is built around the fewest instructions a value:
+//   - A warp owns whole (tile, head) pieces: WPH = warps / HG warps share a
+//     head and take turns at its tiles. It copies its own pieces into its own
+//     ring with cp.async and waits for nobody: no producer, no barriers between
+//     warps until a (sequence, head group) segment ends.
+//   - Codes go from shared memory to registers by ldmatrix on 16-bit units of
+//     four codes. For K a lane gets 8 consecutive dims of its row, for V
+//     (transposed) four dims of two neighbouring tokens. The order in which a
+//     contraction runs through its index is free, so Q is loaded in the order
+//     K's bytes come out in and no code is ever moved to another lane.
+//   - One conversion instruction makes two fp16 values of a code byte, exactly.
+//   - K's scales are powers of two of 32 dims and leave the sum: the tensor
+//     cores add up each block by itself, and the block's sum is scaled in fp32
+//     (with the softmax scale folded in). V's scales differ along the
+//     contraction and go onto the values, one packed multiplication for two.
+//     Both are unpacked once per token through shared memory.
+//   - P is split into two fp16 terms as in the fp16 decode.
+// Tokens past the sequence, and pages that are none, are copied as zeros
+// (cp.async with no source bytes): zero codes with a finite scale, so nothing a
+// page holds behind its sequence can reach the sums.
+#pragma once
+
+#include <climits>
+
+#include "pad_b200.h"
+#include "pad_decode_kernel.cuh"
+#include "pad_fp4.cuh"
+
+namespace pad {
+
+struct Fp4DecodeParams {
+  const __half* q;
+  const uint8_t *k, *ks, *v, *vs;
+  const int32_t *block_table, *seq_lens;
+  __half* out;
+  float* ws_o;      // as in DecodeParams
+  float2* ws_ml;
+  int4* ws_meta;
+  int32_t* error_flags;
+  int64_t q0, q1, bt_stride, out_sb, out_sh;
+  int64_t k0, k1, k2, v0, v1, v2;          // code strides in units of 2^off_shift bytes
+  int64_t ks0, ks1, ks2, vs0, vs1, vs2;    // scale strides in bytes
+  int batch, hkv, gqa, hg_log2, page_size, page_shift, num_pages, max_pages;
+  int off_shift, same_off;                 // K and V have the same strides
+  int meta_by_pair;
+  float scale_log2;
+  TrackParams track;
+};
+
+template <int D_, int NT_, bool WT_>
+struct Fp4Traits {
+  static constexpr int D = D_, NT = NT_;
+  static constexpr bool WT = WT_;
+  static constexpr int NW = NT == 1 ? 16 : 8;      // warps: 128 or 255 registers a thread
+  static constexpr int THREADS = 32 * NW;
+  static constexpr int TT = 32;                    // tokens per tile
+  static constexpr int NB = D / kFp4Block;         // blocks of 32 dims
+  static constexpr int ROW = D / 2;                // code bytes of a row
+  static constexpr int CPR = ROW / 16;             // 16-byte chunks of a row
+  static constexpr int CODES = TT * ROW;
+  static constexpr int STAGE = 2 * CODES + 2 * TT * kFp4ScaleRow;
+  // about 136 KB of ring: one to two pieces in flight per warp at D = 128
+  static constexpr int FIT = 139264 / NW / STAGE;
+  static constexpr int STAGES = FIT > 6 ? 6 : FIT;
+  static_assert(STAGES >= 2, "the ring needs two stages");
+  static constexpr int SCRATCH = TT * 16 + TT / 2 * 16;  // unpacked scales of K (fp32) and V (fp16 pairs)
+  static constexpr int LD = D + 4;                 // padded row of the epilogue
+  static constexpr int ROWS = 8 * NT;              // query rows a head holds
+  static constexpr int OFF_SCRATCH = NW * STAGES * STAGE;
+  static constexpr int OFF_EPI = OFF_SCRATCH + NW * SCRATCH;
+  static constexpr int OFF_ML = OFF_EPI + NW * ROWS * LD * 4;
+  static constexpr int OFF_MISC = OFF_ML + NW * ROWS * 8;
+  static constexpr int SMEM_BYTES = OFF_MISC + 256 + kSeqCache * 4 + 128 /*align slack*/;
+  static_assert(SMEM_BYTES <= kSmemBudget, "shared memory");
+  // XOR on a row's chunk index that spreads ldmatrix's 8 rows over all banks
+  __device__ static __forceinline__ uint32_t swz(uint32_t row) {
+    if constexpr (CPR == 4) return (row >> 1) & 3u;
+    else if constexpr (CPR == 2) return (row >> 2) & 1u;
+    else return 0u;
+  }
+};
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(bytes),
+               "l"(policy)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_4z(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// Position in the flattened (sequence, head group, tile) list.
+struct Fp4Cursor {
+  int b, hg, i, n, seq;  // tile i of n of the pair
+  int start;             // global index of the pair's tile 0
+};
+
+template <class TR>
+struct Fp4Walk {
+  const Fp4DecodeParams& p;
+  const int* sseq;
+  int cap, ngroups;
+  __device__ __forceinline__ int seq_at(int b) const {
+    return b < kSeqCache ? sseq[b] : clamp_seq(__ldg(p.seq_lens + b), cap);
+  }
+  __device__ __forceinline__ void next_pair(Fp4Cursor& c) const {
+    c.start += c.n;
+    if (++c.hg < ngroups) return;
+    c.hg = 0;
+    do {
+      if (++c.b >= p.batch) {
+        c.n = 0;
+        return;
+      }
+      c.seq = seq_at(c.b);
+      c.n = (c.seq + TR::TT - 1) / TR::TT;
+    } while (c.n == 0);
+  }
+  // Steps on by `step` tiles; past the end n = 0.
+  __device__ __forceinline__ void advance(Fp4Cursor& c, int step) const {
+    c.i += step;
+    while (c.n > 0 && c.i >= c.n) {
+      c.i -= c.n;
+      next_pair(c);
+    }
+  }
+};
+
+template <class TR>
+__global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid_constant__ Fp4DecodeParams p) {
+  constexpr int D = TR::D, NT = TR::NT, NB = TR::NB, S = TR::STAGES, TT = TR::TT, NW = TR::NW;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 127) & ~uintptr_t(127));
+  float* epi = reinterpret_cast<float*>(smem + TR::OFF_EPI);      // [warp][ROWS][LD]
+  float2* sml = reinterpret_cast<float2*>(smem + TR::OFF_ML);     // [warp][ROWS]
+  int* scan = reinterpret_cast<int*>(smem + TR::OFF_MISC);        // [16]
+  int* cur = scan + 16;                                           // the first cursor
+  int* sseq = scan + 64;                                          // [kSeqCache]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cap = p.max_pages * p.page_size;
+  const int64_t W = gridDim.x;
+  const int w = blockIdx.x, G = p.gqa, HG = 1 << p.hg_log2, ngroups = p.hkv >> p.hg_log2;
+  const int WPH = NW >> p.hg_log2;          // warps that share a head
+  const int hl = warp / WPH, turn = warp - hl * WPH;
+  const Fp4Walk<TR> walk{p, sseq, cap, ngroups};
+
+  if (tid == 0) cur[0] = -1;
+  pdl_wait_primary();
+
+  // ---- tiles per sequence, scanned: this CTA's range and its first cursor
+  int t0, t1, total = 0;
+  {
+    const int per = (p.batch + TR::THREADS - 1) / TR::THREADS;
+    const int lo = min(p.batch, tid * per), hi = min(p.batch, lo + per);
+    int local = 0, bad = 0, none = 0;
+    for (int b = lo; b < hi; ++b) {
+      const int raw = __ldg(p.seq_lens + b), sq = clamp_seq(raw, cap);
+      bad |= raw != sq;
+      none |= sq == 0;
+      if (b < kSeqCache) sseq[b] = sq;
+      local += (sq + TT - 1) / TT;
+    }
+    local *= ngroups;
+    int incl = local;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 31) scan[warp] = incl;
+    none = __syncthreads_or(none);
+    int excl = incl - local;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) {
+      const int v = scan[x];
+      if (x < warp) excl += v;
+      total += v;
+    }
+    if (bad && w == 0 && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_SEQ_LEN_RANGE);
+    t0 = total > 0 ? part_begin(w, total, W) : 0;
+    t1 = total > 0 ? part_begin(w + 1, total, W) : 0;
+    if (t0 < total && excl <= t0 && t0 < excl + local) {
+      int acc = excl;
+      for (int b = lo; b < hi; ++b) {
+        const int seq = walk.seq_at(b), n = (seq + TT - 1) / TT;
+        if (t0 < acc + n * ngroups) {
+          const int o = t0 - acc;
+          cur[0] = b;
+          cur[1] = o / n;
+          cur[2] = o % n;
+          cur[3] = n;
+          cur[4] = seq;
+          cur[5] = acc + (o / n) * n;
+          break;
+        }
+        acc += n * ngroups;
+      }
+    }
+    __syncthreads();
+    pdl_launch_dependents();
+    if (tid == 0) {
+      if (!p.meta_by_pair) p.ws_meta[w] = make_int4(-1, 0, 0, 0);
+      if constexpr (TR::WT) {
+        if (w == 0) *p.track.total = total;
+      }
+    }
+    // empty sequences: zero output rows, no merge
+    for (int b = w; none && b < p.batch; b += (int)W) {
+      if (walk.seq_at(b) != 0) continue;
+      if (p.meta_by_pair)
+        for (int x = tid; x < ngroups; x += TR::THREADS) p.ws_meta[b * ngroups + x] = make_int4(-1, 0, 0, 0);
+      for (int x = tid; x < p.hkv * G * (D / 2); x += TR::THREADS)
+        *reinterpret_cast<__half2*>(p.out + b * p.out_sb + (x / (D / 2)) * p.out_sh + (x % (D / 2)) * 2) =
+            __floats2half2_rn(0.f, 0.f);
+    }
+  }
+  Fp4Cursor seg{cur[0], cur[1], cur[2], cur[3], cur[4], cur[5]};
+  if (t1 <= t0) {
+    // an empty partition may still lie between those of a split pair: its
+    // partial there is empty
+    if (seg.b >= 0 && seg.start < t0)
+      for (int x = tid; x < HG * G; x += TR::THREADS)
+        p.ws_ml[(int64_t)(seg.b * ngroups + seg.hg + w) * HG * G + x] = make_float2(-INFINITY, 0.f);
+    return;
+  }
+
+  // ---- this warp's ring and its copies
+  const uint32_t ring = smem_u32(smem) + warp * (S * TR::STAGE);
+  const uint32_t scratch = smem_u32(smem + TR::OFF_SCRATCH) + warp * TR::SCRATCH;
+  const uint64_t policy = l2_evict_first_policy();
+  const uint32_t chunk = lane % TR::CPR, row_of_lane = lane / TR::CPR;
+  const uint32_t copy_dst = row_of_lane * TR::ROW + ((chunk ^ TR::swz(row_of_lane)) << 4);
+  Fp4Cursor ld = seg;     // next tile to copy
+  int ld_t = t0 + turn;
+  walk.advance(ld, turn);
+  // The page id of this lane's token of the tile at `c` (-1: no token).
+  auto page_id = [&](const Fp4Cursor& c, int t) -> int {
+    const int tok = c.i * TT + lane;
+    if (t >= t1 || tok >= c.seq) return -1;
+    const int lp = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size;
+    return ld_nc_early(p.block_table + c.b * p.bt_stride + lp);
+  };
+  auto copy = [&](const Fp4Cursor& c, int t, int page, int stage) {
+    if (t < t1) {
+      const int tok = c.i * TT + lane, h = c.hg * HG + hl;
+      const bool live = tok < c.seq, ok = live && (unsigned)page < (unsigned)p.num_pages;
+      if (live && !ok && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_BAD_PAGE_ID);
+      const int row = p.page_shift >= 0 ? tok & (p.page_size - 1) : tok % p.page_size;
+      const uint32_t good = __ballot_sync(0xffffffffu, ok);
+      const int64_t pg = ok ? page : 0, rw = ok ? row : 0;
+      const uint32_t ko = (uint32_t)(pg * p.k0 + rw * p.k1 + h * p.k2);
+      const uint32_t vo = (uint32_t)(pg * p.v0 + rw * p.v1 + h * p.v2);
+      const uint32_t base = ring + stage * TR::STAGE;
+#pragma unroll
+      for (int x = 0; x < TR::CPR; ++x) {
+        const int r = row_of_lane + x * (32 / TR::CPR);
+        const uint32_t bytes = (good >> r) & 1u ? 16u : 0u;
+        const uint32_t kr = __shfl_sync(0xffffffffu, ko, r);
+        const uint32_t vr = p.same_off ? kr : __shfl_sync(0xffffffffu, vo, r);
+        const uint32_t dst = base + copy_dst + x * (32 / TR::CPR) * TR::ROW;
+        cp_async_16(dst, p.k + ((uint64_t)kr << p.off_shift) + chunk * 16, bytes, policy);
+        cp_async_16(dst + TR::CODES, p.v + ((uint64_t)vr << p.off_shift) + chunk * 16, bytes, policy);
+      }
+      const uint32_t sdst = base + 2 * TR::CODES + lane * kFp4ScaleRow;
+      cp_async_4z(sdst, p.ks + pg * p.ks0 + rw * p.ks1 + h * p.ks2, ok ? 4u : 0u);
+      cp_async_4z(sdst + TT * kFp4ScaleRow, p.vs + pg * p.vs0 + rw * p.vs1 + h * p.vs2, ok ? 4u : 0u);
+    }
+    cp_async_commit();
+  };
+  int next_page;
+  {
+    Fp4Cursor c = ld;
+    int pages[S], t = ld_t;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      pages[s] = page_id(c, t);
+      walk.advance(c, WPH);
+      t += WPH;
+    }
+    next_page = page_id(c, t);
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      copy(ld, ld_t, pages[s], s);
+      walk.advance(ld, WPH);
+      ld_t += WPH;
+    }
+  }
+
+  // ldmatrix addresses of this lane within a tile's codes: rows 0-7 and 8-15 of
+  // one chunk, then of the next (a row of one chunk: rows 0-31)
+  uint32_t mat[NB >= 2 ? NB / 2 : 1];
+  if constexpr (NB >= 2) {
+    const uint32_t r = (lane & 7) + ((lane >> 3) & 1) * 8;
+#pragma unroll
+    for (int jj = 0; jj < NB / 2; ++jj) mat[jj] = r * TR::ROW + (((2 * jj + (lane >> 4)) ^ TR::swz(r)) << 4);
+  } else {
+    mat[0] = lane * TR::ROW;
+  }
+  // codes of blocks 2jj and 2jj + 1 (or the one) of the 16 tokens m: lower and upper 8 rows of each
+  const int gl = lane >> 2, tl = lane & 3;
+
+  uint32_t qf[NT][NB][4];
+  auto load_q = [&](const Fp4Cursor& c) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int g = nt * 8 + gl;
+      const __half* qr = p.q + c.b * p.q0 + (int64_t)((c.hg * HG + hl) * G + g) * p.q1 + 8 * tl;
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (g < G) x = __ldg(reinterpret_cast<const uint4*>(qr + j * 32));
+        qf[nt][j][0] = x.x;
+        qf[nt][j][1] = x.y;
+        qf[nt][j][2] = x.z;
+        qf[nt][j][3] = x.w;
+      }
+    }
+  };
+  load_q(seg);
+
+  float acc[NB][2][NT][4];
+  float m_run[NT][2], l_run[NT][2];
+  int k = t0 + turn, stage = 0;  // this warp's next tile and its ring slot
+  int seg_t = t0;                // first tile of the segment in this CTA
+  for (;;) {
+    const int seg_end = min(t1, seg.start + seg.n);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m_run[nt][0] = m_run[nt][1] = -INFINITY;
+      l_run[nt][0] = l_run[nt][1] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[j][x][nt][0] = acc[j][x][nt][1] = acc[j][x][nt][2] = acc[j][x][nt][3] = 0.f;
+
+    for (; k < seg_end; k += WPH) {
+      cp_async_wait_group<S - 1>();
+      __syncwarp();
+      const uint32_t kb = ring + stage * TR::STAGE, vb = kb + TR::CODES, sb = vb + TR::CODES;
+      const int tok0 = (k - seg.start) * TT, nv = seg.seq - tok0;
+      // ---- scales, a lane per token: K's blocks in fp32 with the softmax scale
+      // and log2 e folded in, V's as fp16, laid out as the fragments want them:
+      // pairs of neighbouring tokens
+      {
+        uint32_t kw, vw;
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(kw) : "r"(sb + lane * 4));
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vw) : "r"(sb + TT * 4 + lane * 4));
+        float kf[4], vf[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          kf[j] = j < NB ? fp4_scale_f32((kw >> (8 * j)) & 255u) * p.scale_log2 : 0.f;
+          vf[j] = j < NB ? fp4_scale_f32((vw >> (8 * j)) & 255u) : 0.f;
+        }
+        asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(scratch + lane * 16), "f"(kf[0]), "f"(kf[1]),
+                     "f"(kf[2]), "f"(kf[3])
+                     : "memory");
+        const uint32_t v01 = pack_half2(vf[0], vf[1]), v23 = pack_half2(vf[2], vf[3]);
+        const bool odd = lane & 1;
+        // an even lane makes the pairs of blocks 0 and 1, its neighbour of 2 and 3
+        const uint32_t mine = odd ? v23 : v01, theirs = __shfl_xor_sync(0xffffffffu, odd ? v01 : v23, 1);
+        const uint32_t first = odd ? theirs : mine, second = odd ? mine : theirs;
+        asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(scratch + TT * 16 + (lane >> 1) * 16 + (lane & 1) * 8),
+                     "r"(__byte_perm(first, second, 0x5410)), "r"(__byte_perm(first, second, 0x7632))
+                     : "memory");
+        __syncwarp();
+      }
+      // ---- S^T = K . Q^T, block by block
+      float sc[2][NT][4];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        float4 f[2];  // scales of rows gl and gl + 8
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(f[x].x), "=f"(f[x].y), "=f"(f[x].z), "=f"(f[x].w)
+                       : "r"(scratch + (m * 16 + x * 8 + gl) * 16));
+        const float f0[4] = {f[0].x, f[0].y, f[0].z, f[0].w}, f1[4] = {f[1].x, f[1].y, f[1].z, f[1].w};
+        uint32_t r[2 * NB];  // [block][rows gl / gl + 8]
+        if constexpr (NB >= 2) {
+#pragma unroll
+          for (int jj = 0; jj < NB / 2; ++jj)
+            ldsm_x4(kb + m * 16 * TR::ROW + mat[jj], r[4 * jj], r[4 * jj + 1], r[4 * jj + 2], r[4 * jj + 3]);
+        } else {
+          uint32_t a, b;
+          if (m == 0) ldsm_x4(kb + mat[0], r[0], r[1], a, b);
+          else ldsm_x4(kb + mat[0], a, b, r[0], r[1]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) sc[m][nt][0] = sc[m][nt][1] = sc[m][nt][2] = sc[m][nt][3] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
+          fp4_unpack4(r[2 * j], a0, a1, a2, a3);
+          fp4_unpack4(r[2 * j + 1], b0, b1, b2, b3);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_16816(d, a0, b0, a1, b1, qf[nt][j][0], qf[nt][j][1]);
+            mma_16816(d, a2, b2, a3, b3, qf[nt][j][2], qf[nt][j][3]);
+            sc[m][nt][0] += d[0] * f0[j];
+            sc[m][nt][1] += d[1] * f0[j];
+            sc[m][nt][2] += d[2] * f1[j];
+            sc[m][nt][3] += d[3] * f1[j];
+          }
+        }
+      }
+      if (nv < TT) {
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (m * 16 + gl + (e >> 1) * 8 >= nv) sc[m][nt][e] = -INFINITY;
+      }
+      if constexpr (TR::WT) {
+        if (k < p.track.raw_tiles) {
+          float* raw = p.track.raw + (int64_t)k * (HG * G * TT) + hl * G * TT + gl;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int g = nt * 8 + 2 * tl + j;
+              if (g >= G) continue;
+#pragma unroll
+              for (int m = 0; m < 2; ++m) {
+                raw[g * TT + m * 16] = sc[m][nt][j];
+                raw[g * TT + m * 16 + 8] = sc[m][nt][j + 2];
+              }
+            }
+          if (hl == 0 && lane == 0) p.track.tiles[k] = make_int4(seg.b, seg.hg, k - seg.start, seg.seq);
+        } else if (lane == 0 && p.error_flags != nullptr) {
+          atomicOr(p.error_flags, PAD_FLAG_SHARED_PAGE);
+        }
+      }
+      // ---- online softmax over the 32 tokens
+      float alpha[NT][2];
+      bool grew = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float mx = fmaxf(fmaxf(sc[0][nt][j], sc[0][nt][j + 2]), fmaxf(sc[1][nt][j], sc[1][nt][j + 2]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float mn = fmaxf(m_run[nt][j], mx), mu = mn == -INFINITY ? 0.f : mn;
+          grew |= mn > m_run[nt][j];
+          alpha[nt][j] = ex2(m_run[nt][j] - mu);
+          m_run[nt][j] = mn;
+          float sum = 0.f;
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            sc[m][nt][j] = ex2(sc[m][nt][j] - mu);
+            sc[m][nt][j + 2] = ex2(sc[m][nt][j + 2] - mu);
+            sum += sc[m][nt][j] + sc[m][nt][j + 2];
+          }
+          l_run[nt][j] = l_run[nt][j] * alpha[nt][j] + sum;
+        }
+      if (__any_sync(0xffffffffu, grew)) {
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              acc[j][x][nt][0] *= alpha[nt][0];
+              acc[j][x][nt][1] *= alpha[nt][1];
+              acc[j][x][nt][2] *= alpha[nt][0];
+              acc[j][x][nt][3] *= alpha[nt][1];
+            }
+      }
+      // ---- O^T += V^T . (P_hi + P_lo)^T
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        uint32_t ph[NT][2], pl[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const float y0 = sc[m][nt][2 * x], y1 = sc[m][nt][2 * x + 1];
+            const __half2 hi = __floats2half2_rn(y0, y1);
+            const float2 hf = __half22float2(hi);
+            ph[nt][x] = movmatrix_trans(*reinterpret_cast<const uint32_t*>(&hi));
+            pl[nt][x] = movmatrix_trans(pack_half2(y0 - hf.x, y1 - hf.y));
+          }
+        uint4 s[2];  // scale pairs of tokens 2 tl, 2 tl + 1 and of those 8 on, per block
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(s[x].x), "=r"(s[x].y), "=r"(s[x].z), "=r"(s[x].w)
+                       : "r"(scratch + TT * 16 + (m * 8 + x * 4 + tl) * 16));
+        const uint32_t s0[4] = {s[0].x, s[0].y, s[0].z, s[0].w}, s1[4] = {s[1].x, s[1].y, s[1].z, s[1].w};
+        uint32_t r[2 * NB];
+        if constexpr (NB >= 2) {
+#pragma unroll
+          for (int jj = 0; jj < NB / 2; ++jj)
+            ldsm_x4_trans(vb + m * 16 * TR::ROW + mat[jj], r[4 * jj], r[4 * jj + 1], r[4 * jj + 2], r[4 * jj + 3]);
+        } else {
+          uint32_t a, b;
+          if (m == 0) ldsm_x4_trans(vb + mat[0], r[0], r[1], a, b);
+          else ldsm_x4_trans(vb + mat[0], a, b, r[0], r[1]);
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+          // bytes: token 2 tl dims (0 1), (2 3); token 2 tl + 1 dims (0 1), (2 3)
+          uint32_t a[4], c[4];
+          fp4_unpack4(r[2 * j], a[0], a[1], a[2], a[3]);
+          fp4_unpack4(r[2 * j + 1], c[0], c[1], c[2], c[3]);
+          const __half2 sa = *reinterpret_cast<const __half2*>(&s0[j]), sc8 = *reinterpret_cast<const __half2*>(&s1[j]);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {  // dims 4 gl + 2 x and the next
+            auto pair = [](uint32_t lo, uint32_t hi, uint32_t sel, __half2 f) {
+              const uint32_t y = __byte_perm(lo, hi, sel);
+              const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y), f);
+              return *reinterpret_cast<const uint32_t*>(&z);
+            };
+            const uint32_t a0 = pair(a[x], a[x + 2], 0x5410, sa), a1 = pair(a[x], a[x + 2], 0x7632, sa);
+            const uint32_t a2 = pair(c[x], c[x + 2], 0x5410, sc8), a3 = pair(c[x], c[x + 2], 0x7632, sc8);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_16816(acc[j][x][nt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
+              mma_16816(acc[j][x][nt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
+            }
+          }
+        }
+      }
+      // ---- the slot is free: copy the tile S turns on into it
+      __syncwarp();
+      copy(ld, ld_t, next_page, stage);
+      walk.advance(ld, WPH);
+      ld_t += WPH;
+      next_page = page_id(ld, ld_t);
+      if (++stage == S) stage = 0;
+    }
+
+    // ---- end of the segment: join the warps of each head
+    const bool split = !(seg.start >= t0 && seg.start + seg.n <= t1);
+    const Fp4Cursor done = seg;
+    const int pair = seg.b * ngroups + seg.hg, slot = pair + w;
+    if (tid == 0 && seg_t == seg.start) {
+      const int owner = split ? part_owner((int64_t)seg.start + seg.n - 1, total, W) : w;
+      if (split || p.meta_by_pair)
+        p.ws_meta[p.meta_by_pair ? pair : w] =
+            split ? make_int4(pair, slot, owner - w + 1, 1) : make_int4(-1, 0, 0, 0);
+      if constexpr (TR::WT) p.track.pairs[pair] = make_int2(slot, owner - w + 1);
+    }
+    const bool more = seg_end < t1;
+    if (more) {  // the next segment's queries arrive while this one is joined
+      seg_t = seg_end;
+      walk.next_pair(seg);
+      load_q(seg);
+    }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float l = l_run[nt][j];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        const int g = nt * 8 + 2 * tl + j;
+        if (gl == 0) sml[warp * TR::ROWS + g] = make_float2(m_run[nt][j], l);
+        if (g < G) {
+          float* row = epi + (warp * TR::ROWS + g) * TR::LD + 4 * gl;
+#pragma unroll
+          for (int blk = 0; blk < NB; ++blk)
+            *reinterpret_cast<float4*>(row + blk * 32) =
+                make_float4(acc[blk][0][nt][j], acc[blk][0][nt][j + 2], acc[blk][1][nt][j], acc[blk][1][nt][j + 2]);
+        }
+      }
+    __syncthreads();
+    for (int x = tid; x < HG * G * (D / 4); x += TR::THREADS) {
+      const int row = x / (D / 4), d = (x % (D / 4)) * 4;
+      const int h = row / G, g = row - h * G;
+      const float2* ml = sml + h * WPH * TR::ROWS + g;
+      const float* src = epi + (h * WPH * TR::ROWS + g) * TR::LD + d;
+      float M = -INFINITY, L = 0.f;
+      for (int x2 = 0; x2 < WPH; ++x2) M = fmaxf(M, ml[x2 * TR::ROWS].x);
+      const float Mu = M == -INFINITY ? 0.f : M;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int x2 = 0; x2 < WPH; ++x2) {
+        const float2 y = ml[x2 * TR::ROWS];
+        const float f = ex2(y.x - Mu);
+        const float4 z = *reinterpret_cast<const float4*>(src + x2 * TR::ROWS * TR::LD);
+        L += y.y * f;
+        o.x += z.x * f;
+        o.y += z.y * f;
+        o.z += z.z * f;
+        o.w += z.w * f;
+      }
+      if (split) {
+        *reinterpret_cast<float4*>(p.ws_o + ((int64_t)slot * HG * G + row) * D + d) = o;
+      } else {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+        __half2* out = reinterpret_cast<__half2*>(p.out + done.b * p.out_sb +
+                                                  (int64_t)(done.hg * HG * G + row) * p.out_sh + d);
+        out[0] = __floats2half2_rn(o.x * inv, o.y * inv);
+        out[1] = __floats2half2_rn(o.z * inv, o.w * inv);
+      }
+      if ((split || TR::WT) && d == 0) p.ws_ml[(int64_t)slot * HG * G + row] = make_float2(Mu, L);
+    }
+    if (!more) break;
+    __syncthreads();  // the buffers are read before the next segment writes them
+  }
+  cp_async_wait_all();
+}
+
+}  // namespace pad

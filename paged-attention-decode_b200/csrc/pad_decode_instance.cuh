@@ -62,6 +62,26 @@ bool pick_decode(int64_t head_dim, int64_t gqa, int hg, bool swz, Instance* out)
   }
 }
 
+// Phase 2 of a decode, launched as a programmatic dependent of phase 1
+// (pad_decode.cu): joins the partials of the split pairs.
+struct MergeLaunch {
+  const float* ws_o;
+  const float2* ws_ml;
+  const int4* ws_meta;
+  __half* out;
+  int64_t out_sb, out_sh;
+  int ngroups, rows;            // head groups; query rows of one
+  int guess_ncap, guess_parts;  // closed-form descriptors (guess_ncap 0: none)
+  int64_t batch, partitions, head_dim;
+  int meta_by_pair;
+};
+int launch_merge(const MergeLaunch& m, cudaStream_t stream);
+
+// KV heads per tile, and the SM count of a device (pad_decode.cu).
+int head_group_for(int64_t hkv, int64_t gqa);
+int sm_count(int device, int* num_sms);
+constexpr int64_t kFewPairs = 16;  // see the num_splits=None heuristic of pad_decode.cu
+
 // The instances that keep their scores (pad_decode_weights.cu).
 bool pick_decode_weights(int64_t head_dim, int64_t gqa, int hg, bool swz, Instance* out);
 

@@ -207,7 +207,8 @@ def test_strides_streams_and_graph():
     with torch.cuda.stream(side):
         a = pad_b200.paged_attention_decode_fp4(unaligned, *cg, btg, slg, scale=0.2)
     side.synchronize()
-    assert torch.equal(a, out)
+    # (a narrower table may split the sequences otherwise, so not bit for bit)
+    assert_parity(a.float().cpu().numpy(), ref)
     graph = torch.cuda.CUDAGraph()
     w = torch.zeros(k.shape[0], 3, 16, device="cuda")
     pad_b200.paged_attention_decode_fp4(unaligned, *cg, btg, slg, scale=0.2, weights=w)
