@@ -109,19 +109,11 @@ int make_plan(int device, int64_t batch, int64_t hkv, int64_t gqa, int64_t head_
   return PAD_OK;
 }
 
-// Offsets within a code cache are kept in 32 bits, in units of the largest
-// power of two (16 to 64 bytes) that divides every stride; the largest must fit.
-int offset_shift(const int64_t* k, const int64_t* v, int64_t pages, int64_t ps, int64_t hkv) {
-  uint64_t all = 0;
-  for (int i = 0; i < 3; ++i) all |= (uint64_t)k[i] | (uint64_t)v[i];
-  int shift = 4;
-  while (shift < 6 && (all >> shift) % 2 == 0) ++shift;
-  for (const int64_t* s : {k, v}) {
-    if (s[0] < 0 || s[1] < 0 || s[2] < 0) return -1;
-    const double last = (double)(pages - 1) * (double)s[0] + (double)(ps - 1) * (double)s[1] + (double)(hkv - 1) * (double)s[2];
-    if (pages > 0 && last / (double)(1 << shift) >= 4294967296.0) return -1;
-  }
-  return shift;
+// Whether every offset of a tensor of these strides stays below 2^32 units.
+bool offsets_fit(const int64_t* s, int64_t pages, int64_t ps, int64_t hkv, int unit) {
+  if (s[0] < 0 || s[1] < 0 || s[2] < 0) return false;
+  const double last = (double)(pages - 1) * (double)s[0] + (double)(ps - 1) * (double)s[1] + (double)(hkv - 1) * (double)s[2];
+  return pages == 0 || last / unit < 4294967296.0;
 }
 
 }  // namespace
@@ -189,9 +181,20 @@ extern "C" int pad_paged_attention_decode_fp4(
   int st = make_plan(0, batch, num_kv_heads, gqa, head_dim, num_pages, page_size, max_pages_per_seq,
                      std::max<int64_t>(num_splits, 1), weights != nullptr, &plan);
   if (st != PAD_OK) return st;
-  const int shift = offset_shift(k_strides, v_strides, num_pages, page_size, num_kv_heads);
-  if (shift < 0)
-    return fail(PAD_ERR_UNSUPPORTED, "%s: cache strides are negative or reach past 2^32 units of 16 to 64 bytes", what);
+  // Offsets are kept in 32 bits, those of codes in units of the largest power of
+  // two (16 to 64 bytes) that divides every stride.
+  uint64_t all = 0;
+  for (int i = 0; i < 3; ++i) all |= (uint64_t)k_strides[i] | (uint64_t)v_strides[i];
+  int unit = 16;
+  while (unit < 64 && all % (2 * unit) == 0) unit *= 2;
+  if (!offsets_fit(k_strides, num_pages, page_size, num_kv_heads, unit) ||
+      !offsets_fit(v_strides, num_pages, page_size, num_kv_heads, unit) ||
+      !offsets_fit(ks_strides, num_pages, page_size, num_kv_heads, kFp4ScaleRow) ||
+      !offsets_fit(vs_strides, num_pages, page_size, num_kv_heads, kFp4ScaleRow))
+    return fail(PAD_ERR_UNSUPPORTED,
+                "%s: cache strides are negative or reach past 2^32 units (codes: %d bytes, scales: 4)", what, unit);
+  if (block_table_stride > INT32_MAX)
+    return fail(PAD_ERR_UNSUPPORTED, "%s: block_table row stride exceeds int32", what);
   if ((e = cudaGetDevice(&device)) != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   if (num_splits <= 0 && (st = make_plan(device, batch, num_kv_heads, gqa, head_dim, num_pages, page_size,
                                          max_pages_per_seq, num_splits, weights != nullptr, &plan)) != PAD_OK)
@@ -220,21 +223,22 @@ extern "C" int pad_paged_attention_decode_fp4(
   p.error_flags = error_flags;
   p.q0 = q_strides[0];
   p.q1 = q_strides[1];
-  p.bt_stride = block_table_stride;
+  p.bt_stride = (int)block_table_stride;
   p.out_sb = out_strides[0];
   p.out_sh = out_strides[1];
-  p.k0 = k_strides[0] >> shift;
-  p.k1 = k_strides[1] >> shift;
-  p.k2 = k_strides[2] >> shift;
-  p.v0 = v_strides[0] >> shift;
-  p.v1 = v_strides[1] >> shift;
-  p.v2 = v_strides[2] >> shift;
-  p.ks0 = ks_strides[0];
-  p.ks1 = ks_strides[1];
-  p.ks2 = ks_strides[2];
-  p.vs0 = vs_strides[0];
-  p.vs1 = vs_strides[1];
-  p.vs2 = vs_strides[2];
+  p.unit = (uint32_t)unit;
+  p.k0 = (uint32_t)(k_strides[0] / unit);
+  p.k1 = (uint32_t)(k_strides[1] / unit);
+  p.k2 = (uint32_t)(k_strides[2] / unit);
+  p.v0 = (uint32_t)(v_strides[0] / unit);
+  p.v1 = (uint32_t)(v_strides[1] / unit);
+  p.v2 = (uint32_t)(v_strides[2] / unit);
+  p.ks0 = (uint32_t)(ks_strides[0] / kFp4ScaleRow);
+  p.ks1 = (uint32_t)(ks_strides[1] / kFp4ScaleRow);
+  p.ks2 = (uint32_t)(ks_strides[2] / kFp4ScaleRow);
+  p.vs0 = (uint32_t)(vs_strides[0] / kFp4ScaleRow);
+  p.vs1 = (uint32_t)(vs_strides[1] / kFp4ScaleRow);
+  p.vs2 = (uint32_t)(vs_strides[2] / kFp4ScaleRow);
   p.batch = (int)batch;
   p.hkv = (int)num_kv_heads;
   p.gqa = (int)gqa;
@@ -243,8 +247,8 @@ extern "C" int pad_paged_attention_decode_fp4(
   p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)page_size) : -1;
   p.num_pages = (int)num_pages;
   p.max_pages = (int)max_pages_per_seq;
-  p.off_shift = shift;
-  p.same_off = p.k0 == p.v0 && p.k1 == p.v1 && p.k2 == p.v2;
+  p.same_codes = p.k0 == p.v0 && p.k1 == p.v1 && p.k2 == p.v2;
+  p.same_scales = p.ks0 == p.vs0 && p.ks1 == p.vs1 && p.ks2 == p.vs2;
   const int64_t pairs = batch * (num_kv_heads / plan.hg);
   p.meta_by_pair = pairs < plan.partitions ? 1 : 0;
   p.scale_log2 = scale * kLog2e;

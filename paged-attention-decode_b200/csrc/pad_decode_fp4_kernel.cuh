@@ -46,11 +46,12 @@ struct Fp4DecodeParams {
   float2* ws_ml;
   int4* ws_meta;
   int32_t* error_flags;
-  int64_t q0, q1, bt_stride, out_sb, out_sh;
-  int64_t k0, k1, k2, v0, v1, v2;          // code strides in units of 2^off_shift bytes
-  int64_t ks0, ks1, ks2, vs0, vs1, vs2;    // scale strides in bytes
-  int batch, hkv, gqa, hg_log2, page_size, page_shift, num_pages, max_pages;
-  int off_shift, same_off;                 // K and V have the same strides
+  int64_t q0, q1, out_sb, out_sh;
+  // Offsets fit 32 bits: code strides in units of `unit` bytes, scale strides in
+  // words of 4.
+  uint32_t k0, k1, k2, v0, v1, v2, ks0, ks1, ks2, vs0, vs1, vs2, unit;
+  int batch, hkv, gqa, hg_log2, page_size, page_shift, num_pages, max_pages, bt_stride;
+  int same_codes, same_scales;  // K and V have the same strides
   int meta_by_pair;
   float scale_log2;
   TrackParams track;
@@ -239,6 +240,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
   const uint64_t policy = l2_evict_first_policy();
   const uint32_t chunk = lane % TR::CPR, row_of_lane = lane / TR::CPR;
   const uint32_t copy_dst = row_of_lane * TR::ROW + ((chunk ^ TR::swz(row_of_lane)) << 4);
+  const uint8_t *k_chunk = p.k + chunk * 16, *v_chunk = p.v + chunk * 16;
   Fp4Cursor ld = seg;     // next tile to copy
   int ld_t = t0 + turn;
   walk.advance(ld, turn);
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
     const int tok = c.i * TT + lane;
     if (t >= t1 || tok >= c.seq) return -1;
     const int lp = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size;
-    return ld_nc_early(p.block_table + c.b * p.bt_stride + lp);
+    return ld_nc_early(p.block_table + (int64_t)c.b * p.bt_stride + lp);
   };
   auto copy = [&](const Fp4Cursor& c, int t, int page, int stage) {
     if (t < t1) {
@@ -255,24 +257,26 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
       const bool live = tok < c.seq, ok = live && (unsigned)page < (unsigned)p.num_pages;
       if (live && !ok && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_BAD_PAGE_ID);
       const int row = p.page_shift >= 0 ? tok & (p.page_size - 1) : tok % p.page_size;
-      const uint32_t good = __ballot_sync(0xffffffffu, ok);
-      const int64_t pg = ok ? page : 0, rw = ok ? row : 0;
-      const uint32_t ko = (uint32_t)(pg * p.k0 + rw * p.k1 + h * p.k2);
-      const uint32_t vo = (uint32_t)(pg * p.v0 + rw * p.v1 + h * p.v2);
+      const uint32_t good = __ballot_sync(0xffffffffu, ok) >> row_of_lane;
+      const uint32_t pg = ok ? page : 0, rw = ok ? row : 0;
+      const uint32_t ko = pg * p.k0 + rw * p.k1 + h * p.k2;
+      const uint32_t vo = p.same_codes ? ko : pg * p.v0 + rw * p.v1 + h * p.v2;
+      const uint32_t kso = pg * p.ks0 + rw * p.ks1 + h * p.ks2;
+      const uint32_t vso = p.same_scales ? kso : pg * p.vs0 + rw * p.vs1 + h * p.vs2;
       const uint32_t base = ring + stage * TR::STAGE;
 #pragma unroll
       for (int x = 0; x < TR::CPR; ++x) {
-        const int r = row_of_lane + x * (32 / TR::CPR);
-        const uint32_t bytes = (good >> r) & 1u ? 16u : 0u;
-        const uint32_t kr = __shfl_sync(0xffffffffu, ko, r);
-        const uint32_t vr = p.same_off ? kr : __shfl_sync(0xffffffffu, vo, r);
-        const uint32_t dst = base + copy_dst + x * (32 / TR::CPR) * TR::ROW;
-        cp_async_16(dst, p.k + ((uint64_t)kr << p.off_shift) + chunk * 16, bytes, policy);
-        cp_async_16(dst + TR::CODES, p.v + ((uint64_t)vr << p.off_shift) + chunk * 16, bytes, policy);
+        constexpr int STEP = 32 / TR::CPR;  // rows between a lane's chunks
+        const uint32_t bytes = ((good >> (x * STEP)) & 1u) << 4;
+        const uint32_t kr = __shfl_sync(0xffffffffu, ko, row_of_lane + x * STEP);
+        const uint32_t vr = p.same_codes ? kr : __shfl_sync(0xffffffffu, vo, row_of_lane + x * STEP);
+        const uint32_t dst = base + copy_dst + x * STEP * TR::ROW;
+        cp_async_16(dst, k_chunk + (uint64_t)kr * p.unit, bytes, policy);
+        cp_async_16(dst + TR::CODES, v_chunk + (uint64_t)vr * p.unit, bytes, policy);
       }
       const uint32_t sdst = base + 2 * TR::CODES + lane * kFp4ScaleRow;
-      cp_async_4z(sdst, p.ks + pg * p.ks0 + rw * p.ks1 + h * p.ks2, ok ? 4u : 0u);
-      cp_async_4z(sdst + TT * kFp4ScaleRow, p.vs + pg * p.vs0 + rw * p.vs1 + h * p.vs2, ok ? 4u : 0u);
+      cp_async_4z(sdst, p.ks + (uint64_t)kso * 4u, ok ? 4u : 0u);
+      cp_async_4z(sdst + TT * kFp4ScaleRow, p.vs + (uint64_t)vso * 4u, ok ? 4u : 0u);
     }
     cp_async_commit();
   };
@@ -357,16 +361,15 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
         uint32_t kw, vw;
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(kw) : "r"(sb + lane * 4));
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vw) : "r"(sb + TT * 4 + lane * 4));
-        float kf[4], vf[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          kf[j] = j < NB ? fp4_scale_f32((kw >> (8 * j)) & 255u) * p.scale_log2 : 0.f;
-          vf[j] = j < NB ? fp4_scale_f32((vw >> (8 * j)) & 255u) : 0.f;
-        }
+        const uint32_t k01 = fp4_scale2_bf16(kw), k23 = fp4_scale2_bf16(kw >> 16);
+        const uint32_t w01 = fp4_scale2_bf16(vw), w23 = fp4_scale2_bf16(vw >> 16);
+        const float kf[4] = {__uint_as_float(k01 << 16) * p.scale_log2, __uint_as_float(k01 & 0xffff0000u) * p.scale_log2,
+                             __uint_as_float(k23 << 16) * p.scale_log2, __uint_as_float(k23 & 0xffff0000u) * p.scale_log2};
         asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(scratch + lane * 16), "f"(kf[0]), "f"(kf[1]),
                      "f"(kf[2]), "f"(kf[3])
                      : "memory");
-        const uint32_t v01 = pack_half2(vf[0], vf[1]), v23 = pack_half2(vf[2], vf[3]);
+        const uint32_t v01 = pack_half2(__uint_as_float(w01 << 16), __uint_as_float(w01 & 0xffff0000u));
+        const uint32_t v23 = pack_half2(__uint_as_float(w23 << 16), __uint_as_float(w23 & 0xffff0000u));
         const bool odd = lane & 1;
         // an even lane makes the pairs of blocks 0 and 1, its neighbour of 2 and 3
         const uint32_t mine = odd ? v23 : v01, theirs = __shfl_xor_sync(0xffffffffu, odd ? v01 : v23, 1);
@@ -515,20 +518,28 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
         }
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
-          // bytes: token 2 tl dims (0 1), (2 3); token 2 tl + 1 dims (0 1), (2 3)
-          uint32_t a[4], c[4];
-          fp4_unpack4(r[2 * j], a[0], a[1], a[2], a[3]);
-          fp4_unpack4(r[2 * j + 1], c[0], c[1], c[2], c[3]);
-          const __half2 sa = *reinterpret_cast<const __half2*>(&s0[j]), sc8 = *reinterpret_cast<const __half2*>(&s1[j]);
+          // A register holds four codes (dims 4 gl ..) of token 2 tl in its low
+          // half, of the next token in its high half; r[2j] of the lower, r[2j+1]
+          // of the upper 8 tokens. Nibbles are paired across the two tokens before
+          // the conversion, so that it yields (token, next token) of one dim:
+          // bytes of `even` are dims 0 and 2 of the lower, then of the upper
+          // tokens, of `odd` dims 1 and 3.
+          const uint32_t own = __byte_perm(r[2 * j], r[2 * j + 1], 0x5410);
+          const uint32_t nxt = __byte_perm(r[2 * j], r[2 * j + 1], 0x7632);
+          const uint32_t even = (own & 0x0f0f0f0fu) | ((nxt << 4) & 0xf0f0f0f0u);
+          const uint32_t odd = ((own >> 4) & 0x0f0f0f0fu) | (nxt & 0xf0f0f0f0u);
+          uint32_t e[4], o[4];
+          fp4_unpack4(even, e[0], e[1], e[2], e[3]);
+          fp4_unpack4(odd, o[0], o[1], o[2], o[3]);
+          const __half2 lower = *reinterpret_cast<const __half2*>(&s0[j]), upper = *reinterpret_cast<const __half2*>(&s1[j]);
+          auto scaled = [](uint32_t y, __half2 f) {
+            const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y), f);
+            return *reinterpret_cast<const uint32_t*>(&z);
+          };
 #pragma unroll
           for (int x = 0; x < 2; ++x) {  // dims 4 gl + 2 x and the next
-            auto pair = [](uint32_t lo, uint32_t hi, uint32_t sel, __half2 f) {
-              const uint32_t y = __byte_perm(lo, hi, sel);
-              const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y), f);
-              return *reinterpret_cast<const uint32_t*>(&z);
-            };
-            const uint32_t a0 = pair(a[x], a[x + 2], 0x5410, sa), a1 = pair(a[x], a[x + 2], 0x7632, sa);
-            const uint32_t a2 = pair(c[x], c[x + 2], 0x5410, sc8), a3 = pair(c[x], c[x + 2], 0x7632, sc8);
+            const uint32_t a0 = scaled(e[x], lower), a1 = scaled(o[x], lower);
+            const uint32_t a2 = scaled(e[x + 2], upper), a3 = scaled(o[x + 2], upper);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               mma_16816(acc[j][x][nt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);

@@ -39,6 +39,13 @@ __device__ __forceinline__ void fp4_unpack4(uint32_t w, uint32_t& h0, uint32_t& 
       : "r"(w));
 }
 
+// Two scale bytes (low 16 bits) -> 2^(byte - 127) as two bf16, exactly, 255 as NaN.
+__device__ __forceinline__ uint32_t fp4_scale2_bf16(uint32_t two) {
+  uint32_t y;
+  asm("{\n\t.reg .b16 x;\n\tcvt.u16.u32 x, %1;\n\tcvt.rn.bf16x2.ue8m0x2 %0, x;\n\t}" : "=r"(y) : "r"(two));
+  return y;
+}
+
 // Eight fp32 values -> four code bytes, rounded to nearest even and saturated
 // at +-6 (x[0] in the lowest nibble).
 __device__ __forceinline__ uint32_t fp4_pack8(const float (&x)[8]) {
