@@ -244,8 +244,8 @@ int pad_paged_kv_read_fp4(const void* k_cache, const void* k_scales, const void*
  * 16-byte aligned with strides that are multiples of 8 elements, out 4-byte
  * aligned with even strides. weights, slot_positions, total_lens and num_new
  * are those of pad_paged_attention_decode_weights below; weights NULL leaves
- * them out. num_splits >= 1: partitions per (sequence, KV head group), as for
- * the decode. The workspace (pad_decode_fp4_workspace_bytes; with_weights 0 or
+ * them out. num_splits >= 1: partitions per (sequence, group of up to 4 KV
+ * heads). The workspace (pad_decode_fp4_workspace_bytes; with_weights 0 or
  * 1; num_pages matters with weights alone) needs no initialisation. A bad page
  * id reads as zero rows. */
 int pad_decode_fp4_workspace_bytes(int device, int64_t batch, int64_t num_kv_heads, int64_t gqa_ratio,

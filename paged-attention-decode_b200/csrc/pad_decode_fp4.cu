@@ -75,7 +75,8 @@ int make_plan(int device, int64_t batch, int64_t hkv, int64_t gqa, int64_t head_
   if (num_pages > INT32_MAX || max_pages > INT32_MAX || page_size > INT32_MAX || hkv > INT32_MAX ||
       max_pages * page_size > INT32_MAX / 2)
     return fail(PAD_ERR_UNSUPPORTED, "%s: problem too large for 32-bit indexing", what);
-  plan->hg = head_group_for(hkv, gqa);
+  // KV heads per tile: what divides the kernel's 12 or 8 warps
+  plan->hg = std::min(4, head_group_for(hkv, gqa));
   const int64_t groups = hkv / plan->hg, tiles = (max_pages * page_size + kTile - 1) / kTile;
   if (batch > INT32_MAX / 4 / groups || batch * groups > INT32_MAX / 4 / std::max<int64_t>(tiles, 1))
     return fail(PAD_ERR_UNSUPPORTED, "%s: problem too large for 32-bit indexing", what);
@@ -244,11 +245,15 @@ extern "C" int pad_paged_attention_decode_fp4(
   p.gqa = (int)gqa;
   p.hg_log2 = __builtin_ctz((unsigned)plan.hg);
   p.page_size = (int)page_size;
-  p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)page_size) : -1;
+  // division by page_size: with 2^(L - 1) < page_size <= 2^L, the multiplier
+  // floor(2^(31 + L) / page_size) + 1 is exact for every dividend below 2^31
+  int log2_up = 0;
+  while (((int64_t)1 << log2_up) < page_size) ++log2_up;
+  p.page_mul = (uint32_t)((((uint64_t)1 << (31 + log2_up)) / (uint64_t)page_size) + 1);
+  p.page_shr = log2_up;  // umulhi(2 t, mul) >> log2_up = (t * mul) >> (31 + log2_up)
   p.num_pages = (int)num_pages;
   p.max_pages = (int)max_pages_per_seq;
-  p.same_codes = p.k0 == p.v0 && p.k1 == p.v1 && p.k2 == p.v2;
-  p.same_scales = p.ks0 == p.vs0 && p.ks1 == p.vs1 && p.ks2 == p.vs2;
+  p.same_strides = p.k0 == p.v0 && p.k1 == p.v1 && p.k2 == p.v2 && p.ks0 == p.vs0 && p.ks1 == p.vs1 && p.ks2 == p.vs2;
   const int64_t pairs = batch * (num_kv_heads / plan.hg);
   p.meta_by_pair = pairs < plan.partitions ? 1 : 0;
   p.scale_log2 = scale * kLog2e;
@@ -315,7 +320,7 @@ extern "C" int pad_paged_attention_decode_fp4(
     wp.tt = kTile;
     wp.ngroups = (int)(num_kv_heads / plan.hg);
     wp.page_size = (int)page_size;
-    wp.page_shift = p.page_shift;
+    wp.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)page_size) : -1;
     wp.num_pages = (int)num_pages;
     wp.num_new = (int)std::min<int64_t>(num_new, INT32_MAX);
     if ((st = launch_weights(wp, s)) != PAD_OK) return st;

@@ -10,8 +10,8 @@
 // become fp16), so the kernel is built around the fewest instructions a value:
 //   - A warp owns whole (tile, head) pieces: WPH = warps / HG warps share a
 //     head and take turns at its tiles. It copies its own pieces into its own
-//     ring with cp.async and waits for nobody: no producer, no barriers between
-//     warps until a (sequence, head group) segment ends.
+//     ring with cp.async and waits for nobody: no producer, and barriers between
+//     the warps of a head only where a (sequence, head group) ends.
 //   - Codes go from shared memory to registers by ldmatrix on 16-bit units of
 //     four codes. For K a lane gets 8 consecutive dims of its row, for V
 //     (transposed) four dims of two neighbouring tokens. The order in which a
@@ -24,9 +24,9 @@
 //     contraction and go onto the values, one packed multiplication for two.
 //     Both are unpacked once per token through shared memory.
 //   - P is split into two fp16 terms as in the fp16 decode.
-// Tokens past the sequence, and pages that are none, are copied as zeros
-// (cp.async with no source bytes): zero codes with a finite scale, so nothing a
-// page holds behind its sequence can reach the sums.
+// Rows of tokens past the sequence, and of pages that are none, are copied as
+// zeros (cp.async with no source bytes): zero codes with a finite scale, so
+// nothing that a page holds behind its sequence reaches the sums.
 #pragma once
 
 #include <climits>
@@ -36,6 +36,8 @@
 #include "pad_fp4.cuh"
 
 namespace pad {
+
+constexpr int kFp4SeqCache = 512;  // seq_lens kept in shared memory
 
 struct Fp4DecodeParams {
   const __half* q;
@@ -50,18 +52,27 @@ struct Fp4DecodeParams {
   // Offsets fit 32 bits: code strides in units of `unit` bytes, scale strides in
   // words of 4.
   uint32_t k0, k1, k2, v0, v1, v2, ks0, ks1, ks2, vs0, vs1, vs2, unit;
-  int batch, hkv, gqa, hg_log2, page_size, page_shift, num_pages, max_pages, bt_stride;
-  int same_codes, same_scales;  // K and V have the same strides
+  // token / page_size = umulhi(2 * token, page_mul) >> page_shr, for tokens below 2^31
+  uint32_t page_mul, page_shr;
+  int batch, hkv, gqa, hg_log2, page_size, num_pages, max_pages, bt_stride;
+  int same_strides;  // K and V have the same ones
   int meta_by_pair;
   float scale_log2;
   TrackParams track;
 };
 
+// Where a running maximum starts: below every score, and finite, so that a
+// difference to it is never NaN.
+constexpr float kLeastScore = -1e30f;
+
 template <int D_, int NT_, bool WT_>
 struct Fp4Traits {
   static constexpr int D = D_, NT = NT_;
   static constexpr bool WT = WT_;
-  static constexpr int NW = NT == 1 ? 16 : 8;      // warps: 128 or 255 registers a thread
+  // Warps: 12 of 168 registers, 8 of 255 for two query tiles. 16 of 128 spend 70
+  // more instructions a tile on recomputing addresses (64 x 4096, 12/2 heads:
+  // 29.4 us against 28.5), 8 leave two warps a scheduler (30.8).
+  static constexpr int NW = NT == 1 ? 12 : 8;
   static constexpr int THREADS = 32 * NW;
   static constexpr int TT = 32;                    // tokens per tile
   static constexpr int NB = D / kFp4Block;         // blocks of 32 dims
@@ -69,8 +80,8 @@ struct Fp4Traits {
   static constexpr int CPR = ROW / 16;             // 16-byte chunks of a row
   static constexpr int CODES = TT * ROW;
   static constexpr int STAGE = 2 * CODES + 2 * TT * kFp4ScaleRow;
-  // about 136 KB of ring: one to two pieces in flight per warp at D = 128
-  static constexpr int FIT = 139264 / NW / STAGE;
+  // about 150 KB of ring: two or three pieces in flight per warp at D = 128
+  static constexpr int FIT = (NT == 1 ? 156672 : 139264) / NW / STAGE;
   static constexpr int STAGES = FIT > 6 ? 6 : FIT;
   static_assert(STAGES >= 2, "the ring needs two stages");
   static constexpr int SCRATCH = TT * 16 + TT / 2 * 16;  // unpacked scales of K (fp32) and V (fp16 pairs)
@@ -80,7 +91,7 @@ struct Fp4Traits {
   static constexpr int OFF_EPI = OFF_SCRATCH + NW * SCRATCH;
   static constexpr int OFF_ML = OFF_EPI + NW * ROWS * LD * 4;
   static constexpr int OFF_MISC = OFF_ML + NW * ROWS * 8;
-  static constexpr int SMEM_BYTES = OFF_MISC + 256 + kSeqCache * 4 + 128 /*align slack*/;
+  static constexpr int SMEM_BYTES = OFF_MISC + 256 + kFp4SeqCache * 4 + 128 /*align slack*/;
   static_assert(SMEM_BYTES <= kSmemBudget, "shared memory");
   // XOR on a row's chunk index that spreads ldmatrix's 8 rows over all banks
   __device__ static __forceinline__ uint32_t swz(uint32_t row) {
@@ -95,7 +106,11 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint3
                "l"(policy)
                : "memory");
 }
-__device__ __forceinline__ void cp_async_4z(uint32_t dst, const void* src, uint32_t bytes) {
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
@@ -111,7 +126,7 @@ struct Fp4Walk {
   const int* sseq;
   int cap, ngroups;
   __device__ __forceinline__ int seq_at(int b) const {
-    return b < kSeqCache ? sseq[b] : clamp_seq(__ldg(p.seq_lens + b), cap);
+    return b < kFp4SeqCache ? sseq[b] : clamp_seq(__ldg(p.seq_lens + b), cap);
   }
   __device__ __forceinline__ void next_pair(Fp4Cursor& c) const {
     c.start += c.n;
@@ -145,7 +160,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
   float2* sml = reinterpret_cast<float2*>(smem + TR::OFF_ML);     // [warp][ROWS]
   int* scan = reinterpret_cast<int*>(smem + TR::OFF_MISC);        // [16]
   int* cur = scan + 16;                                           // the first cursor
-  int* sseq = scan + 64;                                          // [kSeqCache]
+  int* sseq = scan + 64;                                          // [kFp4SeqCache]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cap = p.max_pages * p.page_size;
   const int64_t W = gridDim.x;
@@ -167,7 +182,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
       const int raw = __ldg(p.seq_lens + b), sq = clamp_seq(raw, cap);
       bad |= raw != sq;
       none |= sq == 0;
-      if (b < kSeqCache) sseq[b] = sq;
+      if (b < kFp4SeqCache) sseq[b] = sq;
       local += (sq + TT - 1) / TT;
     }
     local *= ngroups;
@@ -240,63 +255,82 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
   const uint64_t policy = l2_evict_first_policy();
   const uint32_t chunk = lane % TR::CPR, row_of_lane = lane / TR::CPR;
   const uint32_t copy_dst = row_of_lane * TR::ROW + ((chunk ^ TR::swz(row_of_lane)) << 4);
-  const uint8_t *k_chunk = p.k + chunk * 16, *v_chunk = p.v + chunk * 16;
   Fp4Cursor ld = seg;     // next tile to copy
   int ld_t = t0 + turn;
   walk.advance(ld, turn);
-  // The page id of this lane's token of the tile at `c` (-1: no token).
-  auto page_id = [&](const Fp4Cursor& c, int t) -> int {
-    const int tok = c.i * TT + lane;
-    if (t >= t1 || tok >= c.seq) return -1;
-    const int lp = p.page_shift >= 0 ? tok >> p.page_shift : tok / p.page_size;
-    return ld_nc_early(p.block_table + (int64_t)c.b * p.bt_stride + lp);
+  // Where this lane's token of a tile lies: its page (-1: it has no token) and
+  // row, and the tile. Page ids are loaded a turn before the copy that needs them.
+  struct Place {
+    int page, row, left;  // left: tokens of the sequence from the tile's first on (0: no tile)
+    uint32_t head;
   };
-  auto copy = [&](const Fp4Cursor& c, int t, int page, int stage) {
-    if (t < t1) {
-      const int tok = c.i * TT + lane, h = c.hg * HG + hl;
-      const bool live = tok < c.seq, ok = live && (unsigned)page < (unsigned)p.num_pages;
-      if (live && !ok && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_BAD_PAGE_ID);
-      const int row = p.page_shift >= 0 ? tok & (p.page_size - 1) : tok % p.page_size;
-      const uint32_t good = __ballot_sync(0xffffffffu, ok) >> row_of_lane;
-      const uint32_t pg = ok ? page : 0, rw = ok ? row : 0;
-      const uint32_t ko = pg * p.k0 + rw * p.k1 + h * p.k2;
-      const uint32_t vo = p.same_codes ? ko : pg * p.v0 + rw * p.v1 + h * p.v2;
-      const uint32_t kso = pg * p.ks0 + rw * p.ks1 + h * p.ks2;
-      const uint32_t vso = p.same_scales ? kso : pg * p.vs0 + rw * p.vs1 + h * p.vs2;
-      const uint32_t base = ring + stage * TR::STAGE;
-#pragma unroll
-      for (int x = 0; x < TR::CPR; ++x) {
-        constexpr int STEP = 32 / TR::CPR;  // rows between a lane's chunks
-        const uint32_t bytes = ((good >> (x * STEP)) & 1u) << 4;
-        const uint32_t kr = __shfl_sync(0xffffffffu, ko, row_of_lane + x * STEP);
-        const uint32_t vr = p.same_codes ? kr : __shfl_sync(0xffffffffu, vo, row_of_lane + x * STEP);
-        const uint32_t dst = base + copy_dst + x * STEP * TR::ROW;
-        cp_async_16(dst, k_chunk + (uint64_t)kr * p.unit, bytes, policy);
-        cp_async_16(dst + TR::CODES, v_chunk + (uint64_t)vr * p.unit, bytes, policy);
+  const int32_t* ids = p.block_table + (int64_t)ld.b * p.bt_stride;  // page ids of ld's sequence
+  int ids_of = ld.b;
+  auto place = [&](Place& o) {
+    o.left = 0;
+    if (ld_t < t1) {
+      if (ld.b != ids_of) {
+        ids_of = ld.b;
+        ids = p.block_table + (int64_t)ids_of * p.bt_stride;
       }
-      const uint32_t sdst = base + 2 * TR::CODES + lane * kFp4ScaleRow;
-      cp_async_4z(sdst, p.ks + (uint64_t)kso * 4u, ok ? 4u : 0u);
-      cp_async_4z(sdst + TT * kFp4ScaleRow, p.vs + (uint64_t)vso * 4u, ok ? 4u : 0u);
+      const int tok = ld.i * TT + lane;
+      const int lp = __umulhi(2u * (uint32_t)tok, p.page_mul) >> p.page_shr;
+      o.row = tok - lp * p.page_size;
+      o.left = ld.seq - ld.i * TT;
+      o.head = ld.hg * HG + hl;
+      o.page = lane < o.left ? ld_nc_early(ids + lp) : -1;
+      ld_t += WPH;
+      walk.advance(ld, WPH);
+    }
+  };
+  bool bad_page = false;
+  const uint8_t *k_chunk = p.k + chunk * 16, *v_chunk = p.v + chunk * 16;
+  auto copy = [&](const Place& at, int stage) {
+    if (at.left > 0) {
+      const bool ok = (unsigned)at.page < (unsigned)p.num_pages;
+      const uint32_t pg = ok ? at.page : 0, rw = ok ? at.row : 0;
+      const uint32_t ko = pg * p.k0 + rw * p.k1 + at.head * p.k2;
+      const uint32_t kso = pg * p.ks0 + rw * p.ks1 + at.head * p.ks2;
+      const uint32_t dst = ring + stage * TR::STAGE + copy_dst;
+      const uint32_t sdst = ring + stage * TR::STAGE + 2 * TR::CODES + lane * kFp4ScaleRow;
+      constexpr int STEP = 32 / TR::CPR;  // rows between a lane's chunks
+      const uint32_t good = __ballot_sync(0xffffffffu, ok);
+      if (good == 0xffffffffu && p.same_strides) {
+        // a whole tile, offsets of K and V alike: nearly always
+#pragma unroll
+        for (int x = 0; x < TR::CPR; ++x) {
+          const uint32_t o = __shfl_sync(0xffffffffu, ko, row_of_lane + x * STEP);
+          cp_async_16(dst + x * STEP * TR::ROW, k_chunk + (uint64_t)o * p.unit, policy);
+          cp_async_16(dst + TR::CODES + x * STEP * TR::ROW, v_chunk + (uint64_t)o * p.unit, policy);
+        }
+        cp_async_4(sdst, p.ks + (uint64_t)kso * 4u, 4u);
+        cp_async_4(sdst + TT * kFp4ScaleRow, p.vs + (uint64_t)kso * 4u, 4u);
+      } else {
+        bad_page |= !ok && lane < at.left;
+        const uint32_t vo = pg * p.v0 + rw * p.v1 + at.head * p.v2;
+        const uint32_t vso = pg * p.vs0 + rw * p.vs1 + at.head * p.vs2;
+#pragma unroll 1
+        for (int x = 0; x < TR::CPR; ++x) {
+          const int r = row_of_lane + x * STEP;
+          const uint32_t kr = __shfl_sync(0xffffffffu, ko, r), vr = __shfl_sync(0xffffffffu, vo, r);
+          const uint32_t bytes = ((good >> r) & 1u) << 4;
+          cp_async_16(dst + x * STEP * TR::ROW, k_chunk + (uint64_t)kr * p.unit, bytes, policy);
+          cp_async_16(dst + TR::CODES + x * STEP * TR::ROW, v_chunk + (uint64_t)vr * p.unit, bytes, policy);
+        }
+        cp_async_4(sdst, p.ks + (uint64_t)kso * 4u, ok ? 4u : 0u);
+        cp_async_4(sdst + TT * kFp4ScaleRow, p.vs + (uint64_t)vso * 4u, ok ? 4u : 0u);
+      }
     }
     cp_async_commit();
   };
-  int next_page;
+  Place next;
   {
-    Fp4Cursor c = ld;
-    int pages[S], t = ld_t;
+    Place at[S];
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      pages[s] = page_id(c, t);
-      walk.advance(c, WPH);
-      t += WPH;
-    }
-    next_page = page_id(c, t);
+    for (int s = 0; s < S; ++s) place(at[s]);
+    place(next);
 #pragma unroll
-    for (int s = 0; s < S; ++s) {
-      copy(ld, ld_t, pages[s], s);
-      walk.advance(ld, WPH);
-      ld_t += WPH;
-    }
+    for (int s = 0; s < S; ++s) copy(at[s], s);
   }
 
   // ldmatrix addresses of this lane within a tile's codes: rows 0-7 and 8-15 of
@@ -339,7 +373,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
     const int seg_end = min(t1, seg.start + seg.n);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m_run[nt][0] = m_run[nt][1] = -INFINITY;
+      m_run[nt][0] = m_run[nt][1] = kLeastScore;
       l_run[nt][0] = l_run[nt][1] = 0.f;
     }
 #pragma unroll
@@ -402,21 +436,37 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) sc[m][nt][0] = sc[m][nt][1] = sc[m][nt][2] = sc[m][nt][3] = 0.f;
+        // blocks two at a time, so that no two neighbouring products depend on
+        // each other
+        constexpr int JP = NB >= 2 ? 2 : 1;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) {
-          uint32_t a0, a1, a2, a3, b0, b1, b2, b3;
-          fp4_unpack4(r[2 * j], a0, a1, a2, a3);
-          fp4_unpack4(r[2 * j + 1], b0, b1, b2, b3);
+        for (int j0 = 0; j0 < NB; j0 += JP) {
+          uint32_t a[JP][4], b[JP][4];
+          float d[JP][NT][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_16816(d, a0, b0, a1, b1, qf[nt][j][0], qf[nt][j][1]);
-            mma_16816(d, a2, b2, a3, b3, qf[nt][j][2], qf[nt][j][3]);
-            sc[m][nt][0] += d[0] * f0[j];
-            sc[m][nt][1] += d[1] * f0[j];
-            sc[m][nt][2] += d[2] * f1[j];
-            sc[m][nt][3] += d[3] * f1[j];
+          for (int j = 0; j < JP; ++j) {
+            fp4_unpack4(r[2 * (j0 + j)], a[j][0], a[j][1], a[j][2], a[j][3]);
+            fp4_unpack4(r[2 * (j0 + j) + 1], b[j][0], b[j][1], b[j][2], b[j][3]);
           }
+#pragma unroll
+          for (int j = 0; j < JP; ++j)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_16816_zero(d[j][nt], a[j][0], b[j][0], a[j][1], b[j][1], qf[nt][j0 + j][0], qf[nt][j0 + j][1]);
+#pragma unroll
+          for (int j = 0; j < JP; ++j)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_16816(d[j][nt], a[j][2], b[j][2], a[j][3], b[j][3], qf[nt][j0 + j][2], qf[nt][j0 + j][3]);
+#pragma unroll
+          for (int j = 0; j < JP; ++j)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              sc[m][nt][0] += d[j][nt][0] * f0[j0 + j];
+              sc[m][nt][1] += d[j][nt][1] * f0[j0 + j];
+              sc[m][nt][2] += d[j][nt][2] * f1[j0 + j];
+              sc[m][nt][3] += d[j][nt][3] * f1[j0 + j];
+            }
         }
       }
       if (nv < TT) {
@@ -459,10 +509,10 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float mn = fmaxf(m_run[nt][j], mx), mu = mn == -INFINITY ? 0.f : mn;
-          grew |= mn > m_run[nt][j];
+          const float mu = fmaxf(m_run[nt][j], mx);
+          grew |= mu > m_run[nt][j];
           alpha[nt][j] = ex2(m_run[nt][j] - mu);
-          m_run[nt][j] = mn;
+          m_run[nt][j] = mu;
           float sum = 0.f;
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
@@ -536,24 +586,30 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
             const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&y), f);
             return *reinterpret_cast<const uint32_t*>(&z);
           };
+          uint32_t va[2][4];
 #pragma unroll
           for (int x = 0; x < 2; ++x) {  // dims 4 gl + 2 x and the next
-            const uint32_t a0 = scaled(e[x], lower), a1 = scaled(o[x], lower);
-            const uint32_t a2 = scaled(e[x + 2], upper), a3 = scaled(o[x + 2], upper);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_16816(acc[j][x][nt], a0, a1, a2, a3, ph[nt][0], ph[nt][1]);
-              mma_16816(acc[j][x][nt], a0, a1, a2, a3, pl[nt][0], pl[nt][1]);
-            }
+            va[x][0] = scaled(e[x], lower);
+            va[x][1] = scaled(o[x], lower);
+            va[x][2] = scaled(e[x + 2], upper);
+            va[x][3] = scaled(o[x + 2], upper);
           }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              mma_16816(acc[j][x][nt], va[x][0], va[x][1], va[x][2], va[x][3], ph[nt][0], ph[nt][1]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              mma_16816(acc[j][x][nt], va[x][0], va[x][1], va[x][2], va[x][3], pl[nt][0], pl[nt][1]);
         }
       }
       // ---- the slot is free: copy the tile S turns on into it
       __syncwarp();
-      copy(ld, ld_t, next_page, stage);
-      walk.advance(ld, WPH);
-      ld_t += WPH;
-      next_page = page_id(ld, ld_t);
+      copy(next, stage);
+      place(next);
       if (++stage == S) stage = 0;
     }
 
@@ -592,15 +648,14 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
                 make_float4(acc[blk][0][nt][j], acc[blk][0][nt][j + 2], acc[blk][1][nt][j], acc[blk][1][nt][j + 2]);
         }
       }
-    __syncthreads();
-    for (int x = tid; x < HG * G * (D / 4); x += TR::THREADS) {
-      const int row = x / (D / 4), d = (x % (D / 4)) * 4;
-      const int h = row / G, g = row - h * G;
-      const float2* ml = sml + h * WPH * TR::ROWS + g;
-      const float* src = epi + (h * WPH * TR::ROWS + g) * TR::LD + d;
-      float M = -INFINITY, L = 0.f;
-      for (int x2 = 0; x2 < WPH; ++x2) M = fmaxf(M, ml[x2 * TR::ROWS].x);
-      const float Mu = M == -INFINITY ? 0.f : M;
+    // (the warps of a head wait for one another, not for the other heads)
+    named_barrier(1 + hl, 32 * WPH);
+    for (int x = turn * 32 + lane; x < G * (D / 4); x += 32 * WPH) {
+      const int g = x / (D / 4), d = (x % (D / 4)) * 4, row = hl * G + g;
+      const float2* ml = sml + hl * WPH * TR::ROWS + g;
+      const float* src = epi + (hl * WPH * TR::ROWS + g) * TR::LD + d;
+      float Mu = kLeastScore, L = 0.f;
+      for (int x2 = 0; x2 < WPH; ++x2) Mu = fmaxf(Mu, ml[x2 * TR::ROWS].x);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int x2 = 0; x2 < WPH; ++x2) {
         const float2 y = ml[x2 * TR::ROWS];
@@ -624,9 +679,10 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
       if ((split || TR::WT) && d == 0) p.ws_ml[(int64_t)slot * HG * G + row] = make_float2(Mu, L);
     }
     if (!more) break;
-    __syncthreads();  // the buffers are read before the next segment writes them
+    named_barrier(1 + hl, 32 * WPH);  // the buffers are read before the next segment writes them
   }
   cp_async_wait_all();
+  if (bad_page && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_BAD_PAGE_ID);
 }
 
 }  // namespace pad
