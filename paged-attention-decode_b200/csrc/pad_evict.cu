@@ -39,8 +39,10 @@ namespace cg = cooperative_groups;
 using pad::cuda_fail;
 using pad::fail;
 
-constexpr int kPlanThreads = 1024;
+// 512 threads: two CTAs an SM, so that a cluster of 8 finds room.
+constexpr int kPlanThreads = 512;
 constexpr int kPlanWarps = kPlanThreads / 32;
+constexpr int kGather = 8;  // slots of a thread whose loads are in flight together
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 8;
 constexpr uint32_t kRecentKey = 0xffffffffu, kNanKey = 0xfffffffeu;
@@ -74,41 +76,65 @@ struct SlotKeys {
   const PlanParams& p;
   const uint32_t* cached;
   int64_t bt_row;
-  int b, h, first;
+  int h, first;
   int64_t oldest_recent;  // slots whose position is at least this are recent
-  __device__ __forceinline__ uint32_t load(int slot, bool report) const {
-    const int lp = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
-    const int64_t row = slot - (int64_t)lp * p.page_size;
-    const int page = __ldg(p.block_table + bt_row + lp);
-    if ((unsigned)page >= (unsigned)p.num_pages) {
-      if (report && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_BAD_PAGE_ID);
-      return 0u;
-    }
-    if (p.slot_positions != nullptr &&
-        (int64_t)__ldg(p.slot_positions + page * p.p0 + h * p.p1 + row * p.p2) >= oldest_recent)
-      return kRecentKey;
-    return weight_key(__ldg(p.weights + page * p.w0 + h * p.w1 + row * p.w2));
+  __device__ __forceinline__ int page_slot(int slot) const {
+    return p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
   }
-  // Slots past the shared-memory share are read again wherever they are needed.
+  __device__ __forceinline__ uint32_t key(float w, int at) const {
+    return p.slot_positions != nullptr && at >= oldest_recent ? kRecentKey : weight_key(w);
+  }
+  // Slots past the shared-memory share are read again wherever they are needed;
+  // those of a page that is none weigh least.
   __device__ __forceinline__ uint32_t at(int slot) const {
     const int i = slot - first;
-    return i < p.key_cap ? cached[i] : load(slot, false);
+    if (i < p.key_cap) return cached[i];
+    const int lp = page_slot(slot), page = __ldg(p.block_table + bt_row + lp);
+    const int64_t row = slot - (int64_t)lp * p.page_size;
+    if ((unsigned)page >= (unsigned)p.num_pages) return 0u;
+    const int pos = p.slot_positions != nullptr ? __ldg(p.slot_positions + page * p.p0 + h * p.p1 + row * p.p2) : 0;
+    return key(__ldg(p.weights + page * p.w0 + h * p.w1 + row * p.w2), pos);
   }
 };
 
-// Largest bin d with (keys in bins above d) < need, searched by the whole
-// block; `get(bin)` is the bin's count over the cluster. Sets sh.bin and
-// sh.above.
-template <class Get>
-__device__ void find_bin(PlanShared& sh, int need, Get get) {
+// Counts `bin` (-1: none) of every lane of a warp: lanes with the same bin add
+// once (weights tie a lot, and equal addresses would be served one by one).
+__device__ __forceinline__ void count_bin(int* hist, int bin) {
+  const uint32_t same = __match_any_sync(0xffffffffu, bin);
+  if (bin >= 0 && (int)(threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(hist + bin, __popc(same));
+}
+
+template <int RANKS>
+__device__ __forceinline__ void rank_sync() {
+  if constexpr (RANKS == 1) __syncthreads();
+  else cg::this_cluster().sync();
+}
+
+// Largest bin d with (keys in bins above d) < need, searched by every CTA of the
+// cluster for itself; a bin's count is summed over the cluster's histograms.
+// Sets sh.bin and sh.above.
+template <int RANKS>
+__device__ __forceinline__ void find_bin(PlanShared& sh, int pass, int need) {
   constexpr int PER = kBins / kPlanThreads;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int c[PER], sum = 0;
+  int c[PER] = {}, sum = 0;
+  const int top = kBins - PER * (tid + 1);  // thread t holds PER bins from the top
+  static_assert(PER == 4, "a thread's bins are one 16-byte load");
+  int4 part[RANKS];
 #pragma unroll
-  for (int i = 0; i < PER; ++i) {  // thread t holds bins from the top
-    c[i] = get(kBins - 1 - (tid * PER + i));
-    sum += c[i];
+  for (int r = 0; r < RANKS; ++r) {
+    const PlanShared* o = RANKS == 1 ? &sh : cg::this_cluster().map_shared_rank(&sh, r);
+    part[r] = *reinterpret_cast<const int4*>(&o->hist[pass][top]);
   }
+#pragma unroll
+  for (int r = 0; r < RANKS; ++r) {
+    c[0] += part[r].w;
+    c[1] += part[r].z;
+    c[2] += part[r].y;
+    c[3] += part[r].x;
+  }
+#pragma unroll
+  for (int i = 0; i < PER; ++i) sum += c[i];
   int incl = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -118,7 +144,8 @@ __device__ void find_bin(PlanShared& sh, int need, Get get) {
   if (lane == 31) sh.scan[warp] = incl;
   __syncthreads();
   int above = incl - sum;
-  for (int x = 0; x < warp; ++x) above += sh.scan[x];
+#pragma unroll
+  for (int x = 0; x < kPlanWarps; ++x) above += x < warp ? sh.scan[x] : 0;
 #pragma unroll
   for (int i = 0; i < PER; ++i) {
     if (above < need && need <= above + c[i]) {
@@ -136,7 +163,8 @@ __device__ __forceinline__ int warp_base(PlanShared& sh, int mine, int* total) {
   __syncthreads();
   if (lane == 0) sh.scan[warp] = mine;
   __syncthreads();
-  int v = sh.scan[lane], incl = v;
+  const int v = lane < kPlanWarps ? sh.scan[lane] : 0;
+  int incl = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, incl, o);
@@ -146,52 +174,76 @@ __device__ __forceinline__ int warp_base(PlanShared& sh, int mine, int* total) {
   return __shfl_sync(0xffffffffu, incl - v, warp);
 }
 
-__global__ void __launch_bounds__(kPlanThreads, 1) evict_plan_kernel(const __grid_constant__ PlanParams p) {
+template <int RANKS>
+__global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __grid_constant__ PlanParams p) {
   extern __shared__ uint32_t keys[];
-  __shared__ PlanShared sh;
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ranks = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
-  const int pair = (int)(blockIdx.x / ranks), b = pair / p.hkv, h = pair % p.hkv;
+  __shared__ __align__(16) PlanShared sh;
+  const int rank = RANKS == 1 ? 0 : (int)cg::this_cluster().block_rank();
+  const int pair = (int)(blockIdx.x / RANKS), b = pair / p.hkv, h = pair % p.hkv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int64_t cap = (int64_t)p.max_pages * p.page_size;
   const int raw = __ldg(p.seq_lens + b);
   const int n = (int)min((int64_t)max(raw, 0), cap);
-  if ((raw < 0 || raw > cap) && tid == 0 && rank == 0 && p.error_flags != nullptr)
-    atomicOr(p.error_flags, PAD_FLAG_SEQ_LEN_RANGE);
+  if (raw != n && tid == 0 && rank == 0 && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_SEQ_LEN_RANGE);
   if (h == 0 && rank == 0 && tid == 0) p.new_lens[b] = min(n, p.budget);
   int32_t* src = p.src + (int64_t)pair * p.max_moves;
   int32_t* dst = p.dst + (int64_t)pair * p.max_moves;
   int count = 0;
   if (n > p.budget) {
-    // this CTA's slots, whole warps' worth of them
-    const int share = (n + ranks - 1) / ranks;
+    const int share = (n + RANKS - 1) / RANKS;
     const int first = min(n, rank * share), last = min(n, first + share);
-    SlotKeys key{p, keys, (int64_t)b * p.bt_stride, b, h, first,
-                 p.slot_positions != nullptr ? (int64_t)__ldg(p.total_lens + b) - p.recent : 0};
-    for (int x = tid; x < 3 * kBins; x += kPlanThreads) (&sh.hist[0][0])[x] = 0;
+    const SlotKeys key{p, keys, (int64_t)b * p.bt_stride, h, first,
+                       p.slot_positions != nullptr ? (int64_t)__ldg(p.total_lens + b) - p.recent : 0};
+    for (int x = tid; x < 3 * kBins / 4; x += kPlanThreads)
+      reinterpret_cast<int4*>(&sh.hist[0][0])[x] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    for (int s = first + tid; s < last; s += kPlanThreads) {
-      const uint32_t k = key.load(s, true);
-      if (s - first < p.key_cap) keys[s - first] = k;
-      atomicAdd(&sh.hist[0][k >> 21], 1);
+    // keys into shared memory, their top digit counted on the way
+    bool bad = false;
+    for (int s0 = first; s0 < last; s0 += kPlanThreads * kGather) {
+      int page[kGather], row[kGather], at[kGather];
+      float w[kGather];
+#pragma unroll
+      for (int u = 0; u < kGather; ++u) {
+        const int s = s0 + u * kPlanThreads + tid;
+        const int lp = key.page_slot(s);
+        row[u] = s - lp * p.page_size;
+        page[u] = s < last ? __ldg(p.block_table + key.bt_row + lp) : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < kGather; ++u) {
+        const bool ok = (unsigned)page[u] < (unsigned)p.num_pages;
+        bad |= !ok && s0 + u * kPlanThreads + tid < last;
+        w[u] = 0.f;
+        at[u] = 0;
+        if (ok) {
+          w[u] = __ldg(p.weights + page[u] * p.w0 + h * p.w1 + row[u] * p.w2);
+          if (p.slot_positions != nullptr) at[u] = __ldg(p.slot_positions + page[u] * p.p0 + h * p.p1 + row[u] * p.p2);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kGather; ++u) {
+        const int s = s0 + u * kPlanThreads + tid;
+        if (s - lane >= last) break;  // (the whole warp is past the end)
+        const uint32_t k = (unsigned)page[u] < (unsigned)p.num_pages ? key.key(w[u], at[u]) : 0u;
+        if (s < last && s - first < p.key_cap) keys[s - first] = k;
+        count_bin(sh.hist[0], s < last ? (int)(k >> 21) : -1);
+      }
     }
+    if (bad && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_BAD_PAGE_ID);
     uint32_t prefix = 0;
     int need = p.budget;
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
       if (pass > 0) {
-        for (int s = first + tid; s < last; s += kPlanThreads) {
-          const uint32_t k = key.at(s);
-          if (pass == 1 ? (k >> 21) == prefix : (k >> 10) == prefix)
-            atomicAdd(&sh.hist[pass][pass == 1 ? (k >> 10) & 2047u : k & 1023u], 1);
+        for (int s = first + tid; s - lane < last; s += kPlanThreads) {
+          const uint32_t k = s < last ? key.at(s) : 0u;
+          const bool in = s < last && (pass == 1 ? (k >> 21) == prefix : (k >> 10) == prefix);
+          if (__any_sync(0xffffffffu, in))
+            count_bin(sh.hist[pass], in ? (int)(pass == 1 ? (k >> 10) & 2047u : k & 1023u) : -1);
         }
       }
-      cluster.sync();
-      find_bin(sh, need, [&](int bin) {
-        int c = 0;
-        for (int r = 0; r < ranks; ++r) c += cluster.map_shared_rank(&sh, r)->hist[pass][bin];
-        return c;
-      });
+      rank_sync<RANKS>();
+      find_bin<RANKS>(sh, pass, need);
       need -= sh.above;
       prefix = pass == 0 ? (uint32_t)sh.bin : (prefix << (pass == 1 ? 11 : 10)) | (uint32_t)sh.bin;
     }
@@ -203,7 +255,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) evict_plan_kernel(const __gri
     int eq = 0, total;
     for (int s = lo + lane; s - lane < hi; s += 32) eq += __popc(__ballot_sync(0xffffffffu, s < hi && key.at(s) == T));
     int eq_base = warp_base(sh, eq, &total);
-    for (int r = 0; r < rank; ++r) eq_base += cluster.map_shared_rank(&sh, r)->hist[2][T & 1023u];
+    if constexpr (RANKS > 1)
+      for (int r = 0; r < rank; ++r) eq_base += cg::this_cluster().map_shared_rank(&sh, r)->hist[2][T & 1023u];
     const uint32_t below = (1u << lane) - 1u;
     // which of 32 slots are kept, and the running number of equals before them
     auto kept = [&](int s, int& seen) {
@@ -223,14 +276,16 @@ __global__ void __launch_bounds__(kPlanThreads, 1) evict_plan_kernel(const __gri
     if (tid == 0) sh.holes = total;
     int mover_at = warp_base(sh, movers, &total);
     if (tid == 0) sh.movers = total;
-    cluster.sync();
-    for (int r = 0; r < ranks; ++r) {
-      const PlanShared* o = cluster.map_shared_rank(&sh, r);
+    rank_sync<RANKS>();
+#pragma unroll
+    for (int r = 0; r < RANKS; ++r) {
+      const PlanShared* o = RANKS == 1 ? &sh : cg::this_cluster().map_shared_rank(&sh, r);
+      const int oh = o->holes, om = o->movers;
       if (r < rank) {
-        hole_at += o->holes;
-        mover_at += o->movers;
+        hole_at += oh;
+        mover_at += om;
       }
-      count += o->movers;
+      count += om;
     }
     seen = eq_base;
     for (int s = lo + lane; s - lane < hi; s += 32) {
@@ -244,10 +299,10 @@ __global__ void __launch_bounds__(kPlanThreads, 1) evict_plan_kernel(const __gri
       mover_at += __popc(m);
       hole_at += __popc(o);
     }
-    cluster.sync();  // no CTA leaves while another may read its shared memory
+    if constexpr (RANKS > 1) cg::this_cluster().sync();  // no CTA leaves while another may read its shared memory
   }
   if (tid == 0 && rank == 0) p.counts[pair] = count;
-  for (int x = count + rank * kPlanThreads + tid; x < p.max_moves; x += ranks * kPlanThreads) {
+  for (int x = count + rank * kPlanThreads + tid; x < p.max_moves; x += RANKS * kPlanThreads) {
     src[x] = -1;
     dst[x] = -1;
   }
@@ -419,8 +474,14 @@ extern "C" int pad_paged_kv_evict_plan(const float* weights, const int32_t* slot
   p.max_moves = (int)moves;
   p.error_flags = error_flags;
   // a CTA per 8192 slots of a sequence, up to a cluster of 8
-  int ranks = 1;
-  while (ranks < kMaxCluster && cap > (int64_t)ranks * 8192) ranks *= 2;
+  int ranks = 1, lg = 0;
+  while (ranks < kMaxCluster && cap > (int64_t)ranks * 8192) {
+    ranks *= 2;
+    ++lg;
+  }
+  static const void* const kernels[4] = {
+      reinterpret_cast<const void*>(&evict_plan_kernel<1>), reinterpret_cast<const void*>(&evict_plan_kernel<2>),
+      reinterpret_cast<const void*>(&evict_plan_kernel<4>), reinterpret_cast<const void*>(&evict_plan_kernel<8>)};
   const int64_t share = (cap + ranks - 1) / ranks;
   p.key_cap = (int)std::min<int64_t>(kKeyCapMax, (share + 255) / 256 * 256);
   int device = 0;
@@ -429,8 +490,10 @@ extern "C" int pad_paged_kv_evict_plan(const float* weights, const int32_t* slot
   if (device < 0 || device >= kMaxDevices) return fail(PAD_ERR_INVALID_ARGUMENT, "device %d out of range", device);
   static std::atomic<bool> smem_set[kMaxDevices];  // set twice by racing threads at worst
   if (!smem_set[device].load()) {
-    e = cudaFuncSetAttribute(evict_plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeyCapMax * 4);
-    if (e != cudaSuccess) return cuda_fail(e, "configuring the evict_plan kernel");
+    for (const void* k : kernels) {
+      e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeyCapMax * 4);
+      if (e != cudaSuccess) return cuda_fail(e, "configuring the evict_plan kernel");
+    }
     smem_set[device].store(true);
   }
   cudaLaunchConfig_t cfg = {};
@@ -446,7 +509,7 @@ extern "C" int pad_paged_kv_evict_plan(const float* weights, const int32_t* slot
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   void* args[] = {&p};
-  e = cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(&evict_plan_kernel), args);
+  e = cudaLaunchKernelExC(&cfg, kernels[lg], args);
   return e == cudaSuccess ? PAD_OK : cuda_fail(e, "launching the evict_plan kernel");
 }
 
