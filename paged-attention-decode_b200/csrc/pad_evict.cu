@@ -68,10 +68,12 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 struct PlanShared {
   int hist[3][kBins];
   int scan[kPlanWarps];
-  int bin, above;         // the digit found in a pass, and the keys above it
+  int bin, above, in_bin;  // the digit found in a pass, the keys above it and in it
   int eq, movers, holes;  // this CTA's counts, read by the cluster
 };
 
+// CACHED: every key lies in shared memory.
+template <bool CACHED>
 struct SlotKeys {
   const PlanParams& p;
   const uint32_t* cached;
@@ -88,7 +90,7 @@ struct SlotKeys {
   // those of a page that is none weigh least.
   __device__ __forceinline__ uint32_t at(int slot) const {
     const int i = slot - first;
-    if (i < p.key_cap) return cached[i];
+    if (CACHED || i < p.key_cap) return cached[i];
     const int lp = page_slot(slot), page = __ldg(p.block_table + bt_row + lp);
     const int64_t row = slot - (int64_t)lp * p.page_size;
     if ((unsigned)page >= (unsigned)p.num_pages) return 0u;
@@ -96,13 +98,6 @@ struct SlotKeys {
     return key(__ldg(p.weights + page * p.w0 + h * p.w1 + row * p.w2), pos);
   }
 };
-
-// Counts `bin` (-1: none) of every lane of a warp: lanes with the same bin add
-// once (weights tie a lot, and equal addresses would be served one by one).
-__device__ __forceinline__ void count_bin(int* hist, int bin) {
-  const uint32_t same = __match_any_sync(0xffffffffu, bin);
-  if (bin >= 0 && (int)(threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(hist + bin, __popc(same));
-}
 
 template <int RANKS>
 __device__ __forceinline__ void rank_sync() {
@@ -151,6 +146,7 @@ __device__ __forceinline__ void find_bin(PlanShared& sh, int pass, int need) {
     if (above < need && need <= above + c[i]) {
       sh.bin = kBins - 1 - (tid * PER + i);
       sh.above = above;
+      sh.in_bin = c[i];
     }
     above += c[i];
   }
@@ -174,7 +170,7 @@ __device__ __forceinline__ int warp_base(PlanShared& sh, int mine, int* total) {
   return __shfl_sync(0xffffffffu, incl - v, warp);
 }
 
-template <int RANKS>
+template <int RANKS, bool CACHED>
 __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __grid_constant__ PlanParams p) {
   extern __shared__ uint32_t keys[];
   __shared__ __align__(16) PlanShared sh;
@@ -192,7 +188,7 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
   if (n > p.budget) {
     const int share = (n + RANKS - 1) / RANKS;
     const int first = min(n, rank * share), last = min(n, first + share);
-    const SlotKeys key{p, keys, (int64_t)b * p.bt_stride, h, first,
+    const SlotKeys<CACHED> key{p, keys, (int64_t)b * p.bt_stride, h, first,
                        p.slot_positions != nullptr ? (int64_t)__ldg(p.total_lens + b) - p.recent : 0};
     for (int x = tid; x < 3 * kBins / 4; x += kPlanThreads)
       reinterpret_cast<int4*>(&sh.hist[0][0])[x] = make_int4(0, 0, 0, 0);
@@ -223,10 +219,11 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
 #pragma unroll
       for (int u = 0; u < kGather; ++u) {
         const int s = s0 + u * kPlanThreads + tid;
-        if (s - lane >= last) break;  // (the whole warp is past the end)
         const uint32_t k = (unsigned)page[u] < (unsigned)p.num_pages ? key.key(w[u], at[u]) : 0u;
-        if (s < last && s - first < p.key_cap) keys[s - first] = k;
-        count_bin(sh.hist[0], s < last ? (int)(k >> 21) : -1);
+        if (s < last) {
+          if (CACHED || s - first < p.key_cap) keys[s - first] = k;
+          atomicAdd(&sh.hist[0][k >> 21], 1);
+        }
       }
     }
     if (bad && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_BAD_PAGE_ID);
@@ -235,11 +232,11 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
       if (pass > 0) {
-        for (int s = first + tid; s - lane < last; s += kPlanThreads) {
-          const uint32_t k = s < last ? key.at(s) : 0u;
-          const bool in = s < last && (pass == 1 ? (k >> 21) == prefix : (k >> 10) == prefix);
-          if (__any_sync(0xffffffffu, in))
-            count_bin(sh.hist[pass], in ? (int)(pass == 1 ? (k >> 10) & 2047u : k & 1023u) : -1);
+#pragma unroll 4
+        for (int s = first + tid; s < last; s += kPlanThreads) {
+          const uint32_t k = key.at(s);
+          if (pass == 1 ? (k >> 21) == prefix : (k >> 10) == prefix)
+            atomicAdd(&sh.hist[pass][pass == 1 ? (k >> 10) & 2047u : k & 1023u], 1);
         }
       }
       rank_sync<RANKS>();
@@ -252,21 +249,28 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
     // each warp walks a contiguous run of the CTA's slots
     const int per = ((last - first + kPlanWarps - 1) / kPlanWarps + 31) / 32 * 32;
     const int lo = min(last, first + warp * per), hi = min(last, lo + per);
-    int eq = 0, total;
-    for (int s = lo + lane; s - lane < hi; s += 32) eq += __popc(__ballot_sync(0xffffffffu, s < hi && key.at(s) == T));
-    int eq_base = warp_base(sh, eq, &total);
-    if constexpr (RANKS > 1)
-      for (int r = 0; r < rank; ++r) eq_base += cg::this_cluster().map_shared_rank(&sh, r)->hist[2][T & 1023u];
     const uint32_t below = (1u << lane) - 1u;
+    int eq_base = 0, total;
+    const bool all_eq = sh.in_bin == need;  // every slot equal to T is kept: their order does not matter
+    if (!all_eq) {
+      int eq = 0;
+#pragma unroll 4
+      for (int s = lo + lane; s - lane < hi; s += 32) eq += __popc(__ballot_sync(0xffffffffu, s < hi && key.at(s) == T));
+      eq_base = warp_base(sh, eq, &total);
+      if constexpr (RANKS > 1)
+        for (int r = 0; r < rank; ++r) eq_base += cg::this_cluster().map_shared_rank(&sh, r)->hist[2][T & 1023u];
+    }
     // which of 32 slots are kept, and the running number of equals before them
     auto kept = [&](int s, int& seen) {
       const uint32_t k = s < hi ? key.at(s) : 0u;
+      if (all_eq) return s < hi && k >= T;
       const uint32_t e = __ballot_sync(0xffffffffu, s < hi && k == T);
       const bool on = s < hi && (k > T || (k == T && seen + __popc(e & below) < need));
       seen += __popc(e);
       return on;
     };
     int holes = 0, movers = 0, seen = eq_base;
+#pragma unroll 4
     for (int s = lo + lane; s - lane < hi; s += 32) {
       const bool on = kept(s, seen);
       movers += __popc(__ballot_sync(0xffffffffu, on && s >= p.budget));
@@ -288,6 +292,7 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
       count += om;
     }
     seen = eq_base;
+#pragma unroll 4
     for (int s = lo + lane; s - lane < hi; s += 32) {
       const bool on = kept(s, seen);
       const uint32_t m = __ballot_sync(0xffffffffu, on && s >= p.budget);
@@ -307,7 +312,6 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
     dst[x] = -1;
   }
 }
-
 // ----------------------------------------------------------------------------- move
 constexpr int kMoveThreads = 256;
 constexpr int kMaxCaches = 4;
@@ -479,11 +483,13 @@ extern "C" int pad_paged_kv_evict_plan(const float* weights, const int32_t* slot
     ranks *= 2;
     ++lg;
   }
-  static const void* const kernels[4] = {
-      reinterpret_cast<const void*>(&evict_plan_kernel<1>), reinterpret_cast<const void*>(&evict_plan_kernel<2>),
-      reinterpret_cast<const void*>(&evict_plan_kernel<4>), reinterpret_cast<const void*>(&evict_plan_kernel<8>)};
+  static const void* const kernels[5] = {
+      reinterpret_cast<const void*>(&evict_plan_kernel<1, true>), reinterpret_cast<const void*>(&evict_plan_kernel<2, true>),
+      reinterpret_cast<const void*>(&evict_plan_kernel<4, true>), reinterpret_cast<const void*>(&evict_plan_kernel<8, true>),
+      reinterpret_cast<const void*>(&evict_plan_kernel<8, false>)};
   const int64_t share = (cap + ranks - 1) / ranks;
   p.key_cap = (int)std::min<int64_t>(kKeyCapMax, (share + 255) / 256 * 256);
+  if (share > p.key_cap) lg = 4;  // (then ranks is 8)
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
