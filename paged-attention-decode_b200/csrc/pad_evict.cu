@@ -325,7 +325,7 @@ struct MoveParams {
   int32_t* slot_positions;
   const int32_t *block_table, *src, *dst, *counts;
   int64_t w0, w1, w2, p0, p1, p2, bt_stride;
-  int64_t items;  // (pair, run of moves) pieces of work
+  int64_t items;  // (pair, run of 32 moves) pieces of work
   int hkv, num_pages, page_size, page_shift, max_pages, max_moves, runs;
   int32_t* error_flags;
 };
@@ -345,51 +345,87 @@ __device__ __forceinline__ void store_piece(uint8_t* x, const uint4& v, int unit
   else *x = (uint8_t)v.x;
 }
 
-// LPM lanes copy one row of every cache (and its weight and position); all
-// loads of a move are issued before its stores.
-template <int LPM>
+// A warp takes up to 32 moves of one pair. Lane i looks up move i (slots, pages;
+// its weight and position it copies itself), so that the chain of dependent loads
+// is walked once for 32 moves; then LPM lanes copy each row, the addresses coming
+// from move i's lane by shuffles, UN rounds of loads before their stores.
+template <int LPM, int NC>
 __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_constant__ MoveParams p) {
-  constexpr int MPB = kMoveThreads / LPM;
-  const int m = threadIdx.x / LPM, l = threadIdx.x % LPM;
-  for (int64_t it = blockIdx.x; it < p.items; it += gridDim.x) {
-    const int pair = (int)(it / p.runs);
-    const int i = (int)(it - (int64_t)pair * p.runs) * MPB + m;
-    if (i >= min(__ldg(p.counts + pair), p.max_moves)) continue;
+  constexpr int MPR = 32 / LPM;           // moves of a round
+  constexpr int UN = NC <= 2 ? 4 : 2;     // rounds in flight
+  constexpr int ROUNDS = LPM;             // 32 / MPR
+  static_assert(ROUNDS % UN == 0, "whole rounds");
+  const int lane = threadIdx.x & 31, l = lane % LPM, mine = lane / LPM;
+  const int64_t cap = (int64_t)p.max_pages * p.page_size;
+  for (int64_t it = (int64_t)blockIdx.x * (kMoveThreads / 32) + (threadIdx.x >> 5); it < p.items;
+       it += (int64_t)gridDim.x * (kMoveThreads / 32)) {
+    const int pair = (int)(it / p.runs), i0 = (int)(it - (int64_t)pair * p.runs) * 32;
+    const int left = min(__ldg(p.counts + pair), p.max_moves) - i0;
+    if (left <= 0) continue;
     const int b = pair / p.hkv, h = pair % p.hkv;
-    const int ss = __ldg(p.src + (int64_t)pair * p.max_moves + i), ds = __ldg(p.dst + (int64_t)pair * p.max_moves + i);
-    const int64_t cap = (int64_t)p.max_pages * p.page_size;
-    if (ss < 0 || ds < 0 || ss >= cap || ds >= cap) {
-      if (l == 0 && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_SEQ_LEN_RANGE);
-      continue;
+    // ---- this lane's move
+    int sp = 0, dp = 0, sr = 0, dr = 0, bad = 0;
+    bool ok = lane < left;
+    if (ok) {
+      const int64_t at = (int64_t)pair * p.max_moves + i0 + lane;
+      const int ss = __ldg(p.src + at), ds = __ldg(p.dst + at);
+      if (ss < 0 || ds < 0 || ss >= cap || ds >= cap) {
+        bad = PAD_FLAG_SEQ_LEN_RANGE;
+      } else {
+        const int slp = p.page_shift >= 0 ? ss >> p.page_shift : ss / p.page_size;
+        const int dlp = p.page_shift >= 0 ? ds >> p.page_shift : ds / p.page_size;
+        sp = __ldg(p.block_table + b * p.bt_stride + slp);
+        dp = __ldg(p.block_table + b * p.bt_stride + dlp);
+        sr = ss - slp * p.page_size;
+        dr = ds - dlp * p.page_size;
+        if ((unsigned)sp >= (unsigned)p.num_pages || (unsigned)dp >= (unsigned)p.num_pages) bad = PAD_FLAG_BAD_PAGE_ID;
+      }
+      ok = bad == 0;
+      if (bad != 0 && p.error_flags != nullptr) atomicOr(p.error_flags, bad);
     }
-    const int slp = p.page_shift >= 0 ? ss >> p.page_shift : ss / p.page_size;
-    const int dlp = p.page_shift >= 0 ? ds >> p.page_shift : ds / p.page_size;
-    const int64_t sp = __ldg(p.block_table + b * p.bt_stride + slp), dp = __ldg(p.block_table + b * p.bt_stride + dlp);
-    if (sp < 0 || dp < 0 || sp >= p.num_pages || dp >= p.num_pages) {
-      if (l == 0 && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_BAD_PAGE_ID);
-      continue;
-    }
-    const int64_t sr = ss - (int64_t)slp * p.page_size, dr = ds - (int64_t)dlp * p.page_size;
-    uint4 v[kMaxCaches];
     float w = 0.f;
-    int32_t at = 0;
+    int32_t pos = 0;
+    if (ok && p.weights != nullptr) w = p.weights[sp * p.w0 + h * p.w1 + sr * p.w2];
+    if (ok && p.slot_positions != nullptr) pos = p.slot_positions[sp * p.p0 + h * p.p1 + sr * p.p2];
+    const uint32_t good = __ballot_sync(0xffffffffu, ok);
+    // ---- the rows
+#pragma unroll 1
+    for (int r0 = 0; r0 < ROUNDS && r0 * MPR < left; r0 += UN) {
+      uint4 v[UN][NC];
+      int64_t to[UN][2];  // page and row of the target
 #pragma unroll
-    for (int c = 0; c < kMaxCaches; ++c)
-      if (l < p.chunks[c])
-        v[c] = load_piece(p.cache[c] + sp * p.s0[c] + sr * p.s1[c] + h * p.s2[c] + ((int64_t)l << p.unit_log2[c]),
-                          p.unit_log2[c]);
-    if (l == 0 && p.weights != nullptr) w = p.weights[sp * p.w0 + h * p.w1 + sr * p.w2];
-    if (l == LPM - 1 && p.slot_positions != nullptr) at = p.slot_positions[sp * p.p0 + h * p.p1 + sr * p.p2];
+      for (int u = 0; u < UN; ++u) {
+        const int m = (r0 + u) * MPR + mine;
+        const int64_t fp = __shfl_sync(0xffffffffu, sp, m), fr = __shfl_sync(0xffffffffu, sr, m);
+        to[u][0] = __shfl_sync(0xffffffffu, dp, m);
+        to[u][1] = __shfl_sync(0xffffffffu, dr, m);
+        if (!((good >> m) & 1u)) to[u][0] = -1;
 #pragma unroll
-    for (int c = 0; c < kMaxCaches; ++c) {
-      const int64_t from = sp * p.s0[c] + sr * p.s1[c] + h * p.s2[c], to = dp * p.s0[c] + dr * p.s1[c] + h * p.s2[c];
-      if (l < p.chunks[c]) store_piece(p.cache[c] + to + ((int64_t)l << p.unit_log2[c]), v[c], p.unit_log2[c]);
-      for (int x = l + LPM; x < p.chunks[c]; x += LPM)
-        store_piece(p.cache[c] + to + ((int64_t)x << p.unit_log2[c]),
-                    load_piece(p.cache[c] + from + ((int64_t)x << p.unit_log2[c]), p.unit_log2[c]), p.unit_log2[c]);
+        for (int c = 0; c < NC; ++c)
+          if (to[u][0] >= 0 && l < p.chunks[c])
+            v[u][c] = load_piece(p.cache[c] + fp * p.s0[c] + fr * p.s1[c] + h * p.s2[c] + ((int64_t)l << p.unit_log2[c]),
+                                 p.unit_log2[c]);
+      }
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const int m = (r0 + u) * MPR + mine;
+        const int64_t fp = __shfl_sync(0xffffffffu, sp, m), fr = __shfl_sync(0xffffffffu, sr, m);
+        if (to[u][0] < 0) continue;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          uint8_t* row = p.cache[c] + to[u][0] * p.s0[c] + to[u][1] * p.s1[c] + h * p.s2[c];
+          if (l < p.chunks[c]) store_piece(row + ((int64_t)l << p.unit_log2[c]), v[u][c], p.unit_log2[c]);
+          // rows of more than LPM pieces
+          for (int x = l + LPM; x < p.chunks[c]; x += LPM)
+            store_piece(row + ((int64_t)x << p.unit_log2[c]),
+                        load_piece(p.cache[c] + fp * p.s0[c] + fr * p.s1[c] + h * p.s2[c] + ((int64_t)x << p.unit_log2[c]),
+                                   p.unit_log2[c]),
+                        p.unit_log2[c]);
+        }
+      }
     }
-    if (l == 0 && p.weights != nullptr) p.weights[dp * p.w0 + h * p.w1 + dr * p.w2] = w;
-    if (l == LPM - 1 && p.slot_positions != nullptr) p.slot_positions[dp * p.p0 + h * p.p1 + dr * p.p2] = at;
+    if (ok && p.weights != nullptr) p.weights[dp * p.w0 + h * p.w1 + dr * p.w2] = w;
+    if (ok && p.slot_positions != nullptr) p.slot_positions[dp * p.p0 + h * p.p1 + dr * p.p2] = pos;
   }
 }
 
@@ -579,17 +615,20 @@ extern "C" int pad_paged_kv_move(int64_t num_caches, void* const* caches, const 
   p.max_pages = (int)max_pages_per_seq;
   p.max_moves = (int)max_moves;
   p.error_flags = error_flags;
-  // lanes per move: enough for the widest row's pieces, 16 at most (a 256-byte
-  // row's 16 pieces; longer rows loop)
-  const int lpm = most <= 4 ? 4 : most <= 8 ? 8 : 16;
-  const int mpb = kMoveThreads / lpm;
-  p.runs = (int)((max_moves + mpb - 1) / mpb);
+  p.runs = (int)((max_moves + 31) / 32);
   p.items = batch * num_kv_heads * (int64_t)p.runs;
-  const unsigned grid = (unsigned)std::min<int64_t>(p.items, kMoveGrid);
+  const unsigned grid = (unsigned)std::min<int64_t>((p.items + kMoveThreads / 32 - 1) / (kMoveThreads / 32), kMoveGrid);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (lpm == 4) kv_move_kernel<4><<<grid, kMoveThreads, 0, s>>>(p);
-  else if (lpm == 8) kv_move_kernel<8><<<grid, kMoveThreads, 0, s>>>(p);
-  else kv_move_kernel<16><<<grid, kMoveThreads, 0, s>>>(p);
+  // lanes per move: enough for the widest row's pieces, 16 at most (a 256-byte
+  // row's 16 pieces; longer rows loop); two caches keep more rounds in flight
+  const int lpm = most <= 4 ? 4 : 16;
+  if (num_caches <= 2) {
+    if (lpm == 4) kv_move_kernel<4, 2><<<grid, kMoveThreads, 0, s>>>(p);
+    else kv_move_kernel<16, 2><<<grid, kMoveThreads, 0, s>>>(p);
+  } else {
+    if (lpm == 4) kv_move_kernel<4, 4><<<grid, kMoveThreads, 0, s>>>(p);
+    else kv_move_kernel<16, 4><<<grid, kMoveThreads, 0, s>>>(p);
+  }
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? PAD_OK : cuda_fail(e, "launching the kv_move kernel");
 }
