@@ -88,39 +88,39 @@ __device__ __forceinline__ uint4 load_row8(const __half* x, int vec) {
 // threads beside it hold; every thread of the block gets the scale byte.
 __device__ __forceinline__ uint32_t quantise8(const uint4& r, uint32_t& scale) {
   const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-  // maximum of |x| as integers, so that NaN and Inf come out above all others
-  uint32_t a = 0;
+  __half2 m[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    a = max(a, w[i] & 0x7fffu);
-    a = max(a, (w[i] >> 16) & 0x7fffu);
-  }
-  a = max(a, __shfl_xor_sync(0xffffffffu, a, 1));
-  a = max(a, __shfl_xor_sync(0xffffffffu, a, 2));
-  const float top = __half2float(__ushort_as_half((unsigned short)a));
+  for (int i = 0; i < 4; ++i) m[i] = __habs2(*reinterpret_cast<const __half2*>(&w[i]));
+  // maxima that keep a NaN
+  __half2 a2 = __hmax2_nan(__hmax2_nan(m[0], m[1]), __hmax2_nan(m[2], m[3]));
+  a2 = __hmax2_nan(a2, __shfl_xor_sync(0xffffffffu, a2, 1));
+  a2 = __hmax2_nan(a2, __shfl_xor_sync(0xffffffffu, a2, 2));
+  const float top = __half2float(__hmax_nan(__low2half(a2), __high2half(a2)));
+  const bool fine = top <= 65504.f;  // neither Inf nor NaN
   const int e = max((int)(__float_as_uint(top) >> 23) - 127 - 2, kFp4MinExp);
-  const bool fine = a < 0x7c00u;
   scale = fine ? (uint32_t)(e + 127) : kFp4NanScale;
-  const float inv = fine ? __uint_as_float((uint32_t)(127 - e) << 23) : 0.f;
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
   float x[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 h = *reinterpret_cast<const __half2*>(&w[i]);
-    x[2 * i] = __low2float(h) * inv;
-    x[2 * i + 1] = __high2float(h) * inv;
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    x[2 * i] = f.x * inv;
+    x[2 * i + 1] = f.y * inv;
   }
   return fine ? fp4_pack8(x) : 0u;
 }
 
-// The scale row's word from the scale bytes of its blocks (held by every
-// thread of a block); lanes past the row's D/8 contribute nothing.
+// A row's scale bytes, by the first thread of each block; the row's unused
+// bytes become 0.
 template <int D>
-__device__ __forceinline__ uint32_t scale_word(uint32_t scale, uint32_t lane) {
-  const uint32_t first = lane & ~(D / 8 - 1);
-  uint32_t w = 0;
-#pragma unroll
-  for (int j = 0; j < D / kFp4Block; ++j) w |= __shfl_sync(0xffffffffu, scale, first + 4 * j) << (8 * j);
-  return w;
+__device__ __forceinline__ void store_scale(uint8_t* row, int c, uint32_t scale) {
+  if (c % 4 != 0) return;
+  if constexpr (D == 32) {
+    *reinterpret_cast<uint32_t*>(row) = scale;
+  } else {
+    row[c / 4] = (uint8_t)scale;
+    if constexpr (D == 64) row[c / 4 + 2] = 0;
+  }
 }
 
 template <int D, int HU>
@@ -128,50 +128,69 @@ __global__ void __launch_bounds__(kThreadsFp4) fp4_append_kernel(const __grid_co
   constexpr int LPR = D / 8;  // threads per row
   const uint32_t r = blockIdx.x * (kThreadsFp4 / LPR) + threadIdx.x / LPR;  // (token, run of HU heads)
   const int c = (int)(threadIdx.x % LPR);
-  const uint32_t lane = threadIdx.x & 31, groups = p.hkv / HU;
+  const uint32_t groups = p.hkv / HU;
   const bool on = r < p.rows;
   const int64_t t = on ? r / groups : 0;
   const int h0 = on ? (int)(r % groups) * HU : 0;
+  const __half* kn = p.k_in + t * p.kr_t + h0 * p.kr_h + c * 8;
+  const __half* vn = p.v_in + t * p.vr_t + h0 * p.vr_h + c * 8;
   uint4 kx[HU], vx[HU];
 #pragma unroll
   for (int u = 0; u < HU; ++u) {
     kx[u] = vx[u] = make_uint4(0, 0, 0, 0);
     if (on) {
-      kx[u] = load_row8(p.k_in + t * p.kr_t + (h0 + u) * p.kr_h + c * 8, p.vec);
-      vx[u] = load_row8(p.v_in + t * p.vr_t + (h0 + u) * p.vr_h + c * 8, p.vec);
+      kx[u] = load_row8(kn, p.vec);
+      vx[u] = load_row8(vn, p.vec);
     }
+    kn += p.kr_h;
+    vn += p.vr_h;
   }
   int64_t page = 0, row = 0;
   const bool ok = on && locate(p, t, page, row, c == 0);
+  uint8_t* ko = p.k + page * p.k_st.s0 + row * p.k_st.s1 + h0 * p.k_st.s2 + c * 4;
+  uint8_t* vo = p.v + page * p.v_st.s0 + row * p.v_st.s1 + h0 * p.v_st.s2 + c * 4;
+  uint8_t* kso = p.ks + page * p.ks_st.s0 + row * p.ks_st.s1 + h0 * p.ks_st.s2;
+  uint8_t* vso = p.vs + page * p.vs_st.s0 + row * p.vs_st.s1 + h0 * p.vs_st.s2;
 #pragma unroll
   for (int u = 0; u < HU; ++u) {
-    const int h = h0 + u;
     uint32_t ksc, vsc;
     const uint32_t kc = quantise8(kx[u], ksc), vc = quantise8(vx[u], vsc);
-    const uint32_t kw = scale_word<D>(ksc, lane), vw = scale_word<D>(vsc, lane);
-    if (!ok) continue;
-    *reinterpret_cast<uint32_t*>(p.k + page * p.k_st.s0 + row * p.k_st.s1 + h * p.k_st.s2 + c * 4) = kc;
-    *reinterpret_cast<uint32_t*>(p.v + page * p.v_st.s0 + row * p.v_st.s1 + h * p.v_st.s2 + c * 4) = vc;
-    if (c == 0) {
-      *reinterpret_cast<uint32_t*>(p.ks + page * p.ks_st.s0 + row * p.ks_st.s1 + h * p.ks_st.s2) = kw;
-      *reinterpret_cast<uint32_t*>(p.vs + page * p.vs_st.s0 + row * p.vs_st.s1 + h * p.vs_st.s2) = vw;
+    if (ok) {
+      *reinterpret_cast<uint32_t*>(ko) = kc;
+      *reinterpret_cast<uint32_t*>(vo) = vc;
+      store_scale<D>(kso, c, ksc);
+      store_scale<D>(vso, c, vsc);
     }
+    ko += p.k_st.s2;
+    vo += p.v_st.s2;
+    kso += p.ks_st.s2;
+    vso += p.vs_st.s2;
   }
 }
 
 // Four code bytes and their scale -> 8 fp16 values, rounded once (exact for
-// every row that fp4_append_kernel wrote).
+// every row that fp4_append_kernel wrote). A scale that fp16 holds, which is all
+// the append writes, multiplies as fp16; any other goes through fp32.
 __device__ __forceinline__ uint4 dequantise8(uint32_t codes, uint32_t scale) {
   uint32_t h[4];
   fp4_unpack4(codes, h[0], h[1], h[2], h[3]);
   const float f = fp4_scale_f32(scale);
   uint4 r;
   uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+  if (scale - 103u <= 39u) {  // 2^-24 .. 2^15
+    const __half2 f2 = __float2half2_rn(f);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-    const __half2 o = __floats2half2_rn(v.x * f, v.y * f);
-    w[i] = *reinterpret_cast<const uint32_t*>(&o);
+    for (int i = 0; i < 4; ++i) {
+      const __half2 o = __hmul2(*reinterpret_cast<const __half2*>(&h[i]), f2);
+      w[i] = *reinterpret_cast<const uint32_t*>(&o);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+      const __half2 o = __floats2half2_rn(v.x * f, v.y * f);
+      w[i] = *reinterpret_cast<const uint32_t*>(&o);
+    }
   }
   return r;
 }
@@ -201,21 +220,33 @@ __global__ void __launch_bounds__(kThreadsFp4) fp4_read_kernel(const __grid_cons
   int64_t page = 0, row = 0;
   uint32_t kc[HU], vc[HU], ks[HU], vs[HU];
   const bool ok = locate(p, t, page, row, c == 0);
+  const uint8_t* ki = p.k + page * p.k_st.s0 + row * p.k_st.s1 + h0 * p.k_st.s2 + c * 4;
+  const uint8_t* vi = p.v + page * p.v_st.s0 + row * p.v_st.s1 + h0 * p.v_st.s2 + c * 4;
+  const uint8_t* ksi = p.ks + page * p.ks_st.s0 + row * p.ks_st.s1 + h0 * p.ks_st.s2 + c / 4;
+  const uint8_t* vsi = p.vs + page * p.vs_st.s0 + row * p.vs_st.s1 + h0 * p.vs_st.s2 + c / 4;
 #pragma unroll
   for (int u = 0; u < HU; ++u) {
-    const int h = h0 + u;
-    kc[u] = vc[u] = ks[u] = vs[u] = 0;  // a token without a place reads as zero
+    kc[u] = vc[u] = 0;  // a token without a place reads as zero
+    ks[u] = vs[u] = 127;
     if (ok) {
-      kc[u] = *reinterpret_cast<const uint32_t*>(p.k + page * p.k_st.s0 + row * p.k_st.s1 + h * p.k_st.s2 + c * 4);
-      vc[u] = *reinterpret_cast<const uint32_t*>(p.v + page * p.v_st.s0 + row * p.v_st.s1 + h * p.v_st.s2 + c * 4);
-      ks[u] = p.ks[page * p.ks_st.s0 + row * p.ks_st.s1 + h * p.ks_st.s2 + c / 4];
-      vs[u] = p.vs[page * p.vs_st.s0 + row * p.vs_st.s1 + h * p.vs_st.s2 + c / 4];
+      kc[u] = *reinterpret_cast<const uint32_t*>(ki);
+      vc[u] = *reinterpret_cast<const uint32_t*>(vi);
+      ks[u] = *ksi;
+      vs[u] = *vsi;
     }
+    ki += p.k_st.s2;
+    vi += p.v_st.s2;
+    ksi += p.ks_st.s2;
+    vsi += p.vs_st.s2;
   }
+  __half* kr = p.k_out + t * p.kr_t + h0 * p.kr_h + c * 8;
+  __half* vr = p.v_out + t * p.vr_t + h0 * p.vr_h + c * 8;
 #pragma unroll
   for (int u = 0; u < HU; ++u) {
-    store_row8(p.k_out + t * p.kr_t + (h0 + u) * p.kr_h + c * 8, dequantise8(kc[u], ks[u]), p.vec);
-    store_row8(p.v_out + t * p.vr_t + (h0 + u) * p.vr_h + c * 8, dequantise8(vc[u], vs[u]), p.vec);
+    store_row8(kr, dequantise8(kc[u], ks[u]), p.vec);
+    store_row8(vr, dequantise8(vc[u], vs[u]), p.vec);
+    kr += p.kr_h;
+    vr += p.vr_h;
   }
 }
 
