@@ -137,7 +137,7 @@ struct Plan {
   size_t off_meta = 0, off_ml = 0, off_o = 0, bytes = 0;
   // the decode with attention weights
   int64_t raw_tiles = 0;
-  size_t off_raw = 0, off_tiles = 0, off_pairs = 0, off_total = 0;
+  size_t off_raw = 0, off_tiles = 0, off_norm = 0, off_total = 0;
 };
 
 size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
@@ -204,8 +204,8 @@ int make_plan(int device, int64_t batch, int64_t hkv, int64_t gqa, int64_t head_
       return fail(PAD_ERR_UNSUPPORTED, "num_pages * page_size exceeds 64 bits");
     plan->raw_tiles = std::min(tiles_ub, groups * (weight_pages * page_size / tt + batch));
     plan->off_total = plan->bytes;
-    plan->off_pairs = plan->off_total + 256;
-    plan->off_tiles = align_up(plan->off_pairs + (size_t)(batch * groups) * sizeof(int2), 256);
+    plan->off_norm = plan->off_total + 256;
+    plan->off_tiles = align_up(plan->off_norm + (size_t)(batch * groups * hg * gqa) * sizeof(float2), 256);
     plan->off_raw = align_up(plan->off_tiles + (size_t)plan->raw_tiles * sizeof(int4), 256);
     plan->bytes = align_up(plan->off_raw + (size_t)plan->raw_tiles * kTileRows * gqa * sizeof(float), 256);
   }
@@ -308,7 +308,7 @@ int launch_merge(const MergeLaunch& m, cudaStream_t stream) {
   }
   MergeLaunch a = m;
   void* args[] = {&a.ws_o, &a.ws_ml, &a.ws_meta, &a.out, &a.out_sb, &a.out_sh, &a.ngroups, &a.rows, &a.guess_ncap,
-                  &a.guess_parts};
+                  &a.guess_parts, &a.norm};
   cudaLaunchConfig_t cfg = {};
   const int64_t pairs = m.batch * m.ngroups;
   const bool wide = m.partitions > kMergeWide * pairs;
@@ -541,7 +541,7 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
   if (wa != nullptr) {
     prm.track.raw = reinterpret_cast<float*>(ws + plan.off_raw);
     prm.track.tiles = reinterpret_cast<int4*>(ws + plan.off_tiles);
-    prm.track.pairs = reinterpret_cast<int2*>(ws + plan.off_pairs);
+    prm.track.norm = reinterpret_cast<float2*>(ws + plan.off_norm);
     prm.track.total = reinterpret_cast<int*>(ws + plan.off_total);
     prm.track.raw_tiles = (int)plan.raw_tiles;
   }
@@ -581,12 +581,12 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
     m.partitions = plan.partitions;
     m.head_dim = head_dim;
     m.meta_by_pair = prm.meta_by_pair;
+    m.norm = prm.track.norm;
     if ((st = launch_merge(m, s)) != PAD_OK) return st;
   }
   if (wa != nullptr) {
     WeightParams wp = {};
     wp.track = prm.track;
-    wp.ml = prm.ws_ml;
     wp.block_table = block_table;
     wp.total_lens = wa->total_lens;
     wp.weights = wa->weights;
@@ -600,9 +600,9 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
       wp.p2 = wa->position_strides[2];
     }
     wp.bt_stride = block_table_stride;
-    wp.hg = in.hg;
+    wp.hg_log2 = __builtin_ctz((unsigned)in.hg);
     wp.gqa = (int)gqa;
-    wp.tt = in.tt;
+    wp.tt_log2 = __builtin_ctz((unsigned)in.tt);
     wp.ngroups = (int)(num_kv_heads / in.hg);
     wp.page_size = (int)page_size;
     wp.page_shift = prm.page_shift;

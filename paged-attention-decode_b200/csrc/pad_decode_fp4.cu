@@ -61,7 +61,7 @@ int prepare(int device, const Fp4Instance& in) {
 struct Fp4Plan {
   int hg = 1;
   int64_t partitions = 1, slots = 0, raw_tiles = 0;
-  size_t off_ml = 0, off_o = 0, off_total = 0, off_pairs = 0, off_tiles = 0, off_raw = 0, bytes = 0;
+  size_t off_ml = 0, off_o = 0, off_total = 0, off_norm = 0, off_tiles = 0, off_raw = 0, bytes = 0;
 };
 
 int make_plan(int device, int64_t batch, int64_t hkv, int64_t gqa, int64_t head_dim, int64_t num_pages,
@@ -102,8 +102,8 @@ int make_plan(int device, int64_t batch, int64_t hkv, int64_t gqa, int64_t head_
     // as for the fp16 decode: no more tiles than the table names or the pool holds
     plan->raw_tiles = std::min(tiles_ub, groups * (num_pages * page_size / kTile + batch));
     plan->off_total = plan->bytes;
-    plan->off_pairs = plan->off_total + 256;
-    plan->off_tiles = align_up(plan->off_pairs + (size_t)pairs * sizeof(int2), 256);
+    plan->off_norm = plan->off_total + 256;
+    plan->off_tiles = align_up(plan->off_norm + (size_t)(pairs * rows) * sizeof(float2), 256);
     plan->off_raw = align_up(plan->off_tiles + (size_t)plan->raw_tiles * sizeof(int4), 256);
     plan->bytes = align_up(plan->off_raw + (size_t)(plan->raw_tiles * rows * kTile) * sizeof(float), 256);
   }
@@ -260,7 +260,7 @@ extern "C" int pad_paged_attention_decode_fp4(
   if (weights != nullptr) {
     p.track.raw = reinterpret_cast<float*>(ws + plan.off_raw);
     p.track.tiles = reinterpret_cast<int4*>(ws + plan.off_tiles);
-    p.track.pairs = reinterpret_cast<int2*>(ws + plan.off_pairs);
+    p.track.norm = reinterpret_cast<float2*>(ws + plan.off_norm);
     p.track.total = reinterpret_cast<int*>(ws + plan.off_total);
     p.track.raw_tiles = (int)plan.raw_tiles;
   }
@@ -296,12 +296,12 @@ extern "C" int pad_paged_attention_decode_fp4(
     m.partitions = plan.partitions;
     m.head_dim = head_dim;
     m.meta_by_pair = p.meta_by_pair;
+    m.norm = p.track.norm;
     if ((st = launch_merge(m, s)) != PAD_OK) return st;
   }
   if (weights != nullptr) {
     WeightParams wp = {};
     wp.track = p.track;
-    wp.ml = p.ws_ml;
     wp.block_table = block_table;
     wp.total_lens = total_lens;
     wp.weights = weights;
@@ -315,9 +315,9 @@ extern "C" int pad_paged_attention_decode_fp4(
       wp.p2 = position_strides[2];
     }
     wp.bt_stride = block_table_stride;
-    wp.hg = plan.hg;
+    wp.hg_log2 = p.hg_log2;
     wp.gqa = (int)gqa;
-    wp.tt = kTile;
+    wp.tt_log2 = __builtin_ctz((unsigned)kTile);
     wp.ngroups = (int)(num_kv_heads / plan.hg);
     wp.page_size = (int)page_size;
     wp.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)page_size) : -1;

@@ -618,11 +618,11 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
     const Fp4Cursor done = seg;
     const int pair = seg.b * ngroups + seg.hg, slot = pair + w;
     if (tid == 0 && seg_t == seg.start) {
-      const int owner = split ? part_owner((int64_t)seg.start + seg.n - 1, total, W) : w;
-      if (split || p.meta_by_pair)
+      if (split || p.meta_by_pair) {
+        const int owner = part_owner((int64_t)seg.start + seg.n - 1, total, W);
         p.ws_meta[p.meta_by_pair ? pair : w] =
             split ? make_int4(pair, slot, owner - w + 1, 1) : make_int4(-1, 0, 0, 0);
-      if constexpr (TR::WT) p.track.pairs[pair] = make_int2(slot, owner - w + 1);
+      }
     }
     const bool more = seg_end < t1;
     if (more) {  // the next segment's queries arrive while this one is joined
@@ -676,7 +676,11 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
         out[0] = __floats2half2_rn(o.x * inv, o.y * inv);
         out[1] = __floats2half2_rn(o.z * inv, o.w * inv);
       }
-      if ((split || TR::WT) && d == 0) p.ws_ml[(int64_t)slot * HG * G + row] = make_float2(Mu, L);
+      if (split && d == 0) p.ws_ml[(int64_t)slot * HG * G + row] = make_float2(Mu, L);
+      if constexpr (TR::WT) {
+        if (!split && d == 0)
+          p.track.norm[(int64_t)pair * HG * G + row] = make_float2(Mu, L == 0.f ? 0.f : 1.f / L);
+      }
     }
     if (!more) break;
     named_barrier(1 + hl, 32 * WPH);  // the buffers are read before the next segment writes them

@@ -74,6 +74,7 @@ struct MergeLaunch {
   int guess_ncap, guess_parts;  // closed-form descriptors (guess_ncap 0: none)
   int64_t batch, partitions, head_dim;
   int meta_by_pair;
+  float2* norm;                 // where the rows' (M, 1 / L) go, or null
 };
 int launch_merge(const MergeLaunch& m, cudaStream_t stream);
 

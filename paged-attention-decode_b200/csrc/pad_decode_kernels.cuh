@@ -455,10 +455,6 @@ __global__ void __launch_bounds__(kThreads, 1) decode_stream_kernel(const __grid
         if constexpr (TR::WT) {
           if (t0 + k < p.track.raw_tiles) p.track.tiles[t0 + k] = make_int4(c.b, c.hg, c.i, c.seq);
           else raise_flag(p, PAD_FLAG_SHARED_PAGE);
-          if (c.i == 0) {
-            const int owner = split ? part_owner((int64_t)c.pair_start + c.n - 1, total, W) : w;
-            p.track.pairs[pair] = make_int2(pair + w, owner - w + 1);
-          }
         }
       }
       if (k == 0 && lane == 0) PAD_STAMP(2);
@@ -800,7 +796,12 @@ __global__ void __launch_bounds__(kThreads, 1) decode_stream_kernel(const __grid
             if (g >= G) continue;
             const float L = lsum[nt][j];
             const float inv = L > 0.f ? 1.f / L : 0.f;
-            if ((split || TR::WT) && (lane >> 2) == 0) p.ws_ml[prow + g] = make_float2(m_run[nt][j], L);
+            if (split && (lane >> 2) == 0) p.ws_ml[prow + g] = make_float2(m_run[nt][j], L);
+            if constexpr (TR::WT) {
+              if (!split && (lane >> 2) == 0)
+                p.track.norm[(int64_t)(dsc.b * ngroups + dsc.hg) * (HG * G) + hl * G + g] =
+                    make_float2(m_run[nt][j] == -INFINITY ? 0.f : m_run[nt][j], L == 0.f ? 0.f : 1.f / L);
+            }
 #pragma unroll
             for (int mt = 0; mt < KSTEPS; ++mt)
 #pragma unroll
@@ -911,9 +912,15 @@ __global__ void __launch_bounds__(kThreads, 1) decode_stream_kernel(const __grid
             o4[x] = v;
           }
         }
-        if (split || TR::WT)
-          for (int x = ctid; x < HG * G; x += 32 * kConsumerWarps)
-            p.ws_ml[(int64_t)dsc.slot * HG * G + x] = sML[(x / G) * 8 * NT + x % G];
+        for (int x = ctid; (split || TR::WT) && x < HG * G; x += 32 * kConsumerWarps) {
+          const float2 ml = sML[(x / G) * 8 * NT + x % G];
+          if (split) {
+            p.ws_ml[(int64_t)dsc.slot * HG * G + x] = ml;
+          } else if constexpr (TR::WT) {
+            p.track.norm[(int64_t)(dsc.b * ngroups + dsc.hg) * (HG * G) + x] =
+                make_float2(ml.x, ml.y == 0.f ? 0.f : 1.f / ml.y);
+          }
+        }
         // No trailing sync: the next epilogue's first sync orders these reads
         // before any warp writes the buffer again.
       }
@@ -945,7 +952,8 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const float* __res
                                                               const int4* __restrict__ ws_meta,
                                                               __half* __restrict__ out, int64_t out_sb,
                                                               int64_t out_sh, int ngroups, int rows,
-                                                              int guess_ncap, int guess_parts) {
+                                                              int guess_ncap, int guess_parts,
+                                                              float2* __restrict__ norm) {
   constexpr int DC = D / DS;               // columns of D this CTA merges (blockIdx.z picks which)
   constexpr int C4 = DC / 4;               // float4 columns of one partial row slice
   constexpr int PG = kMergeThreads / C4;   // partial groups folded in parallel
@@ -1065,6 +1073,9 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const float* __res
       L += red_l[x] * wt;
     }
     const float inv = L > 0.f ? 1.f / L : 0.f;
+    // (maximum, 1 / sum) of the row, for the attention weights
+    if (norm != nullptr && tid == 0 && blockIdx.z == 0)
+      norm[(int64_t)pair * rows + y] = make_float2(Mu, L == 0.f ? 0.f : 1.f / L);
     const int b = pair / ngroups, hg = pair % ngroups;
     __half* o = out + b * out_sb + (int64_t)(hg * rows + y) * out_sh + blockIdx.z * DC + tid * 4;
     reinterpret_cast<__half2*>(o)[0] = __floats2half2_rn(t.x * inv, t.y * inv);

@@ -12,7 +12,8 @@ int launch_weights(const WeightParams& p, cudaStream_t stream) {
   WeightParams prm = p;
   void* args[] = {&prm};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)std::min(p.track.raw_tiles, kWeightGrid));
+  const int64_t elements = (int64_t)p.track.raw_tiles << (p.hg_log2 + p.tt_log2);
+  cfg.gridDim = dim3((unsigned)std::min<int64_t>((elements + kWeightThreads - 1) / kWeightThreads, kWeightGrid));
   cfg.blockDim = dim3(kWeightThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -9,7 +9,7 @@
 // and sum of the whole row. The decode kernel holds a token's score long before
 // (M_g, L_g) are known, so it stores the scores in fp32 (4 G bytes a token and
 // KV head beside the 4 D bytes of K and V it reads) and this kernel reads them
-// back, usually from L2, when all (m, l) partials are there. Recomputing them
+// back, usually from L2, when every row's (M, 1 / L) is there. Recomputing them
 // would read K again, 2 D bytes. 2^(s - M) / L instead of 2^(s - M - log2 L):
 // s - M is exact where it matters, so no rounding of a large exponent enters.
 #pragma once
@@ -24,19 +24,19 @@ namespace pad {
 struct TrackParams {
   float* raw;     // [raw_tiles][HG * G][TT] scores in log2 units
   int4* tiles;    // [raw_tiles] {sequence, head group, tile of the pair, seq_len}
-  int2* pairs;    // [batch * head groups] {first (m, l) slot, slots}
+  float2* norm;   // [batch * head groups][HG * G] {M, 1 / L}: by the decode kernel for
+                  // pairs that one CTA finished, by the merge kernel for split ones
   int* total;     // tiles of the batch
   int raw_tiles;  // tiles there is room for: what the pool's pages can hold, each in one sequence
 };
 
 struct WeightParams {
   TrackParams track;
-  const float2* ml;  // [slots][HG * G] (m, l), m in log2 units
   const int32_t *block_table, *total_lens;
   float* weights;
   int32_t* slot_positions;
   int64_t w0, w1, w2, p0, p1, p2, bt_stride;
-  int hg, gqa, tt, ngroups, page_size, page_shift, num_pages, num_new;
+  int hg_log2, gqa, tt_log2, ngroups, page_size, page_shift, num_pages, num_new;
 };
 
 // Adds the weights of the decode whose kernels precede it in the stream.

@@ -8,64 +8,53 @@
 
 namespace pad {
 
-constexpr int kWeightThreads = 128;
-constexpr int kWeightGrid = 148 * 16;  // every SM full; more tiles loop
-constexpr int kMaxTrackRows = 128;  // query rows of a head group: 8 heads x 8, 4 x 16
+constexpr int kWeightThreads = 256;
+constexpr int kWeightGrid = 148 * 8;  // every SM full; more tiles loop
 
-// One tile at a time: fold the (m, l) of its rows (a warp per row, its lanes
-// over the slots), then a thread per (head, token) adds up the heads.
+// A thread per (head, token) of a tile. What it needs is three loads deep: the
+// scores (their place follows from the tile's number) with the tile's record,
+// then the norms with the page id, then the weight itself. Each weight has one
+// writer, so results do not depend on any order.
 __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const __grid_constant__ WeightParams p) {
-  __shared__ float sM[kMaxTrackRows], sI[kMaxTrackRows];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int rows = p.hg * p.gqa;
   pdl_launch_dependents();
   pdl_wait_primary();
-  const int total = min(*p.track.total, p.track.raw_tiles);
-  for (int t = blockIdx.x; t < total; t += gridDim.x) {
-    const int4 d = p.track.tiles[t];
-    const int2 pr = p.track.pairs[d.x * p.ngroups + d.y];
-    for (int r = warp; r < rows; r += kWeightThreads / 32) {
-      float m = -INFINITY, l = 0.f;
-      for (int s = lane; s < pr.y; s += 32) {
-        const float2 x = p.ml[(int64_t)(pr.x + s) * rows + r];
-        const float mn = fmaxf(m, x.x), mu = mn == -INFINITY ? 0.f : mn;
-        l = l * ex2(m - mu) + x.y * ex2(x.x - mu);
-        m = mn;
-      }
-      float M = m;
+  const int per_log2 = p.hg_log2 + p.tt_log2, tt = 1 << p.tt_log2, G = p.gqa;
+  const int64_t total = (int64_t)min(*p.track.total, p.track.raw_tiles) << per_log2;
+  for (int64_t e = (int64_t)blockIdx.x * kWeightThreads + threadIdx.x; e < total; e += (int64_t)gridDim.x * kWeightThreads) {
+    const int64_t t = e >> per_log2, ht = e >> p.tt_log2;  // tile; (tile, head)
+    const int hl = (int)ht & ((1 << p.hg_log2) - 1), tok = (int)e & (tt - 1);
+    const float* raw = p.track.raw + ((ht * G) << p.tt_log2) + tok;
+    float s[4];
+    const int4 d = __ldg(p.track.tiles + t);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-      if (M == -INFINITY) M = 0.f;
-      l *= ex2(m - M);
+    for (int g = 0; g < 4; ++g)
+      if (g < G) s[g] = __ldg(raw + (g << p.tt_log2));
+    const int slot = (d.z << p.tt_log2) + tok;
+    if (slot >= d.w) continue;
+    const int lp = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
+    const int page = __ldg(p.block_table + d.x * p.bt_stride + lp);
+    const float2* norm = p.track.norm + ((int64_t)(d.x * p.ngroups + d.y) << p.hg_log2) * G + hl * G;
+    const int64_t row = slot - (int64_t)lp * p.page_size;
+    if ((unsigned)page >= (unsigned)p.num_pages) continue;  // flagged by the decode kernel
+    const int h = (d.y << p.hg_log2) + hl;
+    float* w = p.weights + page * p.w0 + h * p.w1 + row * p.w2;
+    const bool fresh = slot >= d.w - p.num_new;
+    const float was = fresh ? 0.f : *w;
+    float sum = 0.f;
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-      if (lane == 0) {
-        sM[r] = M;
-        sI[r] = l == 0.f ? 0.f : 1.f / l;
+    for (int g = 0; g < 4; ++g)
+      if (g < G) {
+        const float2 n = __ldg(norm + g);
+        sum += ex2(s[g] - n.x) * n.y;
       }
+#pragma unroll 4
+    for (int g = 4; g < G; ++g) {
+      const float2 n = __ldg(norm + g);
+      sum += ex2(__ldg(raw + (g << p.tt_log2)) - n.x) * n.y;
     }
-    __syncthreads();
-    const float* raw = p.track.raw + (int64_t)t * rows * p.tt;
-    for (int x = tid; x < p.hg * p.tt; x += kWeightThreads) {
-      const int hl = x / p.tt, tok = x - hl * p.tt, slot = d.z * p.tt + tok;
-      if (slot >= d.w) continue;
-      float sum = 0.f;
-      for (int g = 0; g < p.gqa; ++g) {
-        const int r = hl * p.gqa + g;
-        sum += ex2(raw[r * p.tt + tok] - sM[r]) * sI[r];
-      }
-      const int lp = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
-      const int64_t row = slot - (int64_t)lp * p.page_size;
-      const int page = __ldg(p.block_table + d.x * p.bt_stride + lp);
-      if ((unsigned)page >= (unsigned)p.num_pages) continue;  // flagged by the decode kernel
-      const int h = d.y * p.hg + hl;
-      float* w = p.weights + page * p.w0 + h * p.w1 + row * p.w2;
-      const bool fresh = slot >= d.w - p.num_new;
-      *w = fresh ? sum : *w + sum;
-      if (fresh && p.slot_positions != nullptr)
-        p.slot_positions[page * p.p0 + h * p.p1 + row * p.p2] = __ldg(p.total_lens + d.x) - d.w + slot;
-    }
-    __syncthreads();
+    *w = was + sum;
+    if (fresh && p.slot_positions != nullptr)
+      p.slot_positions[page * p.p0 + h * p.p1 + row * p.p2] = __ldg(p.total_lens + d.x) - d.w + slot;
   }
 }
 
