@@ -600,6 +600,8 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
       wp.p2 = wa->position_strides[2];
     }
     wp.bt_stride = block_table_stride;
+    wp.batch = (int)batch;
+    wp.cap = (int)(max_pages_per_seq * page_size);
     wp.hg_log2 = __builtin_ctz((unsigned)in.hg);
     wp.gqa = (int)gqa;
     wp.tt_log2 = __builtin_ctz((unsigned)in.tt);
@@ -607,7 +609,7 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
     wp.page_size = (int)page_size;
     wp.page_shift = prm.page_shift;
     wp.num_pages = (int)num_pages;
-    wp.num_new = (int)std::min<int64_t>(wa->num_new, INT32_MAX);
+    wp.num_new = (int)std::min<int64_t>(wa->num_new, wp.cap);
     if ((st = launch_weights(wp, s)) != PAD_OK) return st;
   }
   return PAD_OK;

@@ -315,6 +315,8 @@ extern "C" int pad_paged_attention_decode_fp4(
       wp.p2 = position_strides[2];
     }
     wp.bt_stride = block_table_stride;
+    wp.batch = (int)batch;
+    wp.cap = (int)(max_pages_per_seq * page_size);
     wp.hg_log2 = p.hg_log2;
     wp.gqa = (int)gqa;
     wp.tt_log2 = __builtin_ctz((unsigned)kTile);
@@ -322,7 +324,7 @@ extern "C" int pad_paged_attention_decode_fp4(
     wp.page_size = (int)page_size;
     wp.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctzll((unsigned long long)page_size) : -1;
     wp.num_pages = (int)num_pages;
-    wp.num_new = (int)std::min<int64_t>(num_new, INT32_MAX);
+    wp.num_new = (int)std::min<int64_t>(num_new, wp.cap);
     if ((st = launch_weights(wp, s)) != PAD_OK) return st;
   }
   return PAD_OK;

@@ -12,7 +12,7 @@ int launch_weights(const WeightParams& p, cudaStream_t stream) {
   WeightParams prm = p;
   void* args[] = {&prm};
   cudaLaunchConfig_t cfg = {};
-  const int64_t elements = (int64_t)p.track.raw_tiles << (p.hg_log2 + p.tt_log2);
+  const int64_t elements = (int64_t)p.track.raw_tiles << (p.hg_log2 + p.tt_log2 - 2);
   cfg.gridDim = dim3((unsigned)std::min<int64_t>((elements + kWeightThreads - 1) / kWeightThreads, kWeightGrid));
   cfg.blockDim = dim3(kWeightThreads);
   cfg.stream = stream;
@@ -21,7 +21,10 @@ int launch_weights(const WeightParams& p, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(&weights_kernel), args);
+  const void* kernel = p.gqa <= 4   ? reinterpret_cast<const void*>(&weights_kernel<4>)
+                       : p.gqa <= 8 ? reinterpret_cast<const void*>(&weights_kernel<8>)
+                                    : reinterpret_cast<const void*>(&weights_kernel<16>);
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, kernel, args);
   return e == cudaSuccess ? PAD_OK : cuda_fail(e, "launching the attention-weight kernel");
 }
 

@@ -36,6 +36,7 @@ struct WeightParams {
   float* weights;
   int32_t* slot_positions;
   int64_t w0, w1, w2, p0, p1, p2, bt_stride;
+  int batch, cap;  // sequences; slots a table row names
   int hg_log2, gqa, tt_log2, ngroups, page_size, page_shift, num_pages, num_new;
 };
 

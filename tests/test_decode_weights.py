@@ -84,7 +84,7 @@ def test_weights_and_positions_match_float64(seqs, hkv, g, d, ps, num_splits):
     ref, probs = co.decode(c.q, c.k_cache, c.v_cache, c.block_table, c.seq_lens)
     bound = rel_bound(d, max(seqs), smax_of(c.q, c.k_cache, d))
     q, k, v, bt, sl = _case_inputs(c)
-    for num_new in (1, 0, 5, 10 ** 6):
+    for num_new in (1, 0, 5, 2 ** 31 - 1):
         w, at = _cuda(w0), _cuda(at0)
         out = pad_b200.paged_attention_decode_weights(q, k, v, bt, sl, w, num_new, num_splits, slot_positions=at,
                                                       total_lens=_cuda(total))
