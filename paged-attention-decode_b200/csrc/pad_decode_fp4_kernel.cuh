@@ -257,33 +257,33 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
   const uint64_t policy = l2_evict_first_policy();
   const uint32_t chunk = lane % TR::CPR, row_of_lane = lane / TR::CPR;
   const uint32_t copy_dst = row_of_lane * TR::ROW + ((chunk ^ TR::swz(row_of_lane)) << 4);
-  Fp4Cursor ld = seg;     // next tile to copy
-  int ld_t = t0 + turn;
-  walk.advance(ld, turn);
   // Where this lane's token of a tile lies: its page (-1: it has no token) and
   // row, and the tile. Page ids are loaded a turn before the copy that needs them.
   struct Place {
     int page, row, left;  // left: tokens of the sequence from the tile's first on (0: no tile)
     uint32_t head;
   };
-  const int32_t* ids = p.block_table + (int64_t)ld.b * p.bt_stride;  // page ids of ld's sequence
-  int ids_of = ld.b;
+  Fp4Cursor ld = seg;                  // the pair of the tile looked up last
+  int ld_t = t0 + turn - WPH;          // that tile (before the first: a turn ahead of it)
+  int ld_tok = (seg.i + turn - WPH) * TT + lane;  // this lane's token in it
+  const int32_t* ids = p.block_table + (int64_t)ld.b * p.bt_stride;  // page ids of its sequence
+  // From the place of one tile of this warp to that of its next.
   auto place = [&](Place& o) {
+    ld_t += WPH;
+    ld_tok += WPH * TT;
     o.left = 0;
-    if (ld_t < t1) {
-      if (ld.b != ids_of) {
-        ids_of = ld.b;
-        ids = p.block_table + (int64_t)ids_of * p.bt_stride;
-      }
-      const int tok = ld.i * TT + lane;
-      const int lp = __umulhi(2u * (uint32_t)tok, p.page_mul) >> p.page_shr;
-      o.row = tok - lp * p.page_size;
-      o.left = ld.seq - ld.i * TT;
-      o.head = ld.hg * HG + hl;
-      o.page = lane < o.left ? ld_nc_early(ids + lp) : -1;
-      ld_t += WPH;
-      walk.advance(ld, WPH);
+    if (ld_t >= t1) return;
+    if (ld_tok - lane >= ld.seq) {  // another pair
+      ld.i = (ld_tok - lane) / TT;
+      walk.advance(ld, 0);
+      ld_tok = ld.i * TT + lane;
+      ids = p.block_table + (int64_t)ld.b * p.bt_stride;
     }
+    const int lp = __umulhi(2u * (uint32_t)ld_tok, p.page_mul) >> p.page_shr;
+    o.row = ld_tok - lp * p.page_size;
+    o.left = ld.seq - (ld_tok - lane);
+    o.head = ld.hg * HG + hl;
+    o.page = ld_tok < ld.seq ? ld_nc_early(ids + lp) : -1;
   };
   bool bad_page = false;
   const uint8_t *k_chunk = p.k + chunk * 16, *v_chunk = p.v + chunk * 16;
