@@ -29,6 +29,7 @@
 #include <atomic>
 #include <climits>
 #include <cstdint>
+#include <cstdlib>
 
 #include "pad_b200.h"
 #include "pad_error.cuh"
@@ -51,7 +52,8 @@ struct PlanParams {
   const float* weights;
   const int32_t *slot_positions, *block_table, *seq_lens, *total_lens;
   int32_t *src, *dst, *counts, *new_lens;
-  int64_t w0, w1, w2, p0, p1, p2;  // element strides of weights and slot_positions [page][head][row]
+  int64_t w1, p1;          // element strides of weights and slot_positions: heads,
+  int w0, w2, p0, p2;      // pages and rows
   int64_t bt_stride;
   int hkv, num_pages, page_size, page_shift, max_pages, budget, recent, max_moves;
   int key_cap;  // keys of shared memory per CTA
@@ -77,25 +79,31 @@ template <bool CACHED>
 struct SlotKeys {
   const PlanParams& p;
   const uint32_t* cached;
-  int64_t bt_row;
-  int h, first;
-  int64_t oldest_recent;  // slots whose position is at least this are recent
+  const float* weights;      // of this KV head
+  const int32_t* positions;  // of this KV head, or null
+  const int32_t* ids;        // page ids of this sequence
+  int first;
+  int64_t oldest_recent;     // slots whose position is at least this are recent
   __device__ __forceinline__ int page_slot(int slot) const {
     return p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
   }
+  __device__ __forceinline__ const float* weight_at(int page, int row) const {
+    return weights + ((int64_t)page * p.w0 + (int64_t)row * p.w2);
+  }
+  __device__ __forceinline__ const int32_t* position_at(int page, int row) const {
+    return positions + ((int64_t)page * p.p0 + (int64_t)row * p.p2);
+  }
   __device__ __forceinline__ uint32_t key(float w, int at) const {
-    return p.slot_positions != nullptr && at >= oldest_recent ? kRecentKey : weight_key(w);
+    return positions != nullptr && at >= oldest_recent ? kRecentKey : weight_key(w);
   }
   // Slots past the shared-memory share are read again wherever they are needed;
   // those of a page that is none weigh least.
   __device__ __forceinline__ uint32_t at(int slot) const {
     const int i = slot - first;
     if (CACHED || i < p.key_cap) return cached[i];
-    const int lp = page_slot(slot), page = __ldg(p.block_table + bt_row + lp);
-    const int64_t row = slot - (int64_t)lp * p.page_size;
+    const int lp = page_slot(slot), page = __ldg(ids + lp), row = slot - lp * p.page_size;
     if ((unsigned)page >= (unsigned)p.num_pages) return 0u;
-    const int pos = p.slot_positions != nullptr ? __ldg(p.slot_positions + page * p.p0 + h * p.p1 + row * p.p2) : 0;
-    return key(__ldg(p.weights + page * p.w0 + h * p.w1 + row * p.w2), pos);
+    return key(__ldg(weight_at(page, row)), positions != nullptr ? __ldg(position_at(page, row)) : 0);
   }
 };
 
@@ -188,8 +196,13 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
   if (n > p.budget) {
     const int share = (n + RANKS - 1) / RANKS;
     const int first = min(n, rank * share), last = min(n, first + share);
-    const SlotKeys<CACHED> key{p, keys, (int64_t)b * p.bt_stride, h, first,
-                       p.slot_positions != nullptr ? (int64_t)__ldg(p.total_lens + b) - p.recent : 0};
+    const SlotKeys<CACHED> key{p,
+                               keys,
+                               p.weights + h * p.w1,
+                               p.slot_positions != nullptr ? p.slot_positions + h * p.p1 : nullptr,
+                               p.block_table + (int64_t)b * p.bt_stride,
+                               first,
+                               p.slot_positions != nullptr ? (int64_t)__ldg(p.total_lens + b) - p.recent : 0};
     for (int x = tid; x < 3 * kBins / 4; x += kPlanThreads)
       reinterpret_cast<int4*>(&sh.hist[0][0])[x] = make_int4(0, 0, 0, 0);
     __syncthreads();
@@ -203,7 +216,7 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
         const int s = s0 + u * kPlanThreads + tid;
         const int lp = key.page_slot(s);
         row[u] = s - lp * p.page_size;
-        page[u] = s < last ? __ldg(p.block_table + key.bt_row + lp) : -1;
+        page[u] = s < last ? __ldg(key.ids + lp) : -1;
       }
 #pragma unroll
       for (int u = 0; u < kGather; ++u) {
@@ -212,8 +225,8 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
         w[u] = 0.f;
         at[u] = 0;
         if (ok) {
-          w[u] = __ldg(p.weights + page[u] * p.w0 + h * p.w1 + row[u] * p.w2);
-          if (p.slot_positions != nullptr) at[u] = __ldg(p.slot_positions + page[u] * p.p0 + h * p.p1 + row[u] * p.p2);
+          w[u] = __ldg(key.weight_at(page[u], row[u]));
+          if (key.positions != nullptr) at[u] = __ldg(key.position_at(page[u], row[u]));
         }
       }
 #pragma unroll
@@ -260,22 +273,30 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
       if constexpr (RANKS > 1)
         for (int r = 0; r < rank; ++r) eq_base += cg::this_cluster().map_shared_rank(&sh, r)->hist[2][T & 1023u];
     }
-    // which of 32 slots are kept, and the running number of equals before them
-    auto kept = [&](int s, int& seen) {
+    // the slots kept of a run of 32, and the running number of equals before them
+    auto kept = [&](int s, int& seen) -> uint32_t {
       const uint32_t k = s < hi ? key.at(s) : 0u;
-      if (all_eq) return s < hi && k >= T;
+      if (all_eq) return __ballot_sync(0xffffffffu, s < hi && k >= T);
       const uint32_t e = __ballot_sync(0xffffffffu, s < hi && k == T);
-      const bool on = s < hi && (k > T || (k == T && seen + __popc(e & below) < need));
+      const uint32_t on = __ballot_sync(0xffffffffu, s < hi && (k > T || (k == T && seen + __popc(e & below) < need)));
       seen += __popc(e);
       return on;
     };
+    // Runs below the budget (those not kept are holes), the run across it, and
+    // runs above it (those kept are movers).
+    const int mid = lo + max(0, min(p.budget, hi) - lo) / 32 * 32;
+    const int mid2 = mid < hi && mid < p.budget ? mid + 32 : mid;
+    const uint32_t low = p.budget - mid >= 32 ? 0xffffffffu : (1u << max(0, p.budget - mid)) - 1u;  // of the run across
     int holes = 0, movers = 0, seen = eq_base;
 #pragma unroll 4
-    for (int s = lo + lane; s - lane < hi; s += 32) {
-      const bool on = kept(s, seen);
-      movers += __popc(__ballot_sync(0xffffffffu, on && s >= p.budget));
-      holes += __popc(__ballot_sync(0xffffffffu, s < hi && !on && s < p.budget));
+    for (int s = lo + lane; s - lane < mid; s += 32) holes += 32 - __popc(kept(s, seen));
+    if (mid2 > mid) {
+      const uint32_t on = kept(mid + lane, seen), in = hi - mid >= 32 ? 0xffffffffu : (1u << (hi - mid)) - 1u;
+      holes += __popc(~on & low & in);
+      movers += __popc(on & ~low);
     }
+#pragma unroll 4
+    for (int s = mid2 + lane; s - lane < hi; s += 32) movers += __popc(kept(s, seen));
     int hole_at = warp_base(sh, holes, &total);
     if (tid == 0) sh.holes = total;
     int mover_at = warp_base(sh, movers, &total);
@@ -292,18 +313,21 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
       count += om;
     }
     seen = eq_base;
+    // (never past max_moves unless the inputs change while the kernel runs)
+    auto put = [&](int32_t* list, int& at, uint32_t on, int s) {
+      const int i = at + __popc(on & below);
+      if (((on >> lane) & 1u) && i < p.max_moves) list[i] = s;
+      at += __popc(on);
+    };
 #pragma unroll 4
-    for (int s = lo + lane; s - lane < hi; s += 32) {
-      const bool on = kept(s, seen);
-      const uint32_t m = __ballot_sync(0xffffffffu, on && s >= p.budget);
-      const uint32_t o = __ballot_sync(0xffffffffu, s < hi && !on && s < p.budget);
-      // (never past max_moves unless the inputs change while the kernel runs)
-      const int mi = mover_at + __popc(m & below), oi = hole_at + __popc(o & below);
-      if (((m >> lane) & 1u) && mi < p.max_moves) src[mi] = s;
-      if (((o >> lane) & 1u) && oi < p.max_moves) dst[oi] = s;
-      mover_at += __popc(m);
-      hole_at += __popc(o);
+    for (int s = lo + lane; s - lane < mid; s += 32) put(dst, hole_at, ~kept(s, seen), s);
+    if (mid2 > mid) {
+      const uint32_t on = kept(mid + lane, seen), in = hi - mid >= 32 ? 0xffffffffu : (1u << (hi - mid)) - 1u;
+      put(dst, hole_at, ~on & low & in, mid + lane);
+      put(src, mover_at, on & ~low, mid + lane);
     }
+#pragma unroll 4
+    for (int s = mid2 + lane; s - lane < hi; s += 32) put(src, mover_at, kept(s, seen), s);
     if constexpr (RANKS > 1) cg::this_cluster().sync();  // no CTA leaves while another may read its shared memory
   }
   if (tid == 0 && rank == 0) p.counts[pair] = count;
@@ -493,15 +517,18 @@ extern "C" int pad_paged_kv_evict_plan(const float* weights, const int32_t* slot
   p.dst = dst;
   p.counts = counts;
   p.new_lens = new_lens;
+  for (const int64_t* st2 : {weight_strides, p.slot_positions != nullptr ? position_strides : nullptr})
+    if (st2 != nullptr && (std::abs(st2[0]) > INT32_MAX || std::abs(st2[2]) > INT32_MAX))
+      return fail(PAD_ERR_UNSUPPORTED, "evict_plan: page and row strides must fit 32 bits");
   if (weight_strides != nullptr) {
-    p.w0 = weight_strides[0];
+    p.w0 = (int)weight_strides[0];
     p.w1 = weight_strides[1];
-    p.w2 = weight_strides[2];
+    p.w2 = (int)weight_strides[2];
   }
   if (p.slot_positions != nullptr) {
-    p.p0 = position_strides[0];
+    p.p0 = (int)position_strides[0];
     p.p1 = position_strides[1];
-    p.p2 = position_strides[2];
+    p.p2 = (int)position_strides[2];
   }
   p.bt_stride = block_table_stride;
   p.hkv = (int)num_kv_heads;
