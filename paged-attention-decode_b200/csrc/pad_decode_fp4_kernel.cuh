@@ -27,6 +27,12 @@
 // Rows of tokens past the sequence, and of pages that are none, are copied as
 // zeros (cp.async with no source bytes): zero codes with a finite scale, so
 // nothing that a page holds behind its sequence reaches the sums.
+//
+// Measured (12/2 heads, head_dim 128, page 16): 64 x 4096 tokens 24.8 us a call
+// (10.9 at the measured copy rate), each further 4096 tokens of the 64 sequences
+// 14.3 us (72% of the copy rate); one sequence of 131072 tokens 16.4 us (5.4).
+// About 625 instructions a piece of 32 tokens; the schedulers issue in 59% of the
+// cycles and the integer pipe, which also converts, is busy in 51%.
 #pragma once
 
 #include <climits>
@@ -71,9 +77,9 @@ template <int D_, int NT_, bool WT_>
 struct Fp4Traits {
   static constexpr int D = D_, NT = NT_;
   static constexpr bool WT = WT_;
-  // Warps: 12 of 168 registers, 8 of 255 for two query tiles. 16 of 128 spend 70
-  // more instructions a tile on recomputing addresses (64 x 4096, 12/2 heads:
-  // 29.4 us against 28.5), 8 leave two warps a scheduler (30.8).
+  // Warps: 12 of 168 registers, 8 of 255 for two query tiles. When this was chosen
+  // (64 x 4096, 12/2 heads) 12 took 28.5 us; 16 of 128 registers 29.4, with 70 more
+  // instructions a tile to recompute addresses; 8, two a scheduler, 30.8.
   static constexpr int NW = NT == 1 ? 12 : 8;
   static constexpr int THREADS = 32 * NW;
   static constexpr int TT = 32;                    // tokens per tile
@@ -496,16 +502,16 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
           atomicOr(p.error_flags, PAD_FLAG_SHARED_PAGE);
         }
       }
-      // ---- copy a later tile into the slot of the one before this. (Here its
-      // instructions fill the gaps between scores and softmax; at the end of a
-      // turn they cost 64 x 4096 28.6 us against 26.4.)
+      // ---- copy a later tile into the slot of the one before this. Here its
+      // instructions fill the gaps between scores and softmax: 26.4 us at 64 x 4096
+      // against 28.6 with the copy at the end of a turn, when it was moved.
       copy(next, stage == 0 ? S - 1 : stage - 1);
       place(next);
       // ---- online softmax over the 32 tokens. The reference point m_run need not be
       // the maximum, only near it: it moves when a score passes it by more than
       // kSlack, so p <= 2^kSlack, which fp16's range takes and which cancels in
-      // O / l. Nearly every tile then needs no exchange between lanes, no rescaling
-      // (always rescaling: 76.1 us at 64 x 16384 against 73.2).
+      // O / l. Nearly every tile then needs no exchange between lanes and no
+      // rescaling (64 x 16384: 71.9 -> 68.7 us).
       bool beyond = false;
       float top[NT][2];
 #pragma unroll
