@@ -303,7 +303,12 @@ at::Tensor decode_weights(const at::Tensor& q_in, const at::Tensor& k, const at:
                           const at::Tensor& sl_in, int64_t num_splits, double scale,
                           const c10::optional<at::Tensor>& out_in, const at::Tensor& weights, int64_t num_new,
                           const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& total_in) {
-  TORCH_CHECK(q_in.dim() == 3 && k.dim() == 4 && v.sizes() == k.sizes(), "bad q / k_cache / v_cache shapes");
+  TORCH_CHECK(q_in.dim() == 3 && k.dim() == 4 && v.sizes() == k.sizes() && k.size(2) > 0 && k.size(3) == q_in.size(2),
+              "libpad_b200 decode_weights: bad q / k_cache / v_cache shapes");
+  TORCH_CHECK(q_in.scalar_type() == at::kHalf && k.scalar_type() == at::kHalf && v.scalar_type() == at::kHalf,
+              "libpad_b200 decode_weights: q, k_cache and v_cache must be fp16");
+  TORCH_CHECK(bt_in.dim() == 2 && bt_in.size(0) == q_in.size(0) && sl_in.dim() == 1 && sl_in.size(0) == q_in.size(0),
+              "libpad_b200 decode_weights: block_table must be [B, max_pages], seq_lens [B]");
   const at::Device dev = q_in.device();
   check_on(dev, {&k, &v}, "decode_weights");
   c10::cuda::CUDAGuard guard(dev);
@@ -339,7 +344,7 @@ at::Tensor decode_fp4(const at::Tensor& q_in, const at::Tensor& k, const at::Ten
   const at::Device dev = q_in.device();
   check_fp4(k, ks, v, vs, "decode_fp4");
   check_on(dev, {&k, &ks, &v, &vs}, "decode_fp4");
-  TORCH_CHECK(q_in.dim() == 3 && q_in.scalar_type() == at::kHalf && q_in.size(2) == 2 * k.size(3),
+  TORCH_CHECK(q_in.dim() == 3 && q_in.scalar_type() == at::kHalf && q_in.size(2) == 2 * k.size(3) && k.size(2) > 0,
               "libpad_b200 decode_fp4: q must be fp16 [B, Hq, D] of the cache's head_dim");
   TORCH_CHECK(bt_in.dim() == 2 && bt_in.size(0) == q_in.size(0) && sl_in.dim() == 1 && sl_in.size(0) == q_in.size(0),
               "libpad_b200 decode_fp4: block_table must be [B, max_pages], seq_lens [B]");
