@@ -110,6 +110,70 @@ def test_weights_and_positions_match_float64(seqs, hkv, g, d, ps, num_splits):
 
 
 @gpu
+@pytest.mark.parametrize("tracked", [False, True])
+def test_more_sequences_than_the_kernel_caches_lengths_of(tracked):
+    _need_cuda()
+    rng = np.random.default_rng(12)
+    seqs = rng.integers(0, 90, 1300).tolist()
+    seqs[0] = seqs[511] = seqs[512] = seqs[-1] = 0
+    q, caches, k, v, bt, sl = fp4_case(seqs, 1, 2, 32, 16, seed=12)
+    ref, probs = co.decode(q, k, v, bt, sl)
+    w = torch.zeros(k.shape[0], 1, 16, device="cuda") if tracked else None
+    out = pad_b200.paged_attention_decode_fp4(_cuda(q, torch.float16), *map(_cuda, caches), _cuda(bt), _cuda(sl),
+                                              weights=w, num_new=100)
+    assert_parity(out.float().cpu().numpy(), ref)
+    if tracked:
+        check_weights(w.cpu().numpy(), co.accumulate(np.zeros(tuple(w.shape)), probs, bt, sl, 100),
+                      rel_bound(32, 90, smax_of(q, k, 32)))
+
+
+@gpu
+@pytest.mark.parametrize("d,ps", [(128, 1), (128, 5), (64, 16), (32, 48)])
+def test_k_and_v_of_different_strides(d, ps):
+    _need_cuda()
+    q, caches, k, v, bt, sl = fp4_case([77, 300, 16], 3, 5, d, ps, seed=13)
+    kc, ks, vc, vs = [_cuda(c) for c in caches]
+    vc = _cuda(caches[2].transpose(0, 2, 1, 3)).permute(0, 2, 1, 3)  # V's pages head-major
+    wide = torch.zeros(*vs.shape[:2], vs.shape[2] + 2, 4, dtype=torch.uint8, device="cuda")
+    wide[:, :, : vs.shape[2]] = vs
+    ref, _ = co.decode(q, k, v, bt, sl)
+    out = pad_b200.paged_attention_decode_fp4(_cuda(q, torch.float16), kc, ks, vc, wide[:, :, : vs.shape[2]], _cuda(bt),
+                                              _cuda(sl))
+    assert_parity(out.float().cpu().numpy(), ref)
+
+
+@gpu
+def test_values_are_checked_when_asked_for(monkeypatch):
+    """PAD_B200_CHECK: flags become the errors of the other entry points."""
+    _need_cuda()
+    from pad_b200 import kernel_cuda_v4
+
+    monkeypatch.setattr(kernel_cuda_v4, "_CHECK_VALUES", True)
+    caches = pad_b200.paged_kv_cache_fp4(4, 16, 2, 64)
+    k16 = torch.zeros(4, 16, 2, 64, dtype=torch.float16, device="cuda")
+    q, new = torch.zeros(1, 4, 64, dtype=torch.float16, device="cuda"), torch.zeros(1, 2, 64, dtype=torch.float16, device="cuda")
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    good, bad, w = i32([0, 1]), i32([0, 9]), torch.zeros(4, 2, 16, device="cuda")
+    one, far = i32(20), i32(33)
+    for call in (lambda bt, n: pad_b200.paged_attention_decode_fp4(q, *caches, bt, n),
+                 lambda bt, n: pad_b200.paged_attention_decode_weights(q, k16, k16, bt, n, w),
+                 lambda bt, n: pad_b200.paged_kv_evict_plan(w, bt, n, 4),
+                 lambda bt, n: pad_b200.paged_kv_append_fp4(new, new, *caches, bt, n),
+                 lambda bt, n: pad_b200.paged_kv_read_fp4(*caches, bt, n)):
+        call(good, one)
+        with pytest.raises(ValueError, match="page id"):
+            call(bad, one)
+        with pytest.raises(ValueError, match="seq_lens"):
+            call(good, far)
+    with pytest.raises(ValueError, match="seq_ids"):
+        pad_b200.paged_kv_append_fp4(new, new, *caches, good, one, i32(1))
+    many = torch.arange(4, dtype=torch.int32, device="cuda").repeat(40, 40)
+    with pytest.raises(ValueError, match="share pages"):
+        pad_b200.paged_attention_decode_fp4(q.expand(40, 4, 64).contiguous(), *caches, many,
+                                            torch.full((40,), 640, dtype=torch.int32, device="cuda"), weights=w)
+
+
+@gpu
 def test_long_context_and_wide_table():
     _need_cuda()
     q, caches, k, v, bt, sl = fp4_case([70001, 50], 2, 6, 128, 32, seed=3)

@@ -100,6 +100,21 @@ def test_weights_and_positions_match_float64(seqs, hkv, g, d, ps, num_splits):
 
 
 @gpu
+def test_more_sequences_than_the_kernel_caches_lengths_of():
+    _need_cuda()
+    rng = np.random.default_rng(13)
+    seqs = rng.integers(0, 40, 1500).tolist()
+    c = explicit_case(seqs, num_kv_heads=1, gqa_ratio=2, head_dim=16, page_size=8, seed=13)
+    ref, probs = co.decode(c.q, c.k_cache, c.v_cache, c.block_table, c.seq_lens)
+    q, k, v, bt, sl = _case_inputs(c)
+    w = torch.zeros(k.shape[0], 1, 8, device="cuda")
+    out = pad_b200.paged_attention_decode_weights(q, k, v, bt, sl, w, num_new=40)
+    assert_parity(out.float().cpu().numpy(), ref)
+    check_weights(w.cpu().numpy(), co.accumulate(np.zeros(tuple(w.shape)), probs, c.block_table, c.seq_lens, 40),
+                  rel_bound(16, 40, smax_of(c.q, c.k_cache, 16)))
+
+
+@gpu
 def test_out_is_the_decode_without_weights_bit_for_bit():
     _need_cuda()
     c = explicit_case([3000, 17, 900], num_kv_heads=2, gqa_ratio=6, head_dim=128, page_size=16, seed=3)

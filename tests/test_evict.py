@@ -140,7 +140,9 @@ PLAN_CASES = [
     ([777, 2000], 300, 0, 24, 5, "odd", None),
     ([2000, 60, 1999], 512, 100, 16, 2, "equal", 4096),      # a table far wider than the sequences (clusters)
     ([8192, 8193, 16385], 4096, 128, 16, 1, "tail", None),   # up to a cluster of 4
+    ([9000, 3], 8990, 2, 8, 2, "odd", None),                 # a cluster of 2
     ([70001], 9999, 200, 64, 2, "ties", None),               # a cluster of 8
+    ([70000, 69999], 1, 0, 16, 1, "equal", None),
     ([450000], 100000, 0, 64, 1, "odd", None),               # more keys than the cluster's shared memory
 ]
 
@@ -175,9 +177,13 @@ def test_plan_strides_and_repeatability():
     wt = _cuda(w.transpose(2, 0, 1)).permute(1, 2, 0)  # row-major last
     btw = torch.zeros(2, bt.shape[1] + 5, dtype=torch.int32, device="cuda")
     btw[:, : bt.shape[1]] = _cuda(bt)
-    ss, dd, _ = co.evict_plan(w, bt, lens, 100)
+    at = rng.integers(0, 400, (pages, hkv, ps)).astype(np.int32)
+    atw = torch.zeros(pages, 2 * hkv, ps, dtype=torch.int32, device="cuda")
+    atw[:, ::2] = _cuda(at)  # every other head of a wider array
+    ss, dd, _ = co.evict_plan(w, bt, lens, 100, 30, at, lens)
     for _ in range(3):
-        got = pad_b200.paged_kv_evict_plan(wt, btw[:, : bt.shape[1]], _cuda(np.array(lens, np.int32)), 100)
+        got = pad_b200.paged_kv_evict_plan(wt, btw[:, : bt.shape[1]], _cuda(np.array(lens, np.int32)), 100, 30,
+                                           slot_positions=atw[:, ::2])
         assert _plan_lists(*got[:3]) == (ss, dd)
 
 
