@@ -21,7 +21,7 @@
 //
 // Bound: plan -- 8 bytes a slot would take 5 us for 4 x 8 x 118 thousand slots;
 // its instructions (a gather, three histogram passes and two votes a slot) and the
-// exchanges in the cluster take 53 us. 64 x 2 x 2080 slots: 9 us, the latency of
+// exchanges in the cluster take 41 us. 64 x 2 x 2080 slots: 8 us, the latency of
 // the same chain. Move -- HBM bytes, 2 x row bytes a move: 131 thousand fp16 rows
 // of 256 + 256 bytes in 33 us (62% of the copy rate); a 4-bit row's 4-byte scales,
 // weight and position each cost a 32-byte sector both ways, so its 39% of the copy
@@ -61,6 +61,7 @@ struct PlanParams {
   int64_t bt_stride;
   int hkv, num_pages, page_size, page_shift, max_pages, budget, recent, max_moves;
   int key_cap;  // keys of shared memory per CTA
+  int quads;    // four neighbouring slots of a page are 16 aligned bytes
   int32_t* error_flags;
 };
 
@@ -184,7 +185,7 @@ __device__ __forceinline__ int warp_base(PlanShared& sh, int mine, int* total) {
 
 template <int RANKS, bool CACHED>
 __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __grid_constant__ PlanParams p) {
-  extern __shared__ uint32_t keys[];
+  extern __shared__ __align__(16) uint32_t keys[];
   __shared__ __align__(16) PlanShared sh;
   const int rank = RANKS == 1 ? 0 : (int)cg::this_cluster().block_rank();
   const int pair = (int)(blockIdx.x / RANKS), b = pair / p.hkv, h = pair % p.hkv;
@@ -198,7 +199,7 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
   int32_t* dst = p.dst + (int64_t)pair * p.max_moves;
   int count = 0;
   if (n > p.budget) {
-    const int share = (n + RANKS - 1) / RANKS;
+    const int share = ((n + RANKS - 1) / RANKS + 3) / 4 * 4;  // whole quads of slots
     const int first = min(n, rank * share), last = min(n, first + share);
     const SlotKeys<CACHED> key{p,
                                keys,
@@ -212,7 +213,49 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
     __syncthreads();
     // keys into shared memory, their top digit counted on the way
     bool bad = false;
-    for (int s0 = first; s0 < last; s0 += kPlanThreads * kGather) {
+    const bool quads = CACHED && p.quads;
+    // four neighbouring slots a load (4 x 8 x 118 thousand slots: 52.8 -> 41.3 us)
+    constexpr int UQ = kGather / 4;
+    for (int s0 = quads ? first : last; s0 < last; s0 += kPlanThreads * 4 * UQ) {
+      int page[UQ], row[UQ];
+      float4 w[UQ];
+      int4 at[UQ];
+#pragma unroll
+      for (int u = 0; u < UQ; ++u) {
+        const int s = s0 + (u * kPlanThreads + tid) * 4, lp = key.page_slot(s);
+        row[u] = s - lp * p.page_size;
+        page[u] = s < last ? __ldg(key.ids + lp) : -1;
+      }
+#pragma unroll
+      for (int u = 0; u < UQ; ++u) {
+        const bool ok = (unsigned)page[u] < (unsigned)p.num_pages;
+        bad |= !ok && s0 + (u * kPlanThreads + tid) * 4 < last;
+        w[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        at[u] = make_int4(0, 0, 0, 0);
+        if (ok) {
+          w[u] = __ldg(reinterpret_cast<const float4*>(key.weight_at(page[u], row[u])));
+          if (key.positions != nullptr) at[u] = __ldg(reinterpret_cast<const int4*>(key.position_at(page[u], row[u])));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < UQ; ++u) {
+        const int s = s0 + (u * kPlanThreads + tid) * 4;
+        if (s >= last) continue;
+        uint32_t k[4] = {0u, 0u, 0u, 0u};
+        if ((unsigned)page[u] < (unsigned)p.num_pages) {
+          k[0] = key.key(w[u].x, at[u].x);
+          k[1] = key.key(w[u].y, at[u].y);
+          k[2] = key.key(w[u].z, at[u].z);
+          k[3] = key.key(w[u].w, at[u].w);
+        }
+        *reinterpret_cast<uint4*>(keys + (s - first)) = make_uint4(k[0], k[1], k[2], k[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (s + j < last) atomicAdd(&sh.hist[0][k[j] >> 21], 1);
+      }
+    }
+    // or one
+    for (int s0 = quads ? last : first; s0 < last; s0 += kPlanThreads * kGather) {
       int page[kGather], row[kGather], at[kGather];
       float w[kGather];
 #pragma unroll
@@ -249,11 +292,22 @@ __global__ void __launch_bounds__(kPlanThreads, 2) evict_plan_kernel(const __gri
 #pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
       if (pass > 0) {
-#pragma unroll 4
-        for (int s = first + tid; s < last; s += kPlanThreads) {
-          const uint32_t k = key.at(s);
+        auto count = [&](uint32_t k) {
           if (pass == 1 ? (k >> 21) == prefix : (k >> 10) == prefix)
             atomicAdd(&sh.hist[pass][pass == 1 ? (k >> 10) & 2047u : k & 1023u], 1);
+        };
+        if constexpr (CACHED) {
+#pragma unroll 2
+          for (int s = first + tid * 4; s < last; s += kPlanThreads * 4) {
+            const uint4 k = *reinterpret_cast<const uint4*>(keys + (s - first));
+            count(k.x);
+            if (s + 1 < last) count(k.y);
+            if (s + 2 < last) count(k.z);
+            if (s + 3 < last) count(k.w);
+          }
+        } else {
+#pragma unroll 4
+          for (int s = first + tid; s < last; s += kPlanThreads) count(key.at(s));
         }
       }
       rank_sync<RANKS>();
@@ -540,6 +594,11 @@ extern "C" int pad_paged_kv_evict_plan(const float* weights, const int32_t* slot
   p.page_size = (int)page_size;
   p.page_shift = shift_of(page_size);
   p.max_pages = (int)max_pages_per_seq;
+  auto quads = [&](const void* x, const int64_t* st4) {
+    return st4[2] == 1 && st4[0] % 4 == 0 && st4[1] % 4 == 0 && reinterpret_cast<uintptr_t>(x) % 16 == 0;
+  };
+  p.quads = page_size % 4 == 0 && weight_strides != nullptr && quads(weights, weight_strides) &&
+            (p.slot_positions == nullptr || quads(slot_positions, position_strides));
   p.budget = (int)std::min<int64_t>(budget, INT32_MAX);
   p.recent = (int)std::min<int64_t>(recent, INT32_MAX);
   p.max_moves = (int)moves;
