@@ -398,9 +398,14 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> kv_evict_plan(
   const at::Tensor total = total_in.has_value() ? as_int32_rows(*total_in, dev) : at::Tensor();
   int64_t moves = 0;
   check(pad_evict_max_moves(budget, ps, bt.size(1), &moves), "kv_evict_plan");
+  // one allocation for the plan, each part starting on 16 bytes; the lengths, which
+  // a caller keeps, have their own
+  const int64_t list = batch * hkv * moves, step = (list + 3) / 4 * 4;
   const auto opt = weights.options().dtype(at::kInt);
-  at::Tensor src = at::empty({batch, hkv, moves}, opt), dst = at::empty({batch, hkv, moves}, opt);
-  at::Tensor counts = at::empty({batch, hkv}, opt), lens = at::empty({batch}, opt);
+  const at::Tensor all = at::empty({2 * step + batch * hkv}, opt), lens = at::empty({batch}, opt);
+  const at::Tensor src = all.as_strided({batch, hkv, moves}, {hkv * moves, moves, 1}, 0);
+  const at::Tensor dst = all.as_strided({batch, hkv, moves}, {hkv * moves, moves, 1}, step);
+  const at::Tensor counts = all.as_strided({batch, hkv}, {hkv, 1}, 2 * step);
   cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   StreamState& st = state_for(dev, stream);
   const Strides ws(weights), pst(positions.has_value() ? *positions : weights);

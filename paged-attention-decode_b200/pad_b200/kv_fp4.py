@@ -94,7 +94,7 @@ def paged_attention_decode_fp4(
     are those of paged_attention_decode_weights (weights=None: not tracked)."""
     assert q.is_cuda and k_cache.is_cuda and v_cache.is_cuda, "pad_b200 requires CUDA tensors"
     assert q.dtype == torch.float16 and q.dim() == 3, "pad_b200 expects fp16 q [B, Hq, D]"
-    batch, num_q_heads, head_dim = q.shape
+    _, num_q_heads, head_dim = q.shape
     assert head_dim in FP4_HEAD_DIMS, f"head_dim must be one of {FP4_HEAD_DIMS}"
     assert num_q_heads % k_cache.shape[2] == 0, "num_q_heads must be divisible by num_kv_heads (GQA)"
     assert num_splits is None or num_splits >= 1, "num_splits must be >= 1"
