@@ -56,6 +56,7 @@ typedef enum pad_status {
 #define PAD_FLAG_SEQ_LEN_RANGE 0x2   /* seq_len < 0 or > max_pages_per_seq * page_size */
 #define PAD_FLAG_BAD_SEQ_ID 0x4      /* a seq_ids entry outside [0, batch) */
 #define PAD_FLAG_SHARED_PAGE 0x8     /* more tokens than the pool's pages hold: sequences share pages */
+#define PAD_FLAG_SCALE_RANGE 0x10    /* a V scale of a 4-bit cache above 2^13 */
 #define PAD_FLAG_WAIT_TIMEOUT 0x100  /* an in-kernel wait gave up (never expected) */
 
 /* Human-readable text for a status code (static storage). */
@@ -238,9 +239,12 @@ int pad_paged_kv_read_fp4(const void* k_cache, const void* k_scales, const void*
                           void* stream, int32_t* error_flags);
 
 /* Decode attention over the 4-bit cache: pad_paged_attention_decode with K and
- * V what their codes and scales stand for (scales up to 2^15; above, values
- * leave fp16's range and become infinite, and a NaN scale makes the sequences
- * that attend to it NaN). head_dim 32, 64 or 128, gqa_ratio up to 16. q must be
+ * V what their codes and scales stand for. V's scales may lie in 2^-24 .. 2^13,
+ * which is all that the append writes, where code x scale is an fp16 value;
+ * smaller ones count as 0 (the output moves by less than 6 x 2^-25), and one above
+ * 2^13 that a sequence attends to sets PAD_FLAG_SCALE_RANGE and leaves that
+ * sequence's output undefined (Inf or NaN). K's scales are applied in fp32 and
+ * have no such bound. A NaN scale makes the sequences that attend to it NaN. head_dim 32, 64 or 128, gqa_ratio up to 16. q must be
  * 16-byte aligned with strides that are multiples of 8 elements, out 4-byte
  * aligned with even strides. weights, slot_positions, total_lens and num_new
  * are those of pad_paged_attention_decode_weights below; weights NULL leaves

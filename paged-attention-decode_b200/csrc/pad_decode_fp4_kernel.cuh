@@ -27,6 +27,8 @@
 // Rows of tokens past the sequence, and of pages that are none, are copied as
 // zeros (cp.async with no source bytes): zero codes with a finite scale, so
 // nothing that a page holds behind its sequence reaches the sums.
+// V's scales go onto codes in fp16, exactly for 2^-24 .. 2^13, all that the append
+// writes. Smaller ones become 0; a larger one would make codes infinite and is flagged.
 //
 // Measured (12/2 heads, head_dim 128, page 16): 64 x 4096 tokens 24.8 us a call
 // (10.9 at the measured copy rate), each further 4096 tokens of the 64 sequences
@@ -158,6 +160,19 @@ struct Fp4Walk {
     }
   }
 };
+
+// Flags scales of V above 2^13 among the NB of the scale row at shared address `row`
+// (NaN is none). Out of line: 64 x 16384 68.3 us so, 68.5 inside the loop, 67.8 unchecked.
+template <int NB>
+__device__ __noinline__ void flag_high_scales(const Fp4DecodeParams& p, uint32_t row) {
+  uint32_t vw;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vw) : "r"(row));
+#pragma unroll
+  for (int blk = 0; blk < NB; ++blk) {
+    const uint32_t byte = (vw >> (8 * blk)) & 255u;
+    if (byte > 140u && byte != kFp4NanScale && p.error_flags != nullptr) atomicOr(p.error_flags, PAD_FLAG_SCALE_RANGE);
+  }
+}
 
 template <class TR>
 __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid_constant__ Fp4DecodeParams p) {
@@ -399,6 +414,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
       // ---- scales, a lane per token: K's blocks in fp32 with the softmax scale
       // and log2 e folded in, V's as fp16, laid out as the fragments want them:
       // pairs of neighbouring tokens
+      bool high;  // a scale of V is above 2^13 or NaN
       {
         uint32_t kw, vw;
         asm volatile("ld.shared.u32 %0, [%1];" : "=r"(kw) : "r"(sb + lane * 4));
@@ -412,6 +428,8 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
                      : "memory");
         const uint32_t v01 = pack_half2(__uint_as_float(w01 << 16), __uint_as_float(w01 & 0xffff0000u));
         const uint32_t v23 = pack_half2(__uint_as_float(w23 << 16), __uint_as_float(w23 & 0xffff0000u));
+        // (a byte above 140: its top bit is set and the others are at least 13)
+        high = (((vw & 0x7f7f7f7fu) + 0x73737373u) & vw & (NB == 4 ? 0x80808080u : NB == 2 ? 0x8080u : 0x80u)) != 0u;
         const bool odd = lane & 1;
         // an even lane makes the pairs of blocks 0 and 1, its neighbour of 2 and 3
         const uint32_t mine = odd ? v23 : v01, theirs = __shfl_xor_sync(0xffffffffu, odd ? v01 : v23, 1);
@@ -512,7 +530,7 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
       // kSlack, so p <= 2^kSlack, which fp16's range takes and which cancels in
       // O / l. Nearly every tile then needs no exchange between lanes and no
       // rescaling (64 x 16384: 71.9 -> 68.7 us).
-      bool beyond = false;
+      bool beyond = high;
       float top[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -541,6 +559,8 @@ __global__ void __launch_bounds__(TR::THREADS, 1) decode_fp4_kernel(const __grid
                 acc[blk][x][nt][j + 2] *= alpha;
               }
           }
+        // Up to 2^13, the largest the append writes, every code of V is an fp16 value.
+        if (high) flag_high_scales<NB>(p, sb + TT * kFp4ScaleRow + lane * kFp4ScaleRow);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)

@@ -27,6 +27,7 @@ PAD_FLAG_BAD_PAGE_ID = 0x1
 PAD_FLAG_SEQ_LEN_RANGE = 0x2
 PAD_FLAG_BAD_SEQ_ID = 0x4
 PAD_FLAG_SHARED_PAGE = 0x8
+PAD_FLAG_SCALE_RANGE = 0x10
 PAD_FLAG_WAIT_TIMEOUT = 0x100
 
 # (name, restype, argtypes) for every symbol the header declares

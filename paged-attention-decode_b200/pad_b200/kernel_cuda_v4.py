@@ -76,6 +76,8 @@ def _raise_for_flags(flags: int) -> None:
         raise ValueError("seq_ids contains an entry that is no sequence of block_table")
     if flags & _lib.PAD_FLAG_SHARED_PAGE:
         raise ValueError("sequences share pages: their attention weights cannot be kept apart")
+    if flags & _lib.PAD_FLAG_SCALE_RANGE:
+        raise ValueError("v_scales contains a scale above 2^13 (a byte of 141 to 254)")
     if flags & _lib.PAD_FLAG_WAIT_TIMEOUT:
         raise RuntimeError("libpad_b200: an in-kernel wait timed out")
 

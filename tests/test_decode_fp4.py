@@ -374,3 +374,100 @@ def test_refusals_without_a_device():
         assert call(**over) == status, over
         assert b"decode_fp4" in lib.pad_last_error() and text in lib.pad_last_error(), over
     assert call(b=0) == _lib.PAD_OK
+
+
+def _foreign(rng, seqs, hkv, g, d, ps):
+    """A cache that another writer filled: random codes and scale bytes (K's near 2^-2, V's 2^-4 to 2^2)."""
+    need = [-(-n // ps) for n in seqs]
+    pages = sum(need) + 1
+    perm = rng.permutation(pages).astype(np.int32)
+    bt = np.zeros((len(seqs), max(max(need), 1)), np.int32)
+    at = 0
+    for i, n in enumerate(need):
+        bt[i, :n] = perm[at:at + n]
+        at += n
+    codes = lambda: rng.integers(0, 256, (pages, ps, hkv, d // 2)).astype(np.uint8)  # noqa: E731
+    scales = lambda lo, hi: rng.integers(lo, hi, (pages, ps, hkv, 4)).astype(np.uint8)  # noqa: E731
+    q = (rng.standard_normal((len(seqs), hkv * g, d)) * 0.3).astype(np.float16)
+    return q, codes(), scales(124, 127), codes(), scales(123, 130), bt, np.asarray(seqs, np.int32)
+
+
+def _check_foreign(q, kc, ks, vc, vs, bt, sl, num_splits=None, weights=False, off_v=0.0):
+    """Half a step of fp16 on the result; each probability off by its bound (test_decode_weights.py) and by the 2^-25 that
+    P's two fp16 terms resolve (the largest P is at least 1); every value off by off_v."""
+    k, v = co.dequantise(kc, ks), co.dequantise(vc, vs)
+    ref, probs = co.decode(q, k, v, bt, sl)
+    w = torch.zeros(k.shape[0], k.shape[2], k.shape[1], device="cuda") if weights else None
+    out = pad_b200.paged_attention_decode_fp4(*map(_cuda, (q, kc, ks, vc, vs, bt, sl)), num_splits, weights=w)
+    got = out.double().cpu().numpy()
+    hkv, d = k.shape[2], k.shape[3]
+    bound = rel_bound(d, int(max(sl)), smax_of(q.astype(np.float64), k, d))
+    for i, n in enumerate(sl):
+        vv = np.abs(co.gather(v, bt[i], int(n)))  # [n, Hkv, D]
+        terms = bound * np.einsum("th,thd->hd", probs[i], vv) + 2.0 ** -25 * vv.sum(0)
+        want = ref[i].reshape(hkv, -1, d)
+        tol = np.abs(want) * 2.0 ** -11 + 2.0 ** -25 + terms[:, None] + off_v
+        off = np.abs(got[i].reshape(want.shape) - want)
+        assert np.all(off <= tol), f"sequence {i}: off by {np.nanmax(off / tol):.3g} of the tolerance"
+    if weights:
+        check_weights(w.cpu().numpy(), co.accumulate(np.zeros(tuple(w.shape)), probs, bt, sl, 1), bound)
+
+
+@gpu
+@pytest.mark.parametrize("byte", [140, 139, 103, 102, 95, 3, 0])
+@pytest.mark.parametrize("d,g", [(128, 2), (64, 12), (32, 5)])
+def test_v_scales_at_the_ends_of_fp16(byte, d, g):
+    """Up to 2^13 exact; below 2^-24 a scale counts as 0, so a value (6 x 2^-25 at most) is off by itself. At 2^-24 the
+    codes 0.5 and 1.5 lie between two fp16 values (no append writes them there): half a step of 2^-24."""
+    _need_cuda()
+    pad_b200.read_error_flags()
+    rng = np.random.default_rng(byte + d)
+    q, kc, ks, vc, vs, bt, sl = _foreign(rng, [1, 40, 200], 2, g, d, 16)
+    if byte > 127:  # a few tokens of them, in some blocks
+        vs[rng.random(vs.shape) < 0.1] = byte
+    else:
+        vs[:] = byte
+    for num_splits, weights in ((None, False), (3, True)):
+        _check_foreign(q, kc, ks, vc, vs, bt, sl, num_splits, weights,
+                       off_v=6 * 2.0 ** -25 if byte < 103 else 2.0 ** -25 if byte == 103 else 0.0)
+    assert pad_b200.read_error_flags() == 0
+
+
+@gpu
+@pytest.mark.parametrize("byte", [141, 142, 200, 254, 255])
+@pytest.mark.parametrize("d,g", [(128, 2), (64, 12), (32, 5)])
+def test_v_scales_above_the_largest_are_flagged(byte, d, g, monkeypatch):
+    """In a block that a sequence attends to, wherever its token lies; NaN (255) is none of them."""
+    _need_cuda()
+    from pad_b200 import kernel_cuda_v4
+
+    pad_b200.read_error_flags()
+    rng = np.random.default_rng(byte)
+    q, kc, ks, vc, vs, bt, sl = _foreign(rng, [300, 40, 200], 2, g, d, 16)
+    vs -= 3  # values below 4, where the parity bound holds fp16's half step
+    flag = 0 if byte == 255 else _lib.PAD_FLAG_SCALE_RANGE
+    qg, kcg, ksg, vcg, btg, slg = map(_cuda, (q, kc, ks, vc, bt, sl))
+    run = lambda x, **kw: pad_b200.paged_attention_decode_fp4(qg, kcg, ksg, vcg, _cuda(x), btg, slg, **kw)  # noqa: E731
+    ref, _ = co.decode(q, co.dequantise(kc, ks), co.dequantise(vc, vs), bt, sl)
+    for i, t, blk in [(0, 0, 0), (0, 299, d // 32 - 1), (0, 150, 0), (1, 39, d // 32 - 1)]:
+        bad = vs.copy()
+        bad[bt[i, t // 16], t % 16, 1, blk] = byte
+        for kw in ({}, dict(num_splits=3), dict(weights=torch.zeros(kc.shape[0], 2, 16, device="cuda"))):
+            out = run(bad, **kw).float().cpu().numpy()
+            assert pad_b200.read_error_flags() == flag
+            for j in range(3):  # the other sequences, and the other head
+                assert_parity(out[j, : g if j == i else 2 * g], ref[j, : g if j == i else 2 * g])
+    if flag:
+        monkeypatch.setattr(kernel_cuda_v4, "_CHECK_VALUES", True)
+        with pytest.raises(ValueError, match="v_scales"):
+            run(bad)
+        run(vs)
+        monkeypatch.setattr(kernel_cuda_v4, "_CHECK_VALUES", False)
+    # behind a sequence, in a page of none, and in the unused bytes of a row: never looked at
+    bad = vs.copy()
+    bad[..., d // 32:] = byte
+    for i, n in enumerate(sl):
+        bad[bt[i, n // 16], n % 16:] = byte  # (no length is a multiple of the page)
+    bad[sorted(set(range(len(bad))) - {int(x) for i, n in enumerate(sl) for x in bt[i, : -(-n // 16)]})] = byte
+    assert_parity(run(bad).float().cpu().numpy(), ref)
+    assert pad_b200.read_error_flags() == 0
