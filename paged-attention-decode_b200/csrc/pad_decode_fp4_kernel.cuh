@@ -37,6 +37,7 @@
 // cycles and the integer pipe, which also converts, is busy in 51%.
 #pragma once
 
+#include <cfloat>
 #include <climits>
 
 #include "pad_b200.h"
@@ -69,9 +70,9 @@ struct Fp4DecodeParams {
   TrackParams track;
 };
 
-// Where a running maximum starts: below every score, and finite, so that a
+// Where a running maximum starts: at or below every score, and finite, so that a
 // difference to it is never NaN.
-constexpr float kLeastScore = -1e30f;
+constexpr float kLeastScore = -FLT_MAX;
 // How far (in log2 units) a score may pass the reference point before it moves.
 constexpr float kSlack = 8.f;
 

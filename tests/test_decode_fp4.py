@@ -471,3 +471,27 @@ def test_v_scales_above_the_largest_are_flagged(byte, d, g, monkeypatch):
     bad[sorted(set(range(len(bad))) - {int(x) for i, n in enumerate(sl) for x in bt[i, : -(-n // 16)]})] = byte
     assert_parity(run(bad).float().cpu().numpy(), ref)
     assert pad_b200.read_error_flags() == 0
+
+
+@gpu
+@pytest.mark.parametrize("n", [1, 100])
+@pytest.mark.parametrize("num_splits", [None, 3])
+def test_scores_far_below_zero(n, num_splits):
+    """Every score below -1e31: the largest of them still takes all."""
+    _need_cuda()
+    caches = pad_b200.paged_kv_cache_fp4(7, 16, 1, 64)
+    caches[0].fill_(0xFF)  # keys of -6 ...
+    caches[0][(n - 1) // 16, (n - 1) % 16] = 0x99  # ... and, in the last token, of -0.5
+    caches[1].fill_(127)
+    gen = torch.Generator(device="cuda")
+    gen.manual_seed(5)
+    v = torch.randint(0, 256, caches[2].shape, device="cuda", generator=gen).to(torch.uint8)
+    caches[2].copy_(v), caches[3].fill_(127)
+    q = torch.ones(1, 2, 64, dtype=torch.float16, device="cuda")
+    bt, sl = torch.arange(7, dtype=torch.int32, device="cuda").view(1, 7), torch.tensor([n], dtype=torch.int32, device="cuda")
+    w = torch.zeros(7, 1, 16, device="cuda")
+    out = pad_b200.paged_attention_decode_fp4(q, *caches, bt, sl, num_splits, scale=1e32, weights=w, num_new=10 ** 6)
+    want = co.dequantise(caches[2].cpu().numpy(), caches[3].cpu().numpy())[(n - 1) // 16, (n - 1) % 16, 0]
+    np.testing.assert_array_equal(out[0].double().cpu().numpy(), np.stack([want, want]))
+    got = w[:, 0].flatten()
+    assert got[n - 1].item() == 2.0 and got.sum().item() == 2.0
