@@ -259,9 +259,11 @@ int fill(Fp4Params* p, const char* what, const void* k_rows, const void* v_rows,
          int64_t tokens, int64_t batch, int64_t num_kv_heads, int64_t head_dim, int64_t num_pages, int64_t page_size,
          int64_t max_pages, const int64_t* kr, const int64_t* vr, const int64_t* k, const int64_t* ks,
          const int64_t* v, const int64_t* vs, int64_t bt_stride, int32_t* error_flags) {
-  if (k_rows == nullptr || v_rows == nullptr || k_cache == nullptr || k_scales == nullptr || v_cache == nullptr ||
-      v_scales == nullptr || block_table == nullptr || positions == nullptr || kr == nullptr || vr == nullptr ||
-      k == nullptr || ks == nullptr || v == nullptr || vs == nullptr)
+  // a pool or a table of nothing has no address: its tokens are flagged before one is needed
+  if (k_rows == nullptr || v_rows == nullptr || positions == nullptr ||
+      (num_pages > 0 && (k_cache == nullptr || k_scales == nullptr || v_cache == nullptr || v_scales == nullptr)) ||
+      (batch > 0 && max_pages > 0 && block_table == nullptr) || kr == nullptr || vr == nullptr || k == nullptr ||
+      ks == nullptr || v == nullptr || vs == nullptr)
     return fail(PAD_ERR_INVALID_ARGUMENT, "%s: null pointer argument", what);
   if (seq_ids == nullptr && tokens > batch)
     return fail(PAD_ERR_INVALID_ARGUMENT, "%s: %lld tokens for %lld sequences need seq_ids", what, (long long)tokens,
@@ -348,7 +350,7 @@ extern "C" int pad_paged_kv_append_fp4(const void* k_new, const void* v_new, voi
                                        const int64_t* ks_strides, const int64_t* v_strides, const int64_t* vs_strides,
                                        int64_t block_table_stride, void* stream, int32_t* error_flags) {
   int st = check_sizes("kv_append_fp4", tokens, batch, num_kv_heads, head_dim, num_pages, page_size, max_pages_per_seq);
-  if (st != PAD_OK || tokens == 0 || batch == 0 || num_pages == 0 || max_pages_per_seq == 0) return st;
+  if (st != PAD_OK || tokens == 0) return st;
   Fp4Params p = {};
   st = fill(&p, "kv_append_fp4", k_new, v_new, k_cache, k_scales, v_cache, v_scales, block_table, positions, seq_ids,
             tokens, batch, num_kv_heads, head_dim, num_pages, page_size, max_pages_per_seq, k_new_strides,

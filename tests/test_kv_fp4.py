@@ -289,3 +289,28 @@ def test_append_and_read_in_a_graph_on_another_stream():
         torch.cuda.synchronize()
         np.testing.assert_array_equal(ko.cpu().numpy().astype(np.float64), co.dequantise(*co.quantise(x[0])))
         np.testing.assert_array_equal(vo.cpu().numpy().astype(np.float64), co.dequantise(*co.quantise(x[1])))
+
+
+@gpu
+def test_a_pool_or_a_table_of_nothing():
+    """Tokens that cannot have a place are flagged, as in any other pool; they read as zeros."""
+    _need_cuda()
+    pad_b200.read_error_flags()
+    k = torch.ones(2, 2, 64, dtype=torch.float16, device="cuda")
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    none, some = pad_b200.paged_kv_cache_fp4(0, 16, 2, 64), pad_b200.paged_kv_cache_fp4(3, 16, 2, 64)
+    table = torch.zeros(2, 4, dtype=torch.int32, device="cuda")
+    for caches, bt, flag in [(none, table, _lib.PAD_FLAG_BAD_PAGE_ID), (some, table[:, :0], _lib.PAD_FLAG_SEQ_LEN_RANGE),
+                             (none, table[:, :0], _lib.PAD_FLAG_SEQ_LEN_RANGE)]:
+        for pos, ids, want in [(i32(3, 0), None, flag), (i32(-1, -1), None, 0), (i32(0, 0), i32(1, 1), flag)]:
+            pad_b200.paged_kv_append_fp4(k, k, *caches, bt, pos, ids)
+            assert pad_b200.read_error_flags() == want
+            for got in pad_b200.paged_kv_read_fp4(*caches, bt, pos, ids):
+                assert got.shape == (2, 2, 64) and got.eq(0).all()
+            assert pad_b200.read_error_flags() == want
+    nobody = table[:0]
+    pad_b200.paged_kv_append_fp4(k, k, *some, nobody, i32(0, 0), i32(0, 0))
+    assert pad_b200.read_error_flags() == _lib.PAD_FLAG_BAD_SEQ_ID
+    assert pad_b200.paged_kv_read_fp4(*some, nobody, i32(0, 0), i32(0, 0))[0].eq(0).all()
+    assert pad_b200.read_error_flags() == _lib.PAD_FLAG_BAD_SEQ_ID
+    assert all(c.eq(0).all() for c in some)
