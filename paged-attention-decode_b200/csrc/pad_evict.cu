@@ -553,14 +553,15 @@ extern "C" int pad_paged_kv_evict_plan(const float* weights, const int32_t* slot
   if (budget < 1) return fail(PAD_ERR_INVALID_ARGUMENT, "evict_plan: budget must be at least 1");
   if (recent < 0 || recent > budget)
     return fail(PAD_ERR_INVALID_ARGUMENT, "evict_plan: recent must lie in [0, budget]");
-  if (recent > 0 && slot_positions == nullptr)
+  // (a pool of nothing has no address: no slot of it is read)
+  if (recent > 0 && slot_positions == nullptr && num_pages > 0)
     return fail(PAD_ERR_INVALID_ARGUMENT, "evict_plan: recent needs slot_positions");
   if (batch == 0) return PAD_OK;
   int64_t moves = 0;
   if ((st = pad_evict_max_moves(budget, page_size, max_pages_per_seq, &moves)) != PAD_OK) return st;
   if (seq_lens == nullptr || counts == nullptr || new_lens == nullptr ||
-      (moves > 0 && (weights == nullptr || block_table == nullptr || src == nullptr || dst == nullptr ||
-                     weight_strides == nullptr)) ||
+      (moves > 0 && ((weights == nullptr && num_pages > 0) || block_table == nullptr || src == nullptr ||
+                     dst == nullptr || weight_strides == nullptr)) ||
       (slot_positions != nullptr && (total_lens == nullptr || position_strides == nullptr)))
     return fail(PAD_ERR_INVALID_ARGUMENT, "evict_plan: null pointer argument");
   const int64_t cap = max_pages_per_seq * page_size, pairs = batch * num_kv_heads;

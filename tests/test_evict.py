@@ -311,3 +311,20 @@ def test_evict_in_a_graph_replayed_on_new_contents():
         assert new.tolist() == want.tolist()
         np.testing.assert_array_equal(cache.cpu().numpy(), co.apply_moves(cn, bt, ss, dd))
         np.testing.assert_array_equal(w.cpu().numpy(), co.apply_moves(wn, bt, ss, dd, 1))
+
+
+@gpu
+def test_plan_and_evict_of_an_empty_pool():
+    _need_cuda()
+    pad_b200.read_error_flags()
+    w, at = torch.zeros(0, 2, 16, device="cuda"), torch.zeros(0, 2, 16, dtype=torch.int32, device="cuda")
+    bt, sl = torch.zeros(3, 4, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+    for kw in ({}, dict(recent=2, slot_positions=at, total_lens=sl)):
+        src, dst, counts, lens = pad_b200.paged_kv_evict_plan(w, bt, sl, 8, **kw)
+        assert src.eq(-1).all() and dst.eq(-1).all() and counts.eq(0).all() and lens.eq(0).all()
+        cache = torch.zeros(0, 16, 2, 64, dtype=torch.float16, device="cuda")
+        assert pad_b200.paged_kv_evict([cache], w, bt, sl, 8, **kw).eq(0).all()
+    assert pad_b200.read_error_flags() == 0
+    # sequences that claim slots of a pool without pages are flagged
+    src, dst, counts, lens = pad_b200.paged_kv_evict_plan(w, bt, sl + 40, 8)
+    assert pad_b200.read_error_flags() == _lib.PAD_FLAG_BAD_PAGE_ID and lens.eq(8).all()
