@@ -265,6 +265,15 @@ int pad_paged_attention_decode_fp4(const void* q, const void* k_cache, const voi
                                    const int64_t* out_strides, const int64_t* weight_strides,
                                    const int64_t* position_strides, float scale, int64_t num_splits, void* workspace,
                                    size_t workspace_bytes, void* stream, int32_t* error_flags);
+int pad_paged_attention_decode_fp4_by_seq(
+    const void* q, const void* k_cache, const void* k_scales, const void* v_cache, const void* v_scales,
+    const int32_t* block_table, const int32_t* seq_lens, void* out, float* weights, int32_t* slot_positions,
+    const int32_t* total_lens, const int32_t* num_new, int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+    int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages_per_seq, const int64_t* q_strides,
+    const int64_t* k_strides, const int64_t* ks_strides, const int64_t* v_strides, const int64_t* vs_strides,
+    int64_t block_table_stride, const int64_t* out_strides, const int64_t* weight_strides,
+    const int64_t* position_strides, float scale, int64_t num_splits, void* workspace, size_t workspace_bytes,
+    void* stream, int32_t* error_flags);
 
 /* ---------------------------------------------------------------------------
  * Eviction by accumulated attention weight. Beside a paged cache live
@@ -279,7 +288,11 @@ int pad_paged_attention_decode_fp4(const void* q, const void* k_cache, const voi
  *   weights = (t >= seq_lens[b] - num_new ? 0 : weights) + the softmax
  *             probabilities of the token, summed over the KV head's query heads
  * so that slots of the num_new newest tokens need no clearing; with
- * slot_positions these slots also get total_lens[b] - seq_lens[b] + t. The
+ * slot_positions these slots also get total_lens[b] - seq_lens[b] + t. num_new is
+ * one number for all sequences, or, with pad_paged_attention_decode_weights_by_seq
+ * (and pad_paged_attention_decode_fp4_by_seq), a device array [batch] int32 of
+ * each one's, for batches that a sequence joins with its prompt; a negative entry
+ * counts as 0. The
  * workspace (pad_decode_weights_workspace_bytes) also holds the call's scores,
  * 4 bytes per query head and token that the batch can hold: of min(batch *
  * max_pages_per_seq, num_pages) pages. Sequences that share pages lose weight
@@ -317,6 +330,14 @@ int pad_paged_attention_decode_weights(const void* q, const void* k_cache, const
                                        const int64_t* out_strides, const int64_t* weight_strides,
                                        const int64_t* position_strides, float scale, int64_t num_splits,
                                        void* workspace, size_t workspace_bytes, void* stream, int32_t* error_flags);
+int pad_paged_attention_decode_weights_by_seq(
+    const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* seq_lens,
+    void* out, float* weights, int32_t* slot_positions, const int32_t* total_lens, const int32_t* num_new,
+    int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t num_pages, int64_t page_size,
+    int64_t max_pages_per_seq, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+    int64_t block_table_stride, const int64_t* out_strides, const int64_t* weight_strides,
+    const int64_t* position_strides, float scale, int64_t num_splits, void* workspace, size_t workspace_bytes,
+    void* stream, int32_t* error_flags);
 int pad_evict_max_moves(int64_t budget, int64_t page_size, int64_t max_pages_per_seq, int64_t* max_moves);
 int pad_paged_kv_evict_plan(const float* weights, const int32_t* slot_positions, const int32_t* block_table,
                             const int32_t* seq_lens, const int32_t* total_lens, int32_t* src, int32_t* dst,

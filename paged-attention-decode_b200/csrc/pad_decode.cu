@@ -410,6 +410,7 @@ struct WeightArgs {
   const int64_t* position_strides;
   const int32_t* total_lens;
   int64_t num_new;
+  const int32_t* num_new_of;  // of each sequence, instead of num_new
 };
 
 int check_weights(const WeightArgs& w) {
@@ -589,6 +590,7 @@ int decode_impl(const void* q, const void* k_cache, const void* v_cache, const i
     wp.track = prm.track;
     wp.block_table = block_table;
     wp.total_lens = wa->total_lens;
+    wp.num_new_of = wa->num_new_of;
     wp.weights = wa->weights;
     wp.slot_positions = wa->slot_positions;
     wp.w0 = wa->weight_strides[0];
@@ -677,7 +679,27 @@ int pad_paged_attention_decode_weights(const void* q, const void* k_cache, const
                                        const int64_t* out_strides, const int64_t* weight_strides,
                                        const int64_t* position_strides, float scale, int64_t num_splits,
                                        void* workspace, size_t workspace_bytes, void* stream, int32_t* error_flags) {
-  const WeightArgs wa{weights, weight_strides, slot_positions, position_strides, total_lens, num_new};
+  const WeightArgs wa{weights, weight_strides, slot_positions, position_strides, total_lens, num_new, nullptr};
+  if (batch > 0 && num_pages > 0 && max_pages_per_seq > 0) {
+    const int st = check_weights(wa);
+    if (st != PAD_OK) return st;
+  }
+  return decode_impl(q, k_cache, v_cache, block_table, seq_lens, nullptr, nullptr, out, batch, num_q_heads,
+                     num_kv_heads, head_dim, num_pages, page_size, max_pages_per_seq, q_strides, k_strides, v_strides,
+                     block_table_stride, out_strides, scale, num_splits, workspace, workspace_bytes, stream,
+                     error_flags, false, &wa);
+}
+
+int pad_paged_attention_decode_weights_by_seq(
+    const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table, const int32_t* seq_lens,
+    void* out, float* weights, int32_t* slot_positions, const int32_t* total_lens, const int32_t* num_new,
+    int64_t batch, int64_t num_q_heads, int64_t num_kv_heads, int64_t head_dim, int64_t num_pages, int64_t page_size,
+    int64_t max_pages_per_seq, const int64_t* q_strides, const int64_t* k_strides, const int64_t* v_strides,
+    int64_t block_table_stride, const int64_t* out_strides, const int64_t* weight_strides,
+    const int64_t* position_strides, float scale, int64_t num_splits, void* workspace, size_t workspace_bytes,
+    void* stream, int32_t* error_flags) {
+  const WeightArgs wa{weights, weight_strides, slot_positions, position_strides, total_lens, 0, num_new};
+  if (batch > 0 && num_new == nullptr) return fail(PAD_ERR_INVALID_ARGUMENT, "null num_new");
   if (batch > 0 && num_pages > 0 && max_pages_per_seq > 0) {
     const int st = check_weights(wa);
     if (st != PAD_OK) return st;

@@ -117,24 +117,11 @@ bool offsets_fit(const int64_t* s, int64_t pages, int64_t ps, int64_t hkv, int u
   return pages == 0 || last / unit < 4294967296.0;
 }
 
-}  // namespace
-
-extern "C" int pad_decode_fp4_workspace_bytes(int device, int64_t batch, int64_t num_kv_heads, int64_t gqa_ratio,
-                                              int64_t head_dim, int64_t num_pages, int64_t page_size,
-                                              int64_t max_pages_per_seq, int64_t num_splits, int with_weights,
-                                              size_t* bytes) {
-  if (bytes == nullptr) return fail(PAD_ERR_INVALID_ARGUMENT, "decode_fp4: null output pointer");
-  Fp4Plan plan;
-  const int st = make_plan(device, batch, num_kv_heads, gqa_ratio, head_dim, num_pages, page_size, max_pages_per_seq,
-                           num_splits, with_weights != 0, &plan);
-  if (st == PAD_OK) *bytes = plan.bytes;
-  return st;
-}
-
-extern "C" int pad_paged_attention_decode_fp4(
+// num_new_of: new tokens of each sequence, or null: num_new of every one.
+int decode_fp4(
     const void* q, const void* k_cache, const void* k_scales, const void* v_cache, const void* v_scales,
     const int32_t* block_table, const int32_t* seq_lens, void* out, float* weights, int32_t* slot_positions,
-    const int32_t* total_lens, int64_t num_new, int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+    const int32_t* total_lens, int64_t num_new, const int32_t* num_new_of, int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
     int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages_per_seq, const int64_t* q_strides,
     const int64_t* k_strides, const int64_t* ks_strides, const int64_t* v_strides, const int64_t* vs_strides,
     int64_t block_table_stride, const int64_t* out_strides, const int64_t* weight_strides,
@@ -304,6 +291,7 @@ extern "C" int pad_paged_attention_decode_fp4(
     wp.track = p.track;
     wp.block_table = block_table;
     wp.total_lens = total_lens;
+    wp.num_new_of = num_new_of;
     wp.weights = weights;
     wp.slot_positions = slot_positions;
     wp.w0 = weight_strides[0];
@@ -328,4 +316,51 @@ extern "C" int pad_paged_attention_decode_fp4(
     if ((st = launch_weights(wp, s)) != PAD_OK) return st;
   }
   return PAD_OK;
+}
+
+}  // namespace
+
+extern "C" int pad_decode_fp4_workspace_bytes(int device, int64_t batch, int64_t num_kv_heads, int64_t gqa_ratio,
+                                              int64_t head_dim, int64_t num_pages, int64_t page_size,
+                                              int64_t max_pages_per_seq, int64_t num_splits, int with_weights,
+                                              size_t* bytes) {
+  if (bytes == nullptr) return fail(PAD_ERR_INVALID_ARGUMENT, "decode_fp4: null output pointer");
+  Fp4Plan plan;
+  const int st = make_plan(device, batch, num_kv_heads, gqa_ratio, head_dim, num_pages, page_size, max_pages_per_seq,
+                           num_splits, with_weights != 0, &plan);
+  if (st == PAD_OK) *bytes = plan.bytes;
+  return st;
+}
+
+extern "C" int pad_paged_attention_decode_fp4(
+    const void* q, const void* k_cache, const void* k_scales, const void* v_cache, const void* v_scales,
+    const int32_t* block_table, const int32_t* seq_lens, void* out, float* weights, int32_t* slot_positions,
+    const int32_t* total_lens, int64_t num_new, int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+    int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages_per_seq, const int64_t* q_strides,
+    const int64_t* k_strides, const int64_t* ks_strides, const int64_t* v_strides, const int64_t* vs_strides,
+    int64_t block_table_stride, const int64_t* out_strides, const int64_t* weight_strides,
+    const int64_t* position_strides, float scale, int64_t num_splits, void* workspace, size_t workspace_bytes,
+    void* stream, int32_t* error_flags) {
+  return decode_fp4(q, k_cache, k_scales, v_cache, v_scales, block_table, seq_lens, out, weights, slot_positions,
+                    total_lens, num_new, nullptr, batch, num_q_heads, num_kv_heads, head_dim, num_pages, page_size,
+                    max_pages_per_seq, q_strides, k_strides, ks_strides, v_strides, vs_strides, block_table_stride,
+                    out_strides, weight_strides, position_strides, scale, num_splits, workspace, workspace_bytes,
+                    stream, error_flags);
+}
+
+extern "C" int pad_paged_attention_decode_fp4_by_seq(
+    const void* q, const void* k_cache, const void* k_scales, const void* v_cache, const void* v_scales,
+    const int32_t* block_table, const int32_t* seq_lens, void* out, float* weights, int32_t* slot_positions,
+    const int32_t* total_lens, const int32_t* num_new, int64_t batch, int64_t num_q_heads, int64_t num_kv_heads,
+    int64_t head_dim, int64_t num_pages, int64_t page_size, int64_t max_pages_per_seq, const int64_t* q_strides,
+    const int64_t* k_strides, const int64_t* ks_strides, const int64_t* v_strides, const int64_t* vs_strides,
+    int64_t block_table_stride, const int64_t* out_strides, const int64_t* weight_strides,
+    const int64_t* position_strides, float scale, int64_t num_splits, void* workspace, size_t workspace_bytes,
+    void* stream, int32_t* error_flags) {
+  if (batch > 0 && num_new == nullptr) return fail(PAD_ERR_INVALID_ARGUMENT, "decode_fp4: null num_new");
+  return decode_fp4(q, k_cache, k_scales, v_cache, v_scales, block_table, seq_lens, out, weights, slot_positions,
+                    total_lens, 0, num_new, batch, num_q_heads, num_kv_heads, head_dim, num_pages, page_size,
+                    max_pages_per_seq, q_strides, k_strides, ks_strides, v_strides, vs_strides, block_table_stride,
+                    out_strides, weight_strides, position_strides, scale, num_splits, workspace, workspace_bytes,
+                    stream, error_flags);
 }

@@ -275,11 +275,11 @@ void check_slots(const at::Tensor& t, at::ScalarType type, int64_t pages, int64_
 
 // What a decode with attention weights takes beside the decode's arguments.
 struct Tracked {
-  at::Tensor total;
+  at::Tensor total, num_new_of;
   Strides ws, ps;
   Tracked(const at::Tensor& weights, const c10::optional<at::Tensor>& positions,
-          const c10::optional<at::Tensor>& total_in, int64_t num_new, int64_t pages, int64_t hkv, int64_t page_size,
-          int64_t batch, const at::Device& dev, const char* what)
+          const c10::optional<at::Tensor>& total_in, int64_t num_new, const c10::optional<at::Tensor>& num_new_in,
+          int64_t pages, int64_t hkv, int64_t page_size, int64_t batch, const at::Device& dev, const char* what)
       : ws(weights), ps(positions.has_value() ? *positions : weights) {
     check_slots(weights, at::kFloat, pages, hkv, page_size, what);
     check_on(dev, {&weights}, what);
@@ -293,6 +293,12 @@ struct Tracked {
                   ": total_lens must be [B]");
       total = as_int32_rows(*total_in, dev);
     }
+    if (num_new_in.has_value()) {
+      const at::Tensor& n = *num_new_in;
+      TORCH_CHECK(n.dim() == 1 && n.size(0) == batch && at::isIntegralType(n.scalar_type(), false), "libpad_b200 ",
+                  what, ": num_new must be a number or an integer tensor [B]");
+      num_new_of = as_int32_rows(n.scalar_type() == at::kLong ? n.clamp(0, INT32_MAX) : n, dev);
+    }
   }
   const int32_t* total_ptr() const { return total.defined() ? total.data_ptr<int32_t>() : nullptr; }
 };
@@ -302,7 +308,8 @@ struct Tracked {
 at::Tensor decode_weights(const at::Tensor& q_in, const at::Tensor& k, const at::Tensor& v, const at::Tensor& bt_in,
                           const at::Tensor& sl_in, int64_t num_splits, double scale,
                           const c10::optional<at::Tensor>& out_in, const at::Tensor& weights, int64_t num_new,
-                          const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& total_in) {
+                          const c10::optional<at::Tensor>& positions, const c10::optional<at::Tensor>& total_in,
+                          const c10::optional<at::Tensor>& num_new_in) {
   TORCH_CHECK(q_in.dim() == 3 && k.dim() == 4 && v.sizes() == k.sizes() && k.size(2) > 0 && k.size(3) == q_in.size(2),
               "libpad_b200 decode_weights: bad q / k_cache / v_cache shapes");
   TORCH_CHECK(q_in.scalar_type() == at::kHalf && k.scalar_type() == at::kHalf && v.scalar_type() == at::kHalf,
@@ -314,7 +321,7 @@ at::Tensor decode_weights(const at::Tensor& q_in, const at::Tensor& k, const at:
   c10::cuda::CUDAGuard guard(dev);
   const int64_t batch = q_in.size(0), hq = q_in.size(1), d = q_in.size(2), pages = k.size(0), ps = k.size(1),
                 hkv = k.size(2);
-  const Tracked tr(weights, positions, total_in, num_new, pages, hkv, ps, batch, dev, "decode_weights");
+  const Tracked tr(weights, positions, total_in, num_new, num_new_in, pages, hkv, ps, batch, dev, "decode_weights");
   const at::Tensor q = aligned_rows(q_in);
   const at::Tensor bt = as_int32_rows(bt_in, dev), sl = as_int32_rows(sl_in, dev);
   at::Tensor out = prepare_out(out_in, q_in);
@@ -327,11 +334,16 @@ at::Tensor decode_weights(const at::Tensor& q_in, const at::Tensor& k, const at:
                                            num_splits, &bytes),
         "workspace size");
   const at::Tensor ws = at::empty({(int64_t)bytes}, st.flags.options().dtype(at::kByte));
-  check(pad_paged_attention_decode_weights(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), bt.data_ptr<int32_t>(), sl.data_ptr<int32_t>(), out.data_ptr(),
-            weights.data_ptr<float>(), positions.has_value() ? positions->data_ptr<int32_t>() : nullptr,
-            tr.total_ptr(), num_new, batch, hq, hkv, d, pages, ps, bt.size(1), qs.s, ks.s, vs.s, Strides(bt).s[0], os.s,
-            tr.ws.s, tr.ps.s, (float)scale, num_splits, ws.data_ptr(), bytes, stream, st.flags.data_ptr<int32_t>()),
+  auto call = [&](auto entry, auto news) {
+    return entry(q.data_ptr(), k.data_ptr(), v.data_ptr(), bt.data_ptr<int32_t>(), sl.data_ptr<int32_t>(),
+                 out.data_ptr(), weights.data_ptr<float>(),
+                 positions.has_value() ? positions->data_ptr<int32_t>() : nullptr, tr.total_ptr(), news, batch, hq, hkv,
+                 d, pages, ps, bt.size(1), qs.s, ks.s, vs.s, Strides(bt).s[0], os.s, tr.ws.s, tr.ps.s, (float)scale,
+                 num_splits, ws.data_ptr(), bytes, stream, st.flags.data_ptr<int32_t>());
+  };
+  check(tr.num_new_of.defined()
+            ? call(pad_paged_attention_decode_weights_by_seq, (const int32_t*)tr.num_new_of.data_ptr<int32_t>())
+            : call(pad_paged_attention_decode_weights, num_new),
         "decode_weights");
   return out;
 }
@@ -340,7 +352,7 @@ at::Tensor decode_fp4(const at::Tensor& q_in, const at::Tensor& k, const at::Ten
                       const at::Tensor& vs, const at::Tensor& bt_in, const at::Tensor& sl_in, int64_t num_splits,
                       double scale, const c10::optional<at::Tensor>& out_in, const c10::optional<at::Tensor>& weights,
                       int64_t num_new, const c10::optional<at::Tensor>& positions,
-                      const c10::optional<at::Tensor>& total_in) {
+                      const c10::optional<at::Tensor>& total_in, const c10::optional<at::Tensor>& num_new_in) {
   const at::Device dev = q_in.device();
   check_fp4(k, ks, v, vs, "decode_fp4");
   check_on(dev, {&k, &ks, &v, &vs}, "decode_fp4");
@@ -353,7 +365,8 @@ at::Tensor decode_fp4(const at::Tensor& q_in, const at::Tensor& k, const at::Ten
   const int64_t batch = q_in.size(0), hq = q_in.size(1), d = q_in.size(2), pages = k.size(0), ps = k.size(1),
                 hkv = k.size(2);
   c10::optional<Tracked> tr;
-  if (weights.has_value()) tr.emplace(*weights, positions, total_in, num_new, pages, hkv, ps, batch, dev, "decode_fp4");
+  if (weights.has_value())
+    tr.emplace(*weights, positions, total_in, num_new, num_new_in, pages, hkv, ps, batch, dev, "decode_fp4");
   const at::Tensor q = aligned_rows(q_in);
   const at::Tensor bt = as_int32_rows(bt_in, dev), sl = as_int32_rows(sl_in, dev);
   at::Tensor out = prepare_out(out_in, q_in);
@@ -366,13 +379,17 @@ at::Tensor decode_fp4(const at::Tensor& q_in, const at::Tensor& k, const at::Ten
                                        weights.has_value() ? 1 : 0, &bytes),
         "workspace size");
   const at::Tensor ws = at::empty({(int64_t)bytes}, k.options());
-  check(pad_paged_attention_decode_fp4(
-            q.data_ptr(), k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), bt.data_ptr<int32_t>(),
-            sl.data_ptr<int32_t>(), out.data_ptr(), tr ? weights->data_ptr<float>() : nullptr,
-            positions.has_value() ? positions->data_ptr<int32_t>() : nullptr, tr ? tr->total_ptr() : nullptr, num_new,
-            batch, hq, hkv, d, pages, ps, bt.size(1), qs.s, k_s.s, ks_s.s, v_s.s, vs_s.s, Strides(bt).s[0], os.s,
-            tr ? tr->ws.s : nullptr, tr ? tr->ps.s : nullptr, (float)scale, num_splits, ws.data_ptr(), bytes, stream,
-            st.flags.data_ptr<int32_t>()),
+  auto call = [&](auto entry, auto news) {
+    return entry(q.data_ptr(), k.data_ptr(), ks.data_ptr(), v.data_ptr(), vs.data_ptr(), bt.data_ptr<int32_t>(),
+                 sl.data_ptr<int32_t>(), out.data_ptr(), tr ? weights->data_ptr<float>() : nullptr,
+                 positions.has_value() ? positions->data_ptr<int32_t>() : nullptr, tr ? tr->total_ptr() : nullptr, news,
+                 batch, hq, hkv, d, pages, ps, bt.size(1), qs.s, k_s.s, ks_s.s, v_s.s, vs_s.s, Strides(bt).s[0], os.s,
+                 tr ? tr->ws.s : nullptr, tr ? tr->ps.s : nullptr, (float)scale, num_splits, ws.data_ptr(), bytes,
+                 stream, st.flags.data_ptr<int32_t>());
+  };
+  check(tr && tr->num_new_of.defined()
+            ? call(pad_paged_attention_decode_fp4_by_seq, (const int32_t*)tr->num_new_of.data_ptr<int32_t>())
+            : call(pad_paged_attention_decode_fp4, num_new),
         "decode_fp4");
   return out;
 }
@@ -488,10 +505,10 @@ TORCH_LIBRARY(pad_b200, m) {
         "Tensor positions) -> ()");
   m.def("decode_weights(Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor seq_lens, int num_splits, "
         "float scale, Tensor(a!)? out, Tensor(b!) weights, int num_new, Tensor(c!)? slot_positions, "
-        "Tensor? total_lens) -> Tensor");
+        "Tensor? total_lens, Tensor? num_new_of=None) -> Tensor");
   m.def("decode_fp4(Tensor q, Tensor k_cache, Tensor k_scales, Tensor v_cache, Tensor v_scales, Tensor block_table, "
         "Tensor seq_lens, int num_splits, float scale, Tensor(a!)? out, Tensor(b!)? weights, int num_new, "
-        "Tensor(c!)? slot_positions, Tensor? total_lens) -> Tensor");
+        "Tensor(c!)? slot_positions, Tensor? total_lens, Tensor? num_new_of=None) -> Tensor");
   m.def("kv_append_fp4(Tensor k_new, Tensor v_new, Tensor(a!) k_cache, Tensor(b!) k_scales, Tensor(c!) v_cache, "
         "Tensor(d!) v_scales, Tensor block_table, Tensor positions, Tensor? seq_ids) -> ()");
   m.def("kv_read_fp4(Tensor k_cache, Tensor k_scales, Tensor v_cache, Tensor v_scales, Tensor block_table, "

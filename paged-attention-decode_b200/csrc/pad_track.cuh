@@ -37,6 +37,7 @@ struct TrackParams {
 struct WeightParams {
   TrackParams track;
   const int32_t *block_table, *total_lens;
+  const int32_t* num_new_of;  // new tokens of each sequence, or null: num_new of every one
   float* weights;
   int32_t* slot_positions;
   int64_t w0, w1, w2, p0, p1, p2, bt_stride;

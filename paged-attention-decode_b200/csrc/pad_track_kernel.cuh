@@ -51,7 +51,8 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(const __grid_co
         row[j] = slot + j - lp * p.page_size;
       }
     }
-    const int h = (d.y << p.hg_log2) + hl, fresh = d.w - p.num_new - slot;  // tokens from `fresh` on are new
+    const int num_new = p.num_new_of != nullptr ? min(max(__ldg(p.num_new_of + d.x), 0), d.w) : p.num_new;
+    const int h = (d.y << p.hg_log2) + hl, fresh = d.w - num_new - slot;  // tokens from `fresh` on are new
     float* w[4];
     float was[4];
 #pragma unroll

@@ -54,11 +54,17 @@ SIGNATURES = {
     "pad_paged_attention_decode_fp4": (ctypes.c_int, [_vp] * 11 + [_c_i64] * 8
                                        + [_c_i64p] * 5 + [_c_i64] + [_c_i64p] * 3
                                        + [ctypes.c_float, _c_i64, _vp, ctypes.c_size_t, _vp, _vp]),
+    "pad_paged_attention_decode_fp4_by_seq": (ctypes.c_int, [_vp] * 12 + [_c_i64] * 7
+                                              + [_c_i64p] * 5 + [_c_i64] + [_c_i64p] * 3
+                                              + [ctypes.c_float, _c_i64, _vp, ctypes.c_size_t, _vp, _vp]),
     "pad_decode_weights_workspace_bytes": (ctypes.c_int, [ctypes.c_int] + [_c_i64] * 8
                                            + [ctypes.POINTER(ctypes.c_size_t)]),
     "pad_paged_attention_decode_weights": (ctypes.c_int, [_vp] * 9 + [_c_i64] * 8
                                            + [_c_i64p, _c_i64p, _c_i64p, _c_i64, _c_i64p, _c_i64p, _c_i64p,
                                               ctypes.c_float, _c_i64, _vp, ctypes.c_size_t, _vp, _vp]),
+    "pad_paged_attention_decode_weights_by_seq": (ctypes.c_int, [_vp] * 10 + [_c_i64] * 7
+                                                  + [_c_i64p, _c_i64p, _c_i64p, _c_i64, _c_i64p, _c_i64p, _c_i64p,
+                                                     ctypes.c_float, _c_i64, _vp, ctypes.c_size_t, _vp, _vp]),
     "pad_evict_max_moves": (ctypes.c_int, [_c_i64] * 3 + [_c_i64p]),
     "pad_paged_kv_evict_plan": (ctypes.c_int, [_vp] * 9 + [_c_i64] * 7 + [_c_i64p] * 2 + [_c_i64, _vp, _vp]),
     "pad_paged_kv_move": (ctypes.c_int, [_c_i64, ctypes.POINTER(_vp), _c_i64p, _c_i64p] + [_vp] * 6 + [_c_i64] * 6

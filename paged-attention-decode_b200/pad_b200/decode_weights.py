@@ -13,6 +13,14 @@ from .kernel_cuda_v4 import _SUPPORTED_HEAD_DIMS, _check_values, _raise_if_check
 _OPS = _lib.ops()
 
 
+def _new_tokens(num_new: int | torch.Tensor) -> tuple[int, torch.Tensor | None]:
+    """num_new as the operators take it: a number, or a tensor with one of each sequence."""
+    if isinstance(num_new, torch.Tensor):
+        return 0, num_new
+    assert num_new >= 0, "num_new must be >= 0"
+    return int(num_new), None
+
+
 def paged_attention_decode_weights(
     q: torch.Tensor,
     k_cache: torch.Tensor,
@@ -20,7 +28,7 @@ def paged_attention_decode_weights(
     block_table: torch.Tensor,
     seq_lens: torch.Tensor,
     weights: torch.Tensor,
-    num_new: int = 1,
+    num_new: int | torch.Tensor = 1,
     num_splits: int | None = None,
     scale: float | None = None,
     *,
@@ -34,7 +42,9 @@ def paged_attention_decode_weights(
     KV head, the token's softmax probability summed over the KV head's query
     heads. The num_new last tokens of each sequence are new: their weight is
     set, not added to, so a page's slots need no clearing before they are used
-    (num_new = 0 only adds). slot_positions [num_pages, Hkv, page_size] int32,
+    (num_new = 0 only adds). num_new is one number for every sequence or an
+    integer tensor [B], one of each: 1 for those that decode, the length of its
+    prompt for one that has just joined them. slot_positions [num_pages, Hkv, page_size] int32,
     if given, gets the new tokens' positions, counted from total_lens [B] (the
     tokens each sequence has seen; None: seq_lens, as before any eviction).
     Sequences must not share pages."""
@@ -48,13 +58,13 @@ def paged_attention_decode_weights(
     assert num_q_heads % k_cache.shape[2] == 0, "num_q_heads must be divisible by num_kv_heads (GQA)"
     assert head_dim in _SUPPORTED_HEAD_DIMS, f"head_dim must be one of {_SUPPORTED_HEAD_DIMS}"
     assert num_splits is None or num_splits >= 1, "num_splits must be >= 1"
-    assert num_new >= 0, "num_new must be >= 0"
+    num_new, num_new_of = _new_tokens(num_new)
     assert slot_positions is not None or total_lens is None, "total_lens goes with slot_positions"
     if slot_positions is not None and total_lens is None:
         total_lens = seq_lens
     _check_values(q.device)
     out = _OPS.decode_weights(q, k_cache, v_cache, block_table, seq_lens, 0 if num_splits is None else int(num_splits),
                               float(scale) if scale is not None else 1.0 / math.sqrt(head_dim), out, weights,
-                              int(num_new), slot_positions, total_lens)
+                              num_new, slot_positions, total_lens, num_new_of)
     _raise_if_checking(q.device)
     return out

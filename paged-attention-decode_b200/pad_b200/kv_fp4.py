@@ -19,6 +19,7 @@ import math
 import torch
 
 from . import _lib
+from .decode_weights import _new_tokens
 from .kernel_cuda_v4 import _check_values, _raise_if_checking
 
 _OPS = _lib.ops()
@@ -81,7 +82,7 @@ def paged_attention_decode_fp4(
     scale: float | None = None,
     *,
     weights: torch.Tensor | None = None,
-    num_new: int = 1,
+    num_new: int | torch.Tensor = 1,
     slot_positions: torch.Tensor | None = None,
     total_lens: torch.Tensor | None = None,
     out: torch.Tensor | None = None,
@@ -100,7 +101,7 @@ def paged_attention_decode_fp4(
     assert head_dim in FP4_HEAD_DIMS, f"head_dim must be one of {FP4_HEAD_DIMS}"
     assert num_q_heads % k_cache.shape[2] == 0, "num_q_heads must be divisible by num_kv_heads (GQA)"
     assert num_splits is None or num_splits >= 1, "num_splits must be >= 1"
-    assert num_new >= 0, "num_new must be >= 0"
+    num_new, num_new_of = _new_tokens(num_new)
     assert weights is not None or slot_positions is None, "slot_positions go with weights"
     assert slot_positions is not None or total_lens is None, "total_lens goes with slot_positions"
     if slot_positions is not None and total_lens is None:
@@ -108,7 +109,7 @@ def paged_attention_decode_fp4(
     _check_values(q.device)
     out = _OPS.decode_fp4(q, k_cache, k_scales, v_cache, v_scales, block_table, seq_lens,
                           0 if num_splits is None else int(num_splits),
-                          float(scale) if scale is not None else 1.0 / math.sqrt(head_dim), out, weights, int(num_new),
-                          slot_positions, total_lens)
+                          float(scale) if scale is not None else 1.0 / math.sqrt(head_dim), out, weights, num_new,
+                          slot_positions, total_lens, num_new_of)
     _raise_if_checking(q.device)
     return out

@@ -10,7 +10,7 @@ import torch
 import cache_oracle as co
 import pad_b200
 from gpu_utils import assert_parity
-from test_decode_weights import check_weights, rel_bound, smax_of
+from test_decode_weights import by_sequence, check_weights, rel_bound, smax_of
 
 gpu = pytest.mark.gpu
 
@@ -177,3 +177,82 @@ def test_without_eviction_the_weights_are_those_of_all_steps():
         # five additions round by 2^-24 each, on top of each probability's own bound
         assert np.all(np.abs(got - want[i, :, :n]) <= (rel_bound(64, 35, worst) + 5 * 2.0 ** -24) * want[i, :, :n] + 1e-7)
     assert lp.lens.cpu().tolist() == [35, 10]
+
+
+@gpu
+@pytest.mark.parametrize("fp4", [False, True])
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_sequence_joins_the_others_with_its_prompt(fp4, captured):
+    """Sequence 2 is empty for three steps, then has a prompt of 90 tokens on pages that others have used, and is
+    evicted by the weights and positions of this step's decode; the others add one token a step all along."""
+    _need_cuda()
+    pad_b200.read_error_flags()
+    lp = Loop(fp4, [70, 33, 0], budget=64, recent=4, seed=9)
+    bt = lp.bt.cpu().numpy()
+    k, v, q = lp.rand(3, lp.hkv, lp.d), lp.rand(3, lp.hkv, lp.d), lp.rand(3, lp.hkv * lp.g, lp.d)
+    news = torch.zeros(3, dtype=torch.int32, device="cuda")
+    q.copy_(lp.rand(*q.shape))
+    lp.decode(q, 10 ** 6)  # the first prompts' weights and positions
+    graph = None
+    for step in range(6):
+        if step == 3:  # the prompt, all but its last token, which this step appends
+            pk, pv = lp.rand(89, lp.hkv, lp.d), lp.rand(89, lp.hkv, lp.d)
+            pos = torch.arange(89, dtype=torch.int32, device="cuda")
+            if fp4:
+                pad_b200.paged_kv_append_fp4(pk, pv, *lp.caches, lp.bt, pos, torch.full_like(pos, 2))
+            else:
+                page, row = lp.bt[2, pos.long() // lp.ps].long(), pos.long() % lp.ps
+                lp.caches[0][page, row], lp.caches[1][page, row] = pk, pv
+            lp.lens[2] = lp.total[2] = 89
+        live = [0, 1] if step < 3 else [0, 1, 2]
+        news.copy_(torch.tensor([1, 1, 0 if step < 3 else 90 if step == 3 else 1]))
+        k.copy_(lp.rand(*k.shape)), v.copy_(lp.rand(*v.shape)), q.copy_(lp.rand(*q.shape))
+        f, kw = (pad_b200.paged_attention_decode_fp4, dict(weights=lp.w)) if fp4 else (pad_b200.paged_attention_decode_weights, {})
+
+        def decode():
+            args = (q, *lp.caches, lp.bt, lp.lens) + (() if fp4 else (lp.w,))
+            return f(*args, num_new=news, slot_positions=lp.at, total_lens=lp.total, **kw)
+
+        lens = lp.lens.clone()
+        lens[2] = -1 if step < 3 else lens[2]  # (a position below 0 appends nothing)
+        (pad_b200.paged_kv_append_fp4 if fp4 else pad_b200.paged_kv_append)(k, v, *lp.caches, lp.bt, lens)
+        lp.lens[live] += 1
+        lp.total[live] += 1
+        w0, at0 = lp.w.cpu().numpy(), lp.at.cpu().numpy()
+        if not captured:
+            out = decode()
+            lp.evict_lens = pad_b200.paged_kv_evict_plan(lp.w, lp.bt, lp.lens, lp.budget, lp.recent, slot_positions=lp.at,
+                                                         total_lens=lp.total)
+        else:
+            if graph is None:
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    out = decode()
+                    lp.evict_lens = pad_b200.paged_kv_evict_plan(lp.w, lp.bt, lp.lens, lp.budget, lp.recent,
+                                                                 slot_positions=lp.at, total_lens=lp.total)
+            graph.replay()
+        torch.cuda.synchronize()
+        seqs, total = lp.lens.tolist(), lp.total.cpu().numpy()
+        kk, vv = lp.values()
+        ref, probs = co.decode(q.cpu().numpy(), kk, vv, bt, seqs)
+        assert_parity(out.float().cpu().numpy(), ref, f"step {step}")
+        w1, at1 = lp.w.cpu().numpy(), lp.at.cpu().numpy()
+        want_w, want_at = by_sequence(w0, at0, probs, bt, seqs, total, news.tolist())
+        check_weights(w1, want_w, rel_bound(lp.d, max(seqs), smax_of(q.cpu().numpy().astype(np.float64), kk, lp.d)))
+        np.testing.assert_array_equal(at1, want_at)
+        src, dst, counts, new = lp.evict_lens
+        ss, dd, want_new = co.evict_plan(w1, bt, seqs, lp.budget, lp.recent, at1, total)
+        assert new.tolist() == want_new.tolist()
+        for (i, h), x in ss.items():
+            n = int(counts[i, h])
+            assert src[i, h, :n].tolist() == x and dst[i, h, :n].tolist() == dd[i, h]
+        pad_b200.paged_kv_move(lp.caches, lp.bt, src, dst, counts, weights=lp.w, slot_positions=lp.at)
+        lp.lens.copy_(new)
+        if step == 3:  # the newcomer keeps its own last tokens
+            at2 = lp.at.cpu().numpy()
+            t = np.arange(64)
+            for h in range(lp.hkv):
+                assert {86, 87, 88, 89} <= set(at2[bt[2, t // lp.ps], h, t % lp.ps].tolist())
+    assert lp.lens.tolist() == [64, 39, 64]
+    assert pad_b200.read_error_flags() == 0

@@ -15,7 +15,7 @@ import pad_b200
 from gpu_utils import assert_parity
 from pad_b200 import _lib
 from pad_b200.cases import explicit_case
-from test_decode_weights import check_weights, rel_bound, smax_of
+from test_decode_weights import NEWS, by_sequence, check_weights, rel_bound, smax_of
 
 gpu = pytest.mark.gpu
 
@@ -495,3 +495,39 @@ def test_scores_far_below_zero(n, num_splits):
     np.testing.assert_array_equal(out[0].double().cpu().numpy(), np.stack([want, want]))
     got = w[:, 0].flatten()
     assert got[n - 1].item() == 2.0 and got.sum().item() == 2.0
+
+
+@gpu
+@pytest.mark.parametrize("hkv,g,d,ps", [(2, 6, 128, 16), (3, 12, 32, 7)])
+@pytest.mark.parametrize("num_splits", [None, 3])
+def test_new_tokens_of_each_sequence(hkv, g, d, ps, num_splits):
+    _need_cuda()
+    seqs = [0, 1, 17, 300, 4000, 65, 64]
+    q, caches, k, v, bt, sl = fp4_case(seqs, hkv, g, d, ps, seed=22)
+    rng = np.random.default_rng(22)
+    w0 = rng.random((k.shape[0], hkv, ps)).astype(np.float32)
+    at0 = rng.integers(0, 99, w0.shape).astype(np.int32)
+    total = np.asarray(seqs, np.int64) + 7
+    ref, probs = co.decode(q, k, v, bt, sl)
+    want_w, want_at = by_sequence(w0, at0, probs, bt, seqs, total, NEWS)
+    w, at = _cuda(w0), _cuda(at0)
+    out = pad_b200.paged_attention_decode_fp4(_cuda(q, torch.float16), *map(_cuda, caches), _cuda(bt), _cuda(sl),
+                                              num_splits, weights=w, num_new=torch.tensor(NEWS, device="cuda"),
+                                              slot_positions=at, total_lens=_cuda(total))
+    assert_parity(out.float().cpu().numpy(), ref)
+    check_weights(w.cpu().numpy(), want_w, rel_bound(d, 4000, smax_of(q, k, d)))
+    np.testing.assert_array_equal(at.cpu().numpy(), want_at)
+    with pytest.raises(RuntimeError, match="num_new"):
+        pad_b200.paged_attention_decode_fp4(_cuda(q, torch.float16), *map(_cuda, caches), _cuda(bt), _cuda(sl),
+                                            weights=w, num_new=torch.ones(6, dtype=torch.int32, device="cuda"))
+
+
+def test_new_tokens_by_sequence_refusals_without_a_device():
+    lib, p, a = _lib.load(), 1 << 20, _lib.i64_array
+    call = lambda new, b, hq=12: lib.pad_paged_attention_decode_fp4_by_seq(  # noqa: E731
+        p, p, p, p, p, p, p, p, p, 0, 0, new, b, hq, 2, 128, 10, 16, 4, a([1536, 128, 1]), a([2048, 128, 64, 1]),
+        a([128, 8, 4, 1]), a([2048, 128, 64, 1]), a([128, 8, 4, 1]), 4, a([1536, 128, 1]), a([32, 16, 1]), None, 0.1, 0,
+        0, 0, 0, 0)
+    for new, hq, text in [(0, 12, b"num_new"), (p, 11, b"divisible")]:
+        assert call(new, 2, hq) == _lib.PAD_ERR_INVALID_ARGUMENT and text in lib.pad_last_error()
+    assert call(0, 0) == _lib.PAD_OK

@@ -310,3 +310,70 @@ def test_wrong_weights_are_refused():
         pad_b200.paged_attention_decode_weights(q, k, k, bt, sl, w, num_new=-1)
     with pytest.raises(AssertionError):
         pad_b200.paged_attention_decode_weights(q, k, k, bt, sl, w, total_lens=sl)
+
+
+NEWS = [1, 10 ** 6, 0, 7, 1, -3, 65]  # one of each of the sequences [0, 1, 17, 300, 4000, 65, 64]
+
+
+def by_sequence(w0, at0, probs, bt, seqs, total, news):
+    """weights and slot_positions after a step with a number of new tokens for each sequence."""
+    w, at, ps = w0.astype(np.float64), at0.copy(), w0.shape[2]
+    for i, n in enumerate(seqs):
+        new = min(max(news[i], 0), n)
+        w = co.accumulate(w, [probs[i]], bt[i:i + 1], seqs[i:i + 1], new)
+        for t in range(n - new, n):
+            at[bt[i, t // ps], :, t % ps] = total[i] - n + t
+    return w, at
+
+
+@gpu
+@pytest.mark.parametrize("hkv,g,d,ps", [(2, 6, 128, 16), (3, 12, 16, 7)])
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64, torch.int16])
+def test_new_tokens_of_each_sequence(hkv, g, d, ps, dtype):
+    _need_cuda()
+    seqs = [0, 1, 17, 300, 4000, 65, 64]
+    c = explicit_case(seqs, num_kv_heads=hkv, gqa_ratio=g, head_dim=d, page_size=ps, seed=21)
+    rng = np.random.default_rng(21)
+    w0 = rng.random((c.k_cache.shape[0], hkv, ps)).astype(np.float32)
+    at0 = rng.integers(0, 99, w0.shape).astype(np.int32)
+    total = np.asarray(seqs, np.int64) + 7
+    ref, probs = co.decode(c.q, c.k_cache, c.v_cache, c.block_table, c.seq_lens)
+    want_w, want_at = by_sequence(w0, at0, probs, c.block_table, seqs, total, NEWS)
+    q, k, v, bt, sl = _case_inputs(c)
+    news = torch.tensor([min(n, torch.iinfo(dtype).max) for n in NEWS], dtype=dtype, device="cuda")
+    if dtype == torch.int64:
+        news[1] = 2 ** 40  # past 32 bits: all of the sequence
+    w, at = _cuda(w0), _cuda(at0)
+    out = pad_b200.paged_attention_decode_weights(q, k, v, bt, sl, w, news, slot_positions=at, total_lens=_cuda(total))
+    assert_parity(out.float().cpu().numpy(), ref)
+    check_weights(w.cpu().numpy(), want_w, rel_bound(d, 4000, smax_of(c.q, c.k_cache, d)))
+    np.testing.assert_array_equal(at.cpu().numpy(), want_at)
+
+
+@gpu
+def test_wrong_numbers_of_new_tokens_are_refused():
+    _need_cuda()
+    q = torch.zeros(2, 4, 64, dtype=torch.float16, device="cuda")
+    k = torch.zeros(4, 16, 2, 64, dtype=torch.float16, device="cuda")
+    bt, sl = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda")
+    w = torch.zeros(4, 2, 16, device="cuda")
+    for bad in (sl[:1], sl.float(), sl.view(2, 1), sl.bool()):
+        with pytest.raises(RuntimeError, match="num_new"):
+            pad_b200.paged_attention_decode_weights(q, k, k, bt, sl, w, bad)
+
+
+def test_new_tokens_by_sequence_refusals_without_a_device():
+    lib, p, a = _lib.load(), 1 << 20, _lib.i64_array
+
+    def call(**over):
+        kw = dict(w=p, new=p, b=2, hq=12)
+        kw.update(over)
+        return lib.pad_paged_attention_decode_weights_by_seq(
+            p, p, p, p, p, p, kw["w"], 0, 0, kw["new"], kw["b"], kw["hq"], 2, 128, 10, 16, 4, a([1536, 128, 1]),
+            a([4096, 256, 128, 1]), a([4096, 256, 128, 1]), 4, a([1536, 128, 1]), a([32, 16, 1]), None, 0.088, 0, 0, 0,
+            0, 0)
+
+    for over, text in [(dict(new=0), b"num_new"), (dict(w=0), b"weights"), (dict(hq=11), b"divisible")]:
+        assert call(**over) == _lib.PAD_ERR_INVALID_ARGUMENT, over
+        assert text in lib.pad_last_error()
+    assert call(b=0, new=0) == _lib.PAD_OK
