@@ -295,9 +295,11 @@ int pad_paged_attention_decode_fp4_by_seq(
  * counts as 0. The
  * workspace (pad_decode_weights_workspace_bytes) also holds the call's scores,
  * 4 bytes per query head and token that the batch can hold: of min(batch *
- * max_pages_per_seq, num_pages) pages. Sequences that share pages lose weight
- * (no atomics: results are repeatable); PAD_FLAG_SHARED_PAGE is set when they
- * hold more tokens than the pool.
+ * max_pages_per_seq, num_pages) pages. Each weight has one writer, so results
+ * are repeatable. Sequences that share pages break that: their weights lose
+ * additions, other ones from run to run, and a move of one overwrites rows of the
+ * other. PAD_FLAG_SHARED_PAGE is set only when they hold more tokens than the
+ * pool; the Python calls refuse any shared page with PAD_B200_CHECK=1.
  *
  * pad_paged_kv_evict_plan chooses, for every sequence b with seq_lens[b] >
  * budget and every KV head, the `budget` slots to keep: first those that are

@@ -8,7 +8,7 @@ import math
 import torch
 
 from . import _lib
-from .kernel_cuda_v4 import _SUPPORTED_HEAD_DIMS, _check_values, _raise_if_checking
+from .kernel_cuda_v4 import _SUPPORTED_HEAD_DIMS, _check_own_pages, _check_values, _raise_if_checking
 
 _OPS = _lib.ops()
 
@@ -47,7 +47,8 @@ def paged_attention_decode_weights(
     prompt for one that has just joined them. slot_positions [num_pages, Hkv, page_size] int32,
     if given, gets the new tokens' positions, counted from total_lens [B] (the
     tokens each sequence has seen; None: seq_lens, as before any eviction).
-    Sequences must not share pages."""
+    Sequences must not share pages (their weights would lose additions, other
+    ones from run to run; refused with PAD_B200_CHECK=1)."""
     assert q.is_cuda and k_cache.is_cuda and v_cache.is_cuda, "pad_b200 requires CUDA tensors"
     assert q.dtype == torch.float16 and k_cache.dtype == torch.float16 and v_cache.dtype == torch.float16, (
         "pad_b200 expects fp16 q/k_cache/v_cache"
@@ -63,6 +64,7 @@ def paged_attention_decode_weights(
     if slot_positions is not None and total_lens is None:
         total_lens = seq_lens
     _check_values(q.device)
+    _check_own_pages(block_table, seq_lens, k_cache.shape[1])
     out = _OPS.decode_weights(q, k_cache, v_cache, block_table, seq_lens, 0 if num_splits is None else int(num_splits),
                               float(scale) if scale is not None else 1.0 / math.sqrt(head_dim), out, weights,
                               num_new, slot_positions, total_lens, num_new_of)

@@ -14,8 +14,8 @@ from typing import Sequence
 
 import torch
 
-from . import _lib
-from .kernel_cuda_v4 import _check_values, _raise_if_checking
+from . import _lib, kernel_cuda_v4
+from .kernel_cuda_v4 import _check_own_pages, _check_values, _raise_if_checking
 
 _OPS = _lib.ops()
 
@@ -33,7 +33,9 @@ def paged_kv_evict_plan(weights: torch.Tensor, block_table: torch.Tensor, seq_le
     new_lens): move i < counts[b, h] copies slot src[b, h, i] to dst[b, h, i]
     (both ascending, -1 behind the last), and new_lens = min(seq_lens, budget).
     Slots keep their place unless they lie at or above the budget, so their
-    order says nothing about age afterwards; attention does not depend on it."""
+    order says nothing about age afterwards; attention does not depend on it.
+    Sequences must not share pages: moving one's rows would overwrite the
+    other's (refused with PAD_B200_CHECK=1)."""
     assert weights.is_cuda, "pad_b200 requires CUDA tensors"
     assert weights.dtype == torch.float32 and weights.dim() == 3, "weights must be fp32 [num_pages, Hkv, page_size]"
     assert budget >= 1, "budget must be >= 1"
@@ -42,10 +44,35 @@ def paged_kv_evict_plan(weights: torch.Tensor, block_table: torch.Tensor, seq_le
     if slot_positions is not None and total_lens is None:
         total_lens = seq_lens
     _check_values(weights.device)
+    _check_own_pages(block_table, seq_lens, weights.shape[2])
     got = _OPS.kv_evict_plan(weights, block_table, seq_lens, budget, recent, slot_positions,
                              total_lens if slot_positions is not None else None)
     _raise_if_checking(weights.device)
     return got
+
+
+def _check_moves(cache: torch.Tensor, block_table: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+                 counts: torch.Tensor) -> None:
+    """With PAD_B200_CHECK=1: refuse moves whose target is a source or the target of another (syncs)."""
+    if (not kernel_cuda_v4._CHECK_VALUES or cache.dim() != 4 or src.dim() != 3 or dst.shape != src.shape or
+            counts.shape != src.shape[:2] or block_table.dim() != 2 or block_table.shape[0] != src.shape[0]):
+        return  # (shapes the operator refuses)
+    batch, heads, most = src.shape
+    page_size, width = cache.shape[1], block_table.shape[1] * cache.shape[1]
+    dev = block_table.device
+    seq = torch.arange(batch, device=dev).view(-1, 1, 1)
+    head = torch.arange(heads, device=dev).view(1, -1, 1)
+    src, dst = src.to(dev).long(), dst.to(dev).long()
+    on = (torch.arange(most, device=dev) < counts.to(dev)[..., None]) & (src >= 0) & (src < width) & (dst >= 0) & (dst < width)
+
+    def rows(slots):
+        slots = slots.clamp(0, max(width - 1, 0))
+        page = block_table[seq, slots // page_size].long() if width > 0 else slots
+        return ((page * page_size + slots % page_size) * heads + head)[on]
+
+    to = rows(dst)
+    if to.unique().numel() != to.numel() or torch.isin(to, rows(src)).any():
+        raise ValueError("a move's target occurs twice or is the source of a move")
 
 
 def paged_kv_move(caches: Sequence[torch.Tensor], block_table: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
@@ -54,9 +81,11 @@ def paged_kv_move(caches: Sequence[torch.Tensor], block_table: torch.Tensor, src
     """Carry out a plan's moves, in place: slot src[b, h, i] -> dst[b, h, i] for
     i < counts[b, h], in 1 to 4 caches [num_pages, page_size, Hkv, row] of any
     type (an fp16 cache's K and V, or a 4-bit cache's four tensors) and in
-    weights and slot_positions. No dst may be a src or occur twice."""
+    weights and slot_positions. No dst may be a src or occur twice, neither by
+    its slot nor by a page that two sequences name (refused with PAD_B200_CHECK=1)."""
     assert len(caches) >= 1 and all(c.is_cuda for c in caches), "pad_b200 requires CUDA tensors"
     _check_values(caches[0].device)
+    _check_moves(caches[0], block_table, src, dst, counts)
     _OPS.kv_move(list(caches), block_table, src, dst, counts, weights, slot_positions)
     _raise_if_checking(caches[0].device)
 

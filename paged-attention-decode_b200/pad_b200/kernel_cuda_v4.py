@@ -139,6 +139,27 @@ def _check_values(device: torch.device) -> None:
         read_error_flags(device)
 
 
+def _live_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, page_size: int) -> torch.Tensor | None:
+    """Mask of the block_table entries that the sequences reach (None: shapes the operator will refuse)."""
+    if block_table.dim() != 2 or seq_lens.dim() != 1 or block_table.shape[0] != seq_lens.shape[0] or page_size < 1:
+        return None
+    pages = (seq_lens.to(block_table.device).long() + page_size - 1) // page_size
+    return torch.arange(block_table.shape[1], device=block_table.device)[None, :] < pages[:, None]
+
+
+def _check_own_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, page_size: int) -> None:
+    """With PAD_B200_CHECK=1: refuse sequences that share a page (syncs)."""
+    if not _CHECK_VALUES:
+        return
+    live = _live_pages(block_table, seq_lens, page_size)
+    if live is None:
+        return
+    ids = block_table[live]
+    ids = ids[ids >= 0]
+    if ids.unique().numel() != ids.numel():
+        raise ValueError("sequences share pages: their attention weights and evictions cannot be kept apart")
+
+
 def _raise_if_checking(device: torch.device) -> None:
     """With PAD_B200_CHECK=1: raise for the flags of the call just made (syncs)."""
     if _CHECK_VALUES:

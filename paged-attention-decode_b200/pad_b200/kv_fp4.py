@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from .decode_weights import _new_tokens
-from .kernel_cuda_v4 import _check_values, _raise_if_checking
+from .kernel_cuda_v4 import _check_own_pages, _check_values, _raise_if_checking
 
 _OPS = _lib.ops()
 FP4_HEAD_DIMS = (32, 64, 128)
@@ -107,6 +107,8 @@ def paged_attention_decode_fp4(
     if slot_positions is not None and total_lens is None:
         total_lens = seq_lens
     _check_values(q.device)
+    if weights is not None:
+        _check_own_pages(block_table, seq_lens, k_cache.shape[1])
     out = _OPS.decode_fp4(q, k_cache, k_scales, v_cache, v_scales, block_table, seq_lens,
                           0 if num_splits is None else int(num_splits),
                           float(scale) if scale is not None else 1.0 / math.sqrt(head_dim), out, weights, num_new,

@@ -328,3 +328,51 @@ def test_plan_and_evict_of_an_empty_pool():
     # sequences that claim slots of a pool without pages are flagged
     src, dst, counts, lens = pad_b200.paged_kv_evict_plan(w, bt, sl + 40, 8)
     assert pad_b200.read_error_flags() == _lib.PAD_FLAG_BAD_PAGE_ID and lens.eq(8).all()
+
+
+@gpu
+def test_shared_pages_and_unsound_moves_are_refused_when_asked_for(monkeypatch):
+    """PAD_B200_CHECK: nothing is written where two sequences name a page, or a move's target is named twice."""
+    _need_cuda()
+    from pad_b200 import kernel_cuda_v4
+
+    monkeypatch.setattr(kernel_cuda_v4, "_CHECK_VALUES", True)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    pages, ps, hkv, d = 50, 16, 2, 64  # a pool far larger than the batch: no flag tells
+    q = torch.randn(3, 4, d, device="cuda").half()
+    k = torch.randn(pages, ps, hkv, d, device="cuda").half()
+    fp4 = pad_b200.paged_kv_cache_fp4(pages, ps, hkv, d)
+    w = torch.rand(pages, hkv, ps, device="cuda")
+    was, k_was = w.clone(), k.clone()
+    calls = [lambda bt, n: pad_b200.paged_attention_decode_weights(q, k, k, bt, n, w),
+             lambda bt, n: pad_b200.paged_attention_decode_fp4(q, *fp4, bt, n, weights=w),
+             lambda bt, n: pad_b200.paged_kv_evict_plan(w, bt, n, 20),
+             lambda bt, n: pad_b200.paged_kv_evict([k], w, bt, n, 20)]
+    shared = [([[0, 1, 2], [0, 3, 4], [5, 6, 7]], [40, 40, 40]),  # a common first page
+              ([[0, 1, 2], [3, 4, 5], [6, 7, 6]], [40, 40, 33]),  # one sequence names a page twice
+              ([[0, 1, 2], [3, 4, 5], [6, 7, 2]], [33, 48, 40])]
+    for bt, n in shared:
+        for call in calls:
+            with pytest.raises(ValueError, match="share pages"):
+                call(i32(bt), torch.tensor(n, device="cuda"))
+    assert torch.equal(w, was) and torch.equal(k, k_was)
+    # ids behind the sequences, of empty ones and of none are no sharing; the decode without weights may share
+    for bt, n in [([[0, 1, 2], [3, 4, 2], [0, 0, 0]], [40, 32, 0]), ([[0, 1, 1], [3, 4, 5], [6, 6, 6]], [17, 48, 16])]:
+        for call in calls:
+            call(i32(bt), torch.tensor(n, device="cuda"))
+    pad_b200.paged_attention_decode_fp4(q, *fp4, i32(shared[0][0]), i32(shared[0][1]))
+    # moves given by hand
+    bt, cache = i32([[0, 1, 2], [3, 4, 0]]), torch.arange(pages * ps * 8, device="cuda").view(pages, ps, 1, 8)
+    was = cache.clone()
+    lists = lambda a, b: torch.tensor([[a], [b]], dtype=torch.int32, device="cuda")  # noqa: E731
+    for src, dst, n in [(lists([40, 41], [40, 41]), lists([3, 3], [1, 2]), [2, 0]),        # a target twice
+                        (lists([40, 20], [40, 41]), lists([20, 3], [1, 2]), [2, 0]),       # a target that is a source
+                        (lists([40, 41], [20, 21]), lists([5, 6], [37, 38]), [2, 2]),      # by way of page 0
+                        (lists([40, 41], [37, 21]), lists([5, 6], [2, 3]), [2, 1])]:
+        with pytest.raises(ValueError, match="target"):
+            pad_b200.paged_kv_move([cache], bt, src, dst, i32(n).view(2, 1))
+    assert torch.equal(cache, was)
+    pad_b200.paged_kv_move([cache], bt, lists([40, 41], [20, 21]), lists([5, 5], [2, 3]), i32([1, 2]).view(2, 1))
+    for (p, r), (p2, r2) in {(0, 5): (2, 8), (3, 2): (4, 4), (3, 3): (4, 5)}.items():
+        was[p, r] = was[p2, r2]
+    assert torch.equal(cache, was)
