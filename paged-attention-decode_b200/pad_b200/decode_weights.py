@@ -8,7 +8,8 @@ import math
 import torch
 
 from . import _lib
-from .kernel_cuda_v4 import _SUPPORTED_HEAD_DIMS, _check_own_pages, _check_values, _raise_if_checking
+from .kernel_cuda_v4 import (_SUPPORTED_HEAD_DIMS, _check_own_pages, _check_positions, _check_values,
+                             _raise_if_checking)
 
 _OPS = _lib.ops()
 
@@ -46,7 +47,9 @@ def paged_attention_decode_weights(
     integer tensor [B], one of each: 1 for those that decode, the length of its
     prompt for one that has just joined them. slot_positions [num_pages, Hkv, page_size] int32,
     if given, gets the new tokens' positions, counted from total_lens [B] (the
-    tokens each sequence has seen; None: seq_lens, as before any eviction).
+    tokens each sequence has seen; None: seq_lens, which is right before a first
+    eviction only, and refused later with PAD_B200_CHECK=1: the new tokens would
+    get positions that older ones have).
     Sequences must not share pages (their weights would lose additions, other
     ones from run to run; refused with PAD_B200_CHECK=1)."""
     assert q.is_cuda and k_cache.is_cuda and v_cache.is_cuda, "pad_b200 requires CUDA tensors"
@@ -59,10 +62,12 @@ def paged_attention_decode_weights(
     assert num_q_heads % k_cache.shape[2] == 0, "num_q_heads must be divisible by num_kv_heads (GQA)"
     assert head_dim in _SUPPORTED_HEAD_DIMS, f"head_dim must be one of {_SUPPORTED_HEAD_DIMS}"
     assert num_splits is None or num_splits >= 1, "num_splits must be >= 1"
+    new = num_new
     num_new, num_new_of = _new_tokens(num_new)
     assert slot_positions is not None or total_lens is None, "total_lens goes with slot_positions"
     if slot_positions is not None and total_lens is None:
         total_lens = seq_lens
+        _check_positions(slot_positions, total_lens, block_table, seq_lens, new)
     _check_values(q.device)
     _check_own_pages(block_table, seq_lens, k_cache.shape[1])
     out = _OPS.decode_weights(q, k_cache, v_cache, block_table, seq_lens, 0 if num_splits is None else int(num_splits),

@@ -15,7 +15,7 @@ from typing import Sequence
 import torch
 
 from . import _lib, kernel_cuda_v4
-from .kernel_cuda_v4 import _check_own_pages, _check_values, _raise_if_checking
+from .kernel_cuda_v4 import _check_own_pages, _check_positions, _check_values, _raise_if_checking
 
 _OPS = _lib.ops()
 
@@ -28,7 +28,8 @@ def paged_kv_evict_plan(weights: torch.Tensor, block_table: torch.Tensor, seq_le
     For every sequence with seq_lens[b] > budget and every KV head the slots
     kept are first those whose slot_positions are at least total_lens[b] -
     recent (total_lens [B]: tokens the sequence has seen; None: seq_lens, which
-    is right before a first eviction only), then the heaviest (NaN above all),
+    is right before a first eviction only, and refused later with
+    PAD_B200_CHECK=1: too many tokens would count as recent), then the heaviest (NaN above all),
     ties to the lower slot. Returns (src, dst, counts,
     new_lens): move i < counts[b, h] copies slot src[b, h, i] to dst[b, h, i]
     (both ascending, -1 behind the last), and new_lens = min(seq_lens, budget).
@@ -45,6 +46,8 @@ def paged_kv_evict_plan(weights: torch.Tensor, block_table: torch.Tensor, seq_le
         total_lens = seq_lens
     _check_values(weights.device)
     _check_own_pages(block_table, seq_lens, weights.shape[2])
+    if recent > 0:
+        _check_positions(slot_positions, total_lens, block_table, seq_lens)
     got = _OPS.kv_evict_plan(weights, block_table, seq_lens, budget, recent, slot_positions,
                              total_lens if slot_positions is not None else None)
     _raise_if_checking(weights.device)
@@ -95,7 +98,9 @@ def paged_kv_evict(caches: Sequence[torch.Tensor], weights: torch.Tensor, block_
                    slot_positions: torch.Tensor | None = None,
                    total_lens: torch.Tensor | None = None) -> torch.Tensor:
     """Cut every sequence to ``budget`` slots in place (paged_kv_evict_plan, then
-    paged_kv_move) and return the new seq_lens. The pages behind them are free."""
+    paged_kv_move) and return the new seq_lens. The pages behind them are free.
+    total_lens may be left out before a sequence's first eviction only (see
+    paged_kv_evict_plan): from then on seq_lens is not what it has seen."""
     src, dst, counts, new_lens = paged_kv_evict_plan(weights, block_table, seq_lens, budget, recent,
                                                      slot_positions=slot_positions, total_lens=total_lens)
     paged_kv_move(caches, block_table, src, dst, counts, weights=weights, slot_positions=slot_positions)

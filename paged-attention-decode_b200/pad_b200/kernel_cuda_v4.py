@@ -160,6 +160,27 @@ def _check_own_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, page_siz
         raise ValueError("sequences share pages: their attention weights and evictions cannot be kept apart")
 
 
+def _check_positions(slot_positions: torch.Tensor, total_lens: torch.Tensor, block_table: torch.Tensor,
+                     seq_lens: torch.Tensor, num_new: int | torch.Tensor = 0) -> None:
+    """With PAD_B200_CHECK=1: refuse tokens (but the num_new last of each sequence) whose position is not below
+    total_lens - num_new, the mark of lengths that an eviction has cut (syncs)."""
+    if not _CHECK_VALUES or slot_positions.dim() != 3 or total_lens.shape != seq_lens.shape:
+        return
+    pages, heads, page_size = slot_positions.shape
+    if _live_pages(block_table, seq_lens, page_size) is None or pages == 0 or block_table.shape[1] == 0:
+        return
+    dev = slot_positions.device
+    slot = torch.arange(block_table.shape[1] * page_size, device=dev)[None, :]
+    n, total = seq_lens.to(dev).long()[:, None], total_lens.to(dev).long()[:, None]
+    new = num_new.to(dev).long()[:, None] if isinstance(num_new, torch.Tensor) else num_new
+    page = block_table.to(dev).long().repeat_interleave(page_size, 1)
+    old = (slot < n - new) & (page >= 0) & (page < pages)
+    at = slot_positions[page.clamp(0, pages - 1), :, slot % page_size]  # [B, slots, heads]
+    if (old[..., None] & (at >= (total - new)[..., None])).any():
+        raise ValueError("slot_positions holds positions that total_lens says are still to come (after an eviction "
+                         "total_lens must be given: the tokens each sequence has seen, not seq_lens)")
+
+
 def _raise_if_checking(device: torch.device) -> None:
     """With PAD_B200_CHECK=1: raise for the flags of the call just made (syncs)."""
     if _CHECK_VALUES:

@@ -20,7 +20,7 @@ import torch
 
 from . import _lib
 from .decode_weights import _new_tokens
-from .kernel_cuda_v4 import _check_own_pages, _check_values, _raise_if_checking
+from .kernel_cuda_v4 import _check_own_pages, _check_positions, _check_values, _raise_if_checking
 
 _OPS = _lib.ops()
 FP4_HEAD_DIMS = (32, 64, 128)
@@ -101,11 +101,13 @@ def paged_attention_decode_fp4(
     assert head_dim in FP4_HEAD_DIMS, f"head_dim must be one of {FP4_HEAD_DIMS}"
     assert num_q_heads % k_cache.shape[2] == 0, "num_q_heads must be divisible by num_kv_heads (GQA)"
     assert num_splits is None or num_splits >= 1, "num_splits must be >= 1"
+    new = num_new
     num_new, num_new_of = _new_tokens(num_new)
     assert weights is not None or slot_positions is None, "slot_positions go with weights"
     assert slot_positions is not None or total_lens is None, "total_lens goes with slot_positions"
     if slot_positions is not None and total_lens is None:
         total_lens = seq_lens
+        _check_positions(slot_positions, total_lens, block_table, seq_lens, new)
     _check_values(q.device)
     if weights is not None:
         _check_own_pages(block_table, seq_lens, k_cache.shape[1])

@@ -256,3 +256,37 @@ def test_a_sequence_joins_the_others_with_its_prompt(fp4, captured):
                 assert {86, 87, 88, 89} <= set(at2[bt[2, t // lp.ps], h, t % lp.ps].tolist())
     assert lp.lens.tolist() == [64, 39, 64]
     assert pad_b200.read_error_flags() == 0
+
+
+@gpu
+@pytest.mark.parametrize("fp4", [False, True])
+def test_lengths_left_out_after_an_eviction_are_refused_when_asked_for(fp4, monkeypatch):
+    """total_lens may be left out until a first eviction; afterwards positions would be given twice and the window of
+    recent tokens be too wide."""
+    _need_cuda()
+    from pad_b200 import kernel_cuda_v4
+
+    monkeypatch.setattr(kernel_cuda_v4, "_CHECK_VALUES", True)
+    lp = Loop(fp4, [100, 20], budget=64, recent=8, seed=4)
+    q = lp.rand(2, lp.hkv * lp.g, lp.d)
+    decode = lambda new, **kw: (pad_b200.paged_attention_decode_fp4(  # noqa: E731
+        q, *lp.caches, lp.bt, lp.lens, weights=lp.w, num_new=new, slot_positions=lp.at, **kw) if fp4 else
+        pad_b200.paged_attention_decode_weights(q, *lp.caches, lp.bt, lp.lens, lp.w, new, slot_positions=lp.at, **kw))
+    evict = lambda **kw: pad_b200.paged_kv_evict(lp.caches, lp.w, lp.bt, lp.lens, lp.budget, lp.recent,  # noqa: E731
+                                                 slot_positions=lp.at, **kw)
+    decode(10 ** 6)
+    decode(0)
+    lp.append(lp.rand(2, lp.hkv, lp.d), lp.rand(2, lp.hkv, lp.d))
+    decode(torch.tensor([1, 1], device="cuda"))
+    lp.lens.copy_(evict())
+    lp.append(lp.rand(2, lp.hkv, lp.d), lp.rand(2, lp.hkv, lp.d))
+    was = lp.at.clone()
+    for new in (1, torch.ones(2, dtype=torch.int32, device="cuda")):
+        with pytest.raises(ValueError, match="total_lens"):
+            decode(new)
+    assert torch.equal(lp.at, was)
+    decode(1, total_lens=lp.total)
+    with pytest.raises(ValueError, match="total_lens"):
+        evict()
+    lp.lens.copy_(evict(total_lens=lp.total))
+    assert lp.lens.tolist() == [64, 22] and lp.at.max().item() == 10 ** 6  # (left by former owners, never looked at)
