@@ -531,3 +531,32 @@ def test_new_tokens_by_sequence_refusals_without_a_device():
     for new, hq, text in [(0, 12, b"num_new"), (p, 11, b"divisible")]:
         assert call(new, 2, hq) == _lib.PAD_ERR_INVALID_ARGUMENT and text in lib.pad_last_error()
     assert call(0, 0) == _lib.PAD_OK
+
+
+@gpu
+@pytest.mark.parametrize("alike", [True, False])
+@pytest.mark.parametrize("bad_id", [-1, 10 ** 6])
+def test_a_bad_page_reads_as_zero_rows(alike, bad_id):
+    """Page 0 and the pages read before hold no zeros, so that anything read in a bad page's place shows."""
+    _need_cuda()
+    pad_b200.read_error_flags()
+    q, caches, k, v, bt, sl = fp4_case([100, 64, 90], 2, 4, 64, 16, seed=31)
+    (kc, ks), (vc, vs) = [[c.copy() for c in x] for x in (caches[:2], caches[2:])]
+    kc[0], vc[0], ks[0], vs[0] = 0x77, 0x77, 126, 126  # values of 3
+    pages = k.shape[0]
+    bt = bt.copy()
+    bt[0, 1] = bt[2, 0] = bad_id
+    zeros = lambda c: np.concatenate([c, np.zeros_like(c[:1])])  # noqa: E731  (one more page, of zeros)
+    good = np.where(bt == bad_id, pages, bt)
+    ref, probs = co.decode(q, co.dequantise(zeros(kc), zeros(ks)), co.dequantise(zeros(vc), zeros(vs)), good, sl)
+    cg = [_cuda(c) for c in (kc, ks, vc, vs)]
+    if not alike:
+        cg[2] = _cuda(vc.transpose(0, 2, 1, 3)).permute(0, 2, 1, 3)
+    w = torch.zeros(pages, 2, 16, device="cuda")
+    for weights in (None, w):
+        out = pad_b200.paged_attention_decode_fp4(_cuda(q, torch.float16), *cg, _cuda(bt), _cuda(sl), weights=weights,
+                                                  num_new=10 ** 6)
+        assert_parity(out.float().cpu().numpy(), ref)
+        assert pad_b200.read_error_flags() == _lib.PAD_FLAG_BAD_PAGE_ID
+    want = co.accumulate(np.zeros((pages + 1, 2, 16)), probs, good, sl, 10 ** 6)[:pages]
+    check_weights(w.cpu().numpy(), want, rel_bound(64, 100, smax_of(q, co.dequantise(kc, ks), 64)))
