@@ -28,13 +28,21 @@ using namespace pad;
 #endif
 constexpr int kMergeCols = PAD_MERGE_COLS;
 
+// The merge kernels of a head dim (this is the one translation unit that
+// instantiates them).
+struct MergeKernels {
+  const void* few;   // merge_kernel<D, 128>: few partials per split pair
+  const void* some;  // merge_kernel<D, 256, D/32, 4>: a handful of partials, D split over CTAs
+  const void* many;  // merge_kernel<D, 256, D/32, 8>: many partials (long context)
+  int dsplit;
+};
+
 template <int D>
-void set_merge(Instance* in) {
+MergeKernels merge_kernels() {
   constexpr int DS = D >= 2 * kMergeCols ? D / kMergeCols : 1;
-  in->merge_small = reinterpret_cast<const void*>(&merge_kernel<D, 128, 1, 4>);
-  in->merge_mid = reinterpret_cast<const void*>(&merge_kernel<D, 256, DS, 4>);
-  in->merge_large = reinterpret_cast<const void*>(&merge_kernel<D, 256, DS, 8>);
-  in->merge_dsplit = DS;
+  return {reinterpret_cast<const void*>(&merge_kernel<D, 128, 1, 4>),
+          reinterpret_cast<const void*>(&merge_kernel<D, 256, DS, 4>),
+          reinterpret_cast<const void*>(&merge_kernel<D, 256, DS, 8>), DS};
 }
 
 // Merge variant by partials per split pair (partitions / pairs): up to
@@ -47,17 +55,10 @@ void set_merge(Instance* in) {
 #define PAD_MERGE_DEEP 32
 #endif
 constexpr int64_t kMergeWide = PAD_MERGE_WIDE, kMergeDeep = PAD_MERGE_DEEP;
+constexpr int64_t kFewPairs = 16;  // the num_splits=None heuristic: see make_plan
 
 bool pick_instance(int64_t head_dim, int64_t gqa, int hg, bool swz, Instance* out, bool weights = false) {
-  if (!(weights ? pick_decode_weights(head_dim, gqa, hg, swz, out) : pick_decode<false>(head_dim, gqa, hg, swz, out)))
-    return false;
-  switch (head_dim) {
-    case 16: set_merge<16>(out); break;
-    case 32: set_merge<32>(out); break;
-    case 64: set_merge<64>(out); break;
-    default: set_merge<128>(out); break;
-  }
-  return true;
+  return weights ? pick_decode_weights(head_dim, gqa, hg, swz, out) : pick_decode<false>(head_dim, gqa, hg, swz, out);
 }
 
 // Largest power of two that divides page_size, capped at the tile's token
@@ -299,13 +300,10 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 namespace pad {
 
 int launch_merge(const MergeLaunch& m, cudaStream_t stream) {
-  Instance in = {};
-  switch (m.head_dim) {
-    case 16: set_merge<16>(&in); break;
-    case 32: set_merge<32>(&in); break;
-    case 64: set_merge<64>(&in); break;
-    default: set_merge<128>(&in); break;
-  }
+  const MergeKernels k = m.head_dim == 16   ? merge_kernels<16>()
+                         : m.head_dim == 32 ? merge_kernels<32>()
+                         : m.head_dim == 64 ? merge_kernels<64>()
+                                            : merge_kernels<128>();
   MergeLaunch a = m;
   void* args[] = {&a.ws_o, &a.ws_ml, &a.ws_meta, &a.out, &a.out_sb, &a.out_sh, &a.ngroups, &a.rows, &a.guess_ncap,
                   &a.guess_parts, &a.norm};
@@ -313,7 +311,7 @@ int launch_merge(const MergeLaunch& m, cudaStream_t stream) {
   const int64_t pairs = m.batch * m.ngroups;
   const bool wide = m.partitions > kMergeWide * pairs;
   cfg.gridDim = dim3((unsigned)(m.meta_by_pair ? pairs : m.partitions), (unsigned)m.rows,
-                     wide ? (unsigned)in.merge_dsplit : 1u);
+                     wide ? (unsigned)k.dsplit : 1u);
   // A split pair has about partitions / pairs partials: fold a handful with a
   // small block, long-context splits (hundreds of partials) with a wide one.
   cfg.blockDim = dim3(wide ? 256 : 128);
@@ -325,7 +323,7 @@ int launch_merge(const MergeLaunch& m, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const bool deep = m.partitions > kMergeDeep * pairs;  // 8 loads in flight
-  const cudaError_t e = cudaLaunchKernelExC(&cfg, wide ? (deep ? in.merge_large : in.merge_mid) : in.merge_small, args);
+  const cudaError_t e = cudaLaunchKernelExC(&cfg, wide ? (deep ? k.many : k.some) : k.few, args);
   return e == cudaSuccess ? PAD_OK : cuda_fail(e, "launching the merge kernel");
 }
 

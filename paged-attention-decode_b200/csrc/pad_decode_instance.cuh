@@ -7,10 +7,6 @@ namespace pad {
 
 struct Instance {
   const void* kernel;          // decode_stream_kernel<TR>
-  const void* merge_small;     // merge_kernel<D, 128>: few partials per split pair
-  const void* merge_mid;       // merge_kernel<D, 256, D/32, 4>: a handful of partials, D split over CTAs
-  const void* merge_large;     // merge_kernel<D, 256, D/32, 8>: many partials (long context)
-  int merge_dsplit;
   int smem_bytes;
   int segw;                    // bytes per row segment (TMA box inner extent)
   bool swz;
@@ -18,8 +14,6 @@ struct Instance {
   int tt;                      // tokens per tile
 };
 
-// The decode kernel's part of an instance (the merge kernels are filled in by
-// pad_decode.cu, the one translation unit that instantiates them).
 template <int D, int NT, int HG, bool SWZ, bool WT>
 Instance make_instance() {
   using TR = Traits<D, NT, HG, SWZ, WT>;
@@ -81,7 +75,6 @@ int launch_merge(const MergeLaunch& m, cudaStream_t stream);
 // KV heads per tile, and the SM count of a device (pad_decode.cu).
 int head_group_for(int64_t hkv, int64_t gqa);
 int sm_count(int device, int* num_sms);
-constexpr int64_t kFewPairs = 16;  // see the num_splits=None heuristic of pad_decode.cu
 
 // The instances that keep their scores (pad_decode_weights.cu).
 bool pick_decode_weights(int64_t head_dim, int64_t gqa, int hg, bool swz, Instance* out);
