@@ -7,18 +7,16 @@ import math
 
 import torch
 
-from . import _lib
-from .kernel_cuda_v4 import (_SUPPORTED_HEAD_DIMS, _check_own_pages, _check_positions, _check_values,
-                             _raise_if_checking)
+from . import _lib, kernel_cuda_v4
+from .kernel_cuda_v4 import _SUPPORTED_HEAD_DIMS, _check_own_pages, _check_positions, _raise_flags_of, read_error_flags
 
 _OPS = _lib.ops()
 
 
 def _new_tokens(num_new: int | torch.Tensor) -> tuple[int, torch.Tensor | None]:
-    """num_new as the operators take it: a number, or a tensor with one of each sequence."""
+    """num_new as the operators take it, unless it is an int: a number, or a tensor with one of each sequence."""
     if isinstance(num_new, torch.Tensor):
         return 0, num_new
-    assert num_new >= 0, "num_new must be >= 0"
     return int(num_new), None
 
 
@@ -62,16 +60,21 @@ def paged_attention_decode_weights(
     assert num_q_heads % k_cache.shape[2] == 0, "num_q_heads must be divisible by num_kv_heads (GQA)"
     assert head_dim in _SUPPORTED_HEAD_DIMS, f"head_dim must be one of {_SUPPORTED_HEAD_DIMS}"
     assert num_splits is None or num_splits >= 1, "num_splits must be >= 1"
-    new = num_new
-    num_new, num_new_of = _new_tokens(num_new)
+    new, num_new_of = num_new, None
+    if type(num_new) is not int:
+        num_new, num_new_of = _new_tokens(num_new)
+    assert num_new >= 0, "num_new must be >= 0"
     assert slot_positions is not None or total_lens is None, "total_lens goes with slot_positions"
     if slot_positions is not None and total_lens is None:
         total_lens = seq_lens
-        _check_positions(slot_positions, total_lens, block_table, seq_lens, new)
-    _check_values(q.device)
-    _check_own_pages(block_table, seq_lens, k_cache.shape[1])
+        if kernel_cuda_v4._CHECK_VALUES:
+            _check_positions(slot_positions, total_lens, block_table, seq_lens, new)
+    if kernel_cuda_v4._CHECK_VALUES:
+        read_error_flags(q.device)
+        _check_own_pages(block_table, seq_lens, k_cache.shape[1])
     out = _OPS.decode_weights(q, k_cache, v_cache, block_table, seq_lens, 0 if num_splits is None else int(num_splits),
                               float(scale) if scale is not None else 1.0 / math.sqrt(head_dim), out, weights,
                               num_new, slot_positions, total_lens, num_new_of)
-    _raise_if_checking(q.device)
+    if kernel_cuda_v4._CHECK_VALUES:
+        _raise_flags_of(q.device)
     return out

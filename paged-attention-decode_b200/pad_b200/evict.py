@@ -15,7 +15,7 @@ from typing import Sequence
 import torch
 
 from . import _lib, kernel_cuda_v4
-from .kernel_cuda_v4 import _check_own_pages, _check_positions, _check_values, _raise_if_checking
+from .kernel_cuda_v4 import _check_own_pages, _check_positions, _raise_flags_of, read_error_flags
 
 _OPS = _lib.ops()
 
@@ -44,21 +44,23 @@ def paged_kv_evict_plan(weights: torch.Tensor, block_table: torch.Tensor, seq_le
     assert recent == 0 or slot_positions is not None, "recent needs slot_positions"
     if slot_positions is not None and total_lens is None:
         total_lens = seq_lens
-    _check_values(weights.device)
-    _check_own_pages(block_table, seq_lens, weights.shape[2])
-    if recent > 0:
-        _check_positions(slot_positions, total_lens, block_table, seq_lens)
+    if kernel_cuda_v4._CHECK_VALUES:
+        read_error_flags(weights.device)
+        _check_own_pages(block_table, seq_lens, weights.shape[2])
+        if recent > 0:
+            _check_positions(slot_positions, total_lens, block_table, seq_lens)
     got = _OPS.kv_evict_plan(weights, block_table, seq_lens, budget, recent, slot_positions,
                              total_lens if slot_positions is not None else None)
-    _raise_if_checking(weights.device)
+    if kernel_cuda_v4._CHECK_VALUES:
+        _raise_flags_of(weights.device)
     return got
 
 
 def _check_moves(cache: torch.Tensor, block_table: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
                  counts: torch.Tensor) -> None:
-    """With PAD_B200_CHECK=1: refuse moves whose target is a source or the target of another (syncs)."""
-    if (not kernel_cuda_v4._CHECK_VALUES or cache.dim() != 4 or src.dim() != 3 or dst.shape != src.shape or
-            counts.shape != src.shape[:2] or block_table.dim() != 2 or block_table.shape[0] != src.shape[0]):
+    """Refuse moves whose target is a source or the target of another."""
+    if (cache.dim() != 4 or src.dim() != 3 or dst.shape != src.shape or counts.shape != src.shape[:2] or
+            block_table.dim() != 2 or block_table.shape[0] != src.shape[0]):
         return  # (shapes the operator refuses)
     batch, heads, most = src.shape
     page_size, width = cache.shape[1], block_table.shape[1] * cache.shape[1]
@@ -87,10 +89,12 @@ def paged_kv_move(caches: Sequence[torch.Tensor], block_table: torch.Tensor, src
     weights and slot_positions. No dst may be a src or occur twice, neither by
     its slot nor by a page that two sequences name (refused with PAD_B200_CHECK=1)."""
     assert len(caches) >= 1 and all(c.is_cuda for c in caches), "pad_b200 requires CUDA tensors"
-    _check_values(caches[0].device)
-    _check_moves(caches[0], block_table, src, dst, counts)
+    if kernel_cuda_v4._CHECK_VALUES:
+        read_error_flags(caches[0].device)
+        _check_moves(caches[0], block_table, src, dst, counts)
     _OPS.kv_move(list(caches), block_table, src, dst, counts, weights, slot_positions)
-    _raise_if_checking(caches[0].device)
+    if kernel_cuda_v4._CHECK_VALUES:
+        _raise_flags_of(caches[0].device)
 
 
 def paged_kv_evict(caches: Sequence[torch.Tensor], weights: torch.Tensor, block_table: torch.Tensor,

@@ -133,12 +133,9 @@ def read_error_flags(device: torch.device | None = None, reset: bool = True) -> 
     return v
 
 
-def _check_values(device: torch.device) -> None:
-    """With PAD_B200_CHECK=1: forget flags of earlier calls (syncs)."""
-    if _CHECK_VALUES:
-        read_error_flags(device)
-
-
+# What the calls do with PAD_B200_CHECK=1, each under a test of _CHECK_VALUES in
+# the call itself (a function call and a device look-up are time that a small call
+# shows). All of them sync.
 def _live_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, page_size: int) -> torch.Tensor | None:
     """Mask of the block_table entries that the sequences reach (None: shapes the operator will refuse)."""
     if block_table.dim() != 2 or seq_lens.dim() != 1 or block_table.shape[0] != seq_lens.shape[0] or page_size < 1:
@@ -148,9 +145,7 @@ def _live_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, page_size: in
 
 
 def _check_own_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, page_size: int) -> None:
-    """With PAD_B200_CHECK=1: refuse sequences that share a page (syncs)."""
-    if not _CHECK_VALUES:
-        return
+    """Refuse sequences that share a page."""
     live = _live_pages(block_table, seq_lens, page_size)
     if live is None:
         return
@@ -162,9 +157,9 @@ def _check_own_pages(block_table: torch.Tensor, seq_lens: torch.Tensor, page_siz
 
 def _check_positions(slot_positions: torch.Tensor, total_lens: torch.Tensor, block_table: torch.Tensor,
                      seq_lens: torch.Tensor, num_new: int | torch.Tensor = 0) -> None:
-    """With PAD_B200_CHECK=1: refuse tokens (but the num_new last of each sequence) whose position is not below
-    total_lens - num_new, the mark of lengths that an eviction has cut (syncs)."""
-    if not _CHECK_VALUES or slot_positions.dim() != 3 or total_lens.shape != seq_lens.shape:
+    """Refuse tokens (but the num_new last of each sequence) whose position is not below total_lens - num_new, the mark
+    of lengths that an eviction has cut."""
+    if slot_positions.dim() != 3 or total_lens.shape != seq_lens.shape:
         return
     pages, heads, page_size = slot_positions.shape
     if _live_pages(block_table, seq_lens, page_size) is None or pages == 0 or block_table.shape[1] == 0:
@@ -181,10 +176,9 @@ def _check_positions(slot_positions: torch.Tensor, total_lens: torch.Tensor, blo
                          "total_lens must be given: the tokens each sequence has seen, not seq_lens)")
 
 
-def _raise_if_checking(device: torch.device) -> None:
-    """With PAD_B200_CHECK=1: raise for the flags of the call just made (syncs)."""
-    if _CHECK_VALUES:
-        _raise_for_flags(read_error_flags(device))
+def _raise_flags_of(device: torch.device) -> None:
+    """Raise for the flags of the call just made."""
+    _raise_for_flags(read_error_flags(device))
 
 
 def paged_kv_indices(block_table: torch.Tensor, seq_lens: torch.Tensor, page_size: int):

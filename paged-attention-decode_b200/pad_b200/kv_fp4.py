@@ -18,9 +18,9 @@ import math
 
 import torch
 
-from . import _lib
+from . import _lib, kernel_cuda_v4
 from .decode_weights import _new_tokens
-from .kernel_cuda_v4 import _check_own_pages, _check_positions, _check_values, _raise_if_checking
+from .kernel_cuda_v4 import _check_own_pages, _check_positions, _raise_flags_of, read_error_flags
 
 _OPS = _lib.ops()
 FP4_HEAD_DIMS = (32, 64, 128)
@@ -50,9 +50,11 @@ def paged_kv_append_fp4(k_new: torch.Tensor, v_new: torch.Tensor, k_cache: torch
     assert k_new.dtype == torch.float16 and v_new.dtype == torch.float16, "pad_b200 expects fp16 k_new/v_new"
     assert k_new.dim() == 3 and k_new.shape[2] in FP4_HEAD_DIMS, f"head_dim must be one of {FP4_HEAD_DIMS}"
     assert seq_ids is not None or k_new.shape[0] <= block_table.shape[0], "more tokens than sequences need seq_ids"
-    _check_values(k_cache.device)
+    if kernel_cuda_v4._CHECK_VALUES:
+        read_error_flags(k_cache.device)
     _OPS.kv_append_fp4(k_new, v_new, k_cache, k_scales, v_cache, v_scales, block_table, positions, seq_ids)
-    _raise_if_checking(k_cache.device)
+    if kernel_cuda_v4._CHECK_VALUES:
+        _raise_flags_of(k_cache.device)
 
 
 def paged_kv_read_fp4(k_cache: torch.Tensor, k_scales: torch.Tensor, v_cache: torch.Tensor, v_scales: torch.Tensor,
@@ -64,9 +66,11 @@ def paged_kv_read_fp4(k_cache: torch.Tensor, k_scales: torch.Tensor, v_cache: to
     assert k_cache.is_cuda, "pad_b200 requires CUDA tensors"
     assert 2 * k_cache.shape[3] in FP4_HEAD_DIMS, f"head_dim must be one of {FP4_HEAD_DIMS}"
     assert seq_ids is not None or positions.shape[0] <= block_table.shape[0], "more tokens than sequences need seq_ids"
-    _check_values(k_cache.device)
+    if kernel_cuda_v4._CHECK_VALUES:
+        read_error_flags(k_cache.device)
     got = _OPS.kv_read_fp4(k_cache, k_scales, v_cache, v_scales, block_table, positions, seq_ids)
-    _raise_if_checking(k_cache.device)
+    if kernel_cuda_v4._CHECK_VALUES:
+        _raise_flags_of(k_cache.device)
     return got
 
 
@@ -101,19 +105,24 @@ def paged_attention_decode_fp4(
     assert head_dim in FP4_HEAD_DIMS, f"head_dim must be one of {FP4_HEAD_DIMS}"
     assert num_q_heads % k_cache.shape[2] == 0, "num_q_heads must be divisible by num_kv_heads (GQA)"
     assert num_splits is None or num_splits >= 1, "num_splits must be >= 1"
-    new = num_new
-    num_new, num_new_of = _new_tokens(num_new)
+    new, num_new_of = num_new, None
+    if type(num_new) is not int:
+        num_new, num_new_of = _new_tokens(num_new)
+    assert num_new >= 0, "num_new must be >= 0"
     assert weights is not None or slot_positions is None, "slot_positions go with weights"
     assert slot_positions is not None or total_lens is None, "total_lens goes with slot_positions"
     if slot_positions is not None and total_lens is None:
         total_lens = seq_lens
-        _check_positions(slot_positions, total_lens, block_table, seq_lens, new)
-    _check_values(q.device)
-    if weights is not None:
-        _check_own_pages(block_table, seq_lens, k_cache.shape[1])
+        if kernel_cuda_v4._CHECK_VALUES:
+            _check_positions(slot_positions, total_lens, block_table, seq_lens, new)
+    if kernel_cuda_v4._CHECK_VALUES:
+        read_error_flags(q.device)
+        if weights is not None:
+            _check_own_pages(block_table, seq_lens, k_cache.shape[1])
     out = _OPS.decode_fp4(q, k_cache, k_scales, v_cache, v_scales, block_table, seq_lens,
                           0 if num_splits is None else int(num_splits),
                           float(scale) if scale is not None else 1.0 / math.sqrt(head_dim), out, weights, num_new,
                           slot_positions, total_lens, num_new_of)
-    _raise_if_checking(q.device)
+    if kernel_cuda_v4._CHECK_VALUES:
+        _raise_flags_of(q.device)
     return out
