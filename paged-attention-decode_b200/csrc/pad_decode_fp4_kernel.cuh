@@ -5,7 +5,7 @@
 // one list of tiles ordered (sequence, head group, tile) and every CTA takes an
 // equal contiguous range of it, as the fp16 decode does.
 //
-// At 4.25 bits a value the arithmetic, not the copy, is close to the limit (an
+// At 4.25 bits a value the arithmetic is as close to the limit as the copy (an
 // SM is sent about 43 values a clock at full bandwidth, and every one has to
 // become fp16), so the kernel is built around the fewest instructions a value:
 //   - A warp owns whole (tile, head) pieces: WPH = warps / HG warps share a
@@ -30,11 +30,13 @@
 // V's scales go onto codes in fp16, exactly for 2^-24 .. 2^13, all that the append
 // writes. Smaller ones become 0; a larger one would make codes infinite and is flagged.
 //
-// Measured (12/2 heads, head_dim 128, page 16): 64 x 4096 tokens 24.8 us a call
+// Measured (12/2 heads, head_dim 128, page 16): 64 x 4096 tokens 25.1 us a call
 // (10.9 at the measured copy rate), each further 4096 tokens of the 64 sequences
-// 14.3 us (72% of the copy rate); one sequence of 131072 tokens 16.4 us (5.4).
-// About 625 instructions a piece of 32 tokens; the schedulers issue in 59% of the
-// cycles and the integer pipe, which also converts, is busy in 51%.
+// 14.4 us (75% of the copy rate); one sequence of 131072 tokens 16.4 us (5.4).
+// About 630 instructions a piece of 32 tokens; the schedulers issue in 59% of the
+// cycles and the integer pipe, which also converts, is busy in 52%. No unit is
+// full: with three warps a scheduler it is latency, and some 10 us of a call do not
+// depend on its length.
 #pragma once
 
 #include <cfloat>

@@ -20,12 +20,14 @@
 // that add up their histograms through distributed shared memory.
 //
 // Bound: plan -- 8 bytes a slot would take 5 us for 4 x 8 x 118 thousand slots;
-// its instructions (a gather, three histogram passes and two votes a slot) and the
-// exchanges in the cluster take 41 us. 64 x 2 x 2080 slots: 8 us, the latency of
-// the same chain. Move -- HBM bytes, 2 x row bytes a move: 131 thousand fp16 rows
-// of 256 + 256 bytes in 33 us (62% of the copy rate); a 4-bit row's 4-byte scales,
-// weight and position each cost a 32-byte sector both ways, so its 39% of the copy
-// rate over useful bytes is about two thirds over sectors.
+// the chain of a gather, three histogram passes, two or three sweeps and the
+// exchanges in the cluster takes 41 us, issuing in 38% of the cycles and waiting
+// for loads and barriers in the others. 64 x 2 x 2080 slots: 8 us, the latency of
+// the same chain. Move -- 2 x row bytes a move: 131 thousand fp16 rows of 256 +
+// 256 bytes in 33 us (62% of the copy rate), the rest the latency of its groups of
+// loads and stores; a 4-bit row's 4-byte scales, weight and position each cost a
+// 32-byte sector both ways, so its 39% of the copy rate over useful bytes is about
+// two thirds over sectors.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
