@@ -29,8 +29,8 @@ def paged_kv_evict_plan(weights: torch.Tensor, block_table: torch.Tensor, seq_le
     kept are first those whose slot_positions are at least total_lens[b] -
     recent (total_lens [B]: tokens the sequence has seen; None: seq_lens, which
     is right before a first eviction only, and refused later with
-    PAD_B200_CHECK=1: too many tokens would count as recent), then the heaviest (NaN above all),
-    ties to the lower slot. Returns (src, dst, counts,
+    PAD_B200_CHECK=1: too many tokens would count as recent), then the heaviest
+    (NaN above all), ties to the lower slot. Returns (src, dst, counts,
     new_lens): move i < counts[b, h] copies slot src[b, h, i] to dst[b, h, i]
     (both ascending, -1 behind the last), and new_lens = min(seq_lens, budget).
     Slots keep their place unless they lie at or above the budget, so their

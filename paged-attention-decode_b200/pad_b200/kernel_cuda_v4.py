@@ -23,7 +23,9 @@ Differences, by design:
   * With ``PAD_B200_CHECK=1`` in the environment the call synchronises and
     raises ValueError for invalid block-table page ids or out-of-range
     seq_lens -- the value checks of the reference oracle
-    (src/reference.py:40-41,107-112); off by default because it syncs.
+    (src/reference.py:40-41,107-112); off by default because it syncs. The
+    calls on a tracked or 4-bit cache also refuse shared pages, positions that
+    total_lens rules out, colliding moves and V scales past their range.
 """
 
 from __future__ import annotations

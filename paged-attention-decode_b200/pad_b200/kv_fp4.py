@@ -97,8 +97,9 @@ def paged_attention_decode_fp4(
     q [B, Hq, D] fp16 -> out [B, Hq, D] fp16; head_dim 32, 64 or 128, up to 16
     query heads per KV head. V's scales lie in 2^-24 .. 2^13 as the append
     writes them: a smaller one counts as 0, a larger one (not NaN) is flagged
-    (an error with PAD_B200_CHECK=1) and its sequence's output undefined. weights, num_new, slot_positions and total_lens
-    are those of paged_attention_decode_weights (weights=None: not tracked)."""
+    (an error with PAD_B200_CHECK=1) and its sequence's output undefined.
+    weights, num_new, slot_positions and total_lens are those of
+    paged_attention_decode_weights (weights=None: not tracked)."""
     assert q.is_cuda and k_cache.is_cuda and v_cache.is_cuda, "pad_b200 requires CUDA tensors"
     assert q.dtype == torch.float16 and q.dim() == 3, "pad_b200 expects fp16 q [B, Hq, D]"
     _, num_q_heads, head_dim = q.shape
