@@ -10,7 +10,8 @@ import torch
 import cache_oracle as co
 import pad_b200
 from gpu_utils import assert_parity
-from test_decode_weights import by_sequence, check_weights, rel_bound, smax_of
+from test_decode_weights import check_weights, rel_bound, smax_of
+from test_decode_weights import by_sequence
 
 gpu = pytest.mark.gpu
 

@@ -15,7 +15,8 @@ import pad_b200
 from gpu_utils import assert_parity
 from pad_b200 import _lib
 from pad_b200.cases import explicit_case
-from test_decode_weights import NEWS, by_sequence, check_weights, rel_bound, smax_of
+from test_decode_weights import check_weights, rel_bound, smax_of
+from test_decode_weights import NEWS, by_sequence
 
 gpu = pytest.mark.gpu
 
