@@ -43,13 +43,13 @@ def paged_attention_decode_weights(
     set, not added to, so a page's slots need no clearing before they are used
     (num_new = 0 only adds). num_new is one number for every sequence or an
     integer tensor [B], one of each: 1 for those that decode, the length of its
-    prompt for one that has just joined them. slot_positions [num_pages, Hkv, page_size] int32,
-    if given, gets the new tokens' positions, counted from total_lens [B] (the
-    tokens each sequence has seen; None: seq_lens, which is right before a first
-    eviction only, and refused later with PAD_B200_CHECK=1: the new tokens would
-    get positions that older ones have).
-    Sequences must not share pages (their weights would lose additions, other
-    ones from run to run; refused with PAD_B200_CHECK=1)."""
+    prompt for one that has just joined them (below 0 counts as 0).
+    slot_positions [num_pages, Hkv, page_size] int32, if given, gets the new
+    tokens' positions, counted from total_lens [B] (the tokens each sequence has
+    seen; None: seq_lens, which is right before a first eviction only, and refused
+    later with PAD_B200_CHECK=1: the new tokens would get positions that older
+    ones have). Sequences must not share pages (their weights would lose
+    additions, other ones from run to run; refused with PAD_B200_CHECK=1)."""
     assert q.is_cuda and k_cache.is_cuda and v_cache.is_cuda, "pad_b200 requires CUDA tensors"
     assert q.dtype == torch.float16 and k_cache.dtype == torch.float16 and v_cache.dtype == torch.float16, (
         "pad_b200 expects fp16 q/k_cache/v_cache"

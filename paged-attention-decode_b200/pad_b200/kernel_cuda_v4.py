@@ -167,9 +167,13 @@ def _check_positions(slot_positions: torch.Tensor, total_lens: torch.Tensor, blo
     if _live_pages(block_table, seq_lens, page_size) is None or pages == 0 or block_table.shape[1] == 0:
         return
     dev = slot_positions.device
+    new = num_new
+    if isinstance(num_new, torch.Tensor):
+        if num_new.shape != seq_lens.shape:
+            return  # (refused by the operator)
+        new = num_new.to(dev).long().clamp(min=0)[:, None]  # as the decode takes it
     slot = torch.arange(block_table.shape[1] * page_size, device=dev)[None, :]
     n, total = seq_lens.to(dev).long()[:, None], total_lens.to(dev).long()[:, None]
-    new = num_new.to(dev).long()[:, None] if isinstance(num_new, torch.Tensor) else num_new
     page = block_table.to(dev).long().repeat_interleave(page_size, 1)
     old = (slot < n - new) & (page >= 0) & (page < pages)
     at = slot_positions[page.clamp(0, pages - 1), :, slot % page_size]  # [B, slots, heads]

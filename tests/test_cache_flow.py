@@ -277,6 +277,10 @@ def test_lengths_left_out_after_an_eviction_are_refused_when_asked_for(fp4, monk
                                                  slot_positions=lp.at, **kw)
     decode(10 ** 6)
     decode(0)
+    decode(torch.tensor([-5, 0], device="cuda"))  # nothing new, and the slots behind the sequences are nobody's
+    for wrong in (torch.tensor(1, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")):
+        with pytest.raises(RuntimeError, match="num_new"):
+            decode(wrong)
     lp.append(lp.rand(2, lp.hkv, lp.d), lp.rand(2, lp.hkv, lp.d))
     decode(torch.tensor([1, 1], device="cuda"))
     lp.lens.copy_(evict())
